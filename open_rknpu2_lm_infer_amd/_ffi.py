@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import (POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int8, c_int32,
+from ctypes import (POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int8, c_int32, c_int64,
                     c_uint32, c_uint64, c_void_p)
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
@@ -42,6 +42,8 @@ RK_NPU_HIP_STATIC_MAX_ROWS = 256
 RK_NPU_ATTENTION_F16_CAUSAL = 0
 RK_NPU_ATTENTION_F16_NO_MASK = 1
 RK_NPU_ATTENTION_F16_STABLE_SOFTMAX = 1
+RK_NPU_HIP_KV_I8 = 0
+RK_NPU_HIP_KV_E4M3 = 1
 
 
 class rk_npu_domain_memory_stats(Structure):
@@ -179,6 +181,14 @@ class rk_npu_attention_f16_cache_info(Structure):
 class rk_npu_attention_f16_timings(Structure):
     _fields_ = [("upload_us", c_double), ("device_us", c_double), ("download_us", c_double),
                 ("total_us", c_double)]
+
+
+class rk_npu_hip_attention_q8_config(Structure):
+    _fields_ = [("attention", rk_npu_attention_f16_config), ("format", c_int32), ("block", c_int32)]
+
+
+class rk_npu_hip_heads(Structure):
+    _fields_ = [("data", c_void_p), ("type", c_int32), ("head_stride", c_int64), ("row_stride", c_int64)]
 
 
 P = POINTER
@@ -352,6 +362,27 @@ SIGNATURES = {
     "rk_npu_hip_attention_cache_append": (c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_void_p]),
     "rk_npu_hip_attention_run": (c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int32,
                                          c_void_p]),
+    "rk_npu_hip_attention_q8_config_init": (None, [P(rk_npu_hip_attention_q8_config)]),
+    "rk_npu_hip_attention_q8_query": (c_int, [P(rk_npu_hip_attention_q8_config), c_int32, c_int32,
+                                              P(rk_npu_attention_f16_sizes)]),
+    "rk_npu_hip_attention_q8_cache_create": (c_int, [c_void_p, P(rk_npu_hip_attention_q8_config), P(c_void_p)]),
+    "rk_npu_hip_attention_q8_cache_free": (None, [c_void_p]),
+    "rk_npu_hip_attention_q8_cache_reserve": (c_int, [c_void_p, c_void_p, c_int32]),
+    "rk_npu_hip_attention_q8_cache_truncate": (c_int, [c_void_p, c_int32]),
+    "rk_npu_hip_attention_q8_cache_get_info": (c_int, [c_void_p, P(rk_npu_attention_f16_cache_info)]),
+    "rk_npu_hip_attention_q8_cache_load": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32]),
+    "rk_npu_hip_attention_q8_cache_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32]),
+    "rk_npu_hip_attention_q8_cache_read": (c_int, [c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p]),
+    "rk_npu_hip_attention_q8_run": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p,
+                                            P(rk_npu_attention_f16_timings)]),
+    "rk_npu_hip_attention_q8_run_half": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p,
+                                                 P(rk_npu_attention_f16_timings)]),
+    "rk_npu_hip_attention_q8_device_append": (c_int, [c_void_p, P(rk_npu_hip_heads), P(rk_npu_hip_heads), c_int32,
+                                                      c_void_p]),
+    "rk_npu_hip_attention_q8_device_read": (c_int, [c_void_p, c_int32, c_int32, P(rk_npu_hip_heads),
+                                                    P(rk_npu_hip_heads), c_void_p]),
+    "rk_npu_hip_attention_q8_device_run": (c_int, [c_void_p, c_void_p, P(rk_npu_hip_heads), c_int32, c_int32,
+                                                   P(rk_npu_hip_heads), c_void_p]),
 }
 
 # Measurement-only library (libhip_probes.so, csrc/probes.hip): the roofline

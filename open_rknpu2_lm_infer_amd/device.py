@@ -116,6 +116,19 @@ class DeviceContext:
                                         L.rk_npu_matmul_workspace_free, "W8 workspace", self.shared)
         return self._ws[key]
 
+    def attention_workspace(self, cache: "KvCacheQ8") -> _Handle:
+        """The context's attention workspace for the cache's geometry, created on
+        first use (rk_npu_attention_f16_prepare)."""
+        c = cache.config.attention
+        key = ("attention", c.query_heads, c.kv_heads, c.head_dim, c.softmax_scale, c.mask_mode, c.max_query_rows)
+        if key not in self._ws:
+            raw = ctypes.c_void_p()
+            check(F.lib().rk_npu_attention_f16_prepare(self.domain, ctypes.byref(c), ctypes.byref(raw)),
+                  "prepare attention")
+            self._ws[key] = _Handle(raw.value, F.lib().rk_npu_attention_f16_workspace_free, "attention workspace",
+                                    self.shared)
+        return self._ws[key]
+
 
 class DeviceWeights:
     def __init__(self, handle: _Handle, bits: int, k: int, n: int):
@@ -143,6 +156,98 @@ def ffn(ctx: DeviceContext, gate_up: DeviceWeights, down: DeviceWeights, x, out,
                                     ctypes.c_void_p(x.data_ptr()), _dtype_code(x), ctypes.c_void_p(out.data_ptr()),
                                     _dtype_code(out), rows, stream if stream is not None else current_stream())
     check(rc, "device FFN")
+
+
+def _stream(stream, t):
+    """`stream`, or torch's current one on the tensor's GPU."""
+    import torch
+    return stream if stream is not None else ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+KV_FORMATS = {"i8": F.RK_NPU_HIP_KV_I8, "e4m3": F.RK_NPU_HIP_KV_E4M3}
+
+
+class KvCacheQ8:
+    """A KV cache of one sequence in 8 bits (rk_npu_attention_q8.h): fmt "i8" or
+    "e4m3", one scale for each `block` tokens (32, 64 or 128) and KV head, the
+    tokens after the last complete block in fp16. Holds up to `capacity` tokens,
+    allocated at once unless initial_capacity is smaller (append on the device
+    allocates nothing: reserve first).
+
+    Arrays are cuda tensors [heads][rows][head_dim], f16 or f32, any strides of
+    heads and rows (the transposed view of a token-major projection, say)."""
+
+    def __init__(self, ctx: DeviceContext, query_heads: int, kv_heads: int, head_dim: int, softmax_scale: float,
+                 capacity: int, fmt: str = "i8", block: int = 32, causal: bool = True, max_query_rows: int = 128,
+                 initial_capacity: Optional[int] = None):
+        ensure(fmt in KV_FORMATS, f"KV format must be one of {sorted(KV_FORMATS)}")
+        L = F.lib()
+        cfg = F.rk_npu_hip_attention_q8_config()
+        L.rk_npu_hip_attention_q8_config_init(ctypes.byref(cfg))
+        a = cfg.attention
+        a.query_heads, a.kv_heads, a.head_dim, a.softmax_scale = query_heads, kv_heads, head_dim, softmax_scale
+        a.max_query_rows, a.max_capacity = max_query_rows, capacity
+        a.initial_capacity = capacity if initial_capacity is None else initial_capacity
+        a.mask_mode = F.RK_NPU_ATTENTION_F16_CAUSAL if causal else F.RK_NPU_ATTENTION_F16_NO_MASK
+        cfg.format, cfg.block = KV_FORMATS[fmt], block
+        raw = ctypes.c_void_p()
+        check(L.rk_npu_hip_attention_q8_cache_create(ctx.domain, ctypes.byref(cfg), ctypes.byref(raw)),
+              "create the 8-bit KV cache")
+        self.handle = _Handle(raw.value, L.rk_npu_hip_attention_q8_cache_free, "8-bit KV cache", ctx.shared)
+        self.ctx, self.config = ctx, cfg
+
+    def info(self) -> F.rk_npu_attention_f16_cache_info:
+        info = F.rk_npu_attention_f16_cache_info()
+        check(F.lib().rk_npu_hip_attention_q8_cache_get_info(self.handle.raw, ctypes.byref(info)), "8-bit KV info")
+        return info
+
+    @property
+    def length(self) -> int:
+        return self.info().length
+
+    def bytes(self) -> int:
+        info = self.info()
+        return info.key_bytes + info.value_bytes + info.tail_bytes
+
+    def reserve(self, capacity: int) -> None:
+        check(F.lib().rk_npu_hip_attention_q8_cache_reserve(self.ctx.shared.ctx.raw, self.handle.raw, capacity),
+              "reserve the 8-bit KV cache")
+
+    def truncate(self, length: int) -> None:
+        """Keeps the first `length` tokens; exact within the open block and the last complete one."""
+        check(F.lib().rk_npu_hip_attention_q8_cache_truncate(self.handle.raw, length), "truncate the 8-bit KV cache")
+
+    def append(self, k, v, stream=None) -> None:
+        """Appends k and v, [kv_heads][rows][head_dim]."""
+        ensure(k.shape == v.shape, "k and v must have the same shape")
+        heads = [_heads(t, self.config.attention.kv_heads, self.config.attention.head_dim) for t in (k, v)]
+        check(F.lib().rk_npu_hip_attention_q8_device_append(self.handle.raw, ctypes.byref(heads[0]),
+                                                            ctypes.byref(heads[1]), k.shape[1], _stream(stream, k)),
+              "append to the 8-bit KV cache")
+
+    def read(self, first: int, k, v, stream=None) -> None:
+        """The values of tokens first.. into k and v, [kv_heads][rows][head_dim]."""
+        ensure(k.shape == v.shape, "k and v must have the same shape")
+        heads = [_heads(t, self.config.attention.kv_heads, self.config.attention.head_dim) for t in (k, v)]
+        check(F.lib().rk_npu_hip_attention_q8_device_read(self.handle.raw, first, k.shape[1], ctypes.byref(heads[0]),
+                                                          ctypes.byref(heads[1]), _stream(stream, k)),
+              "read the 8-bit KV cache")
+
+
+def _heads(t, heads: int, head_dim: int) -> F.rk_npu_hip_heads:
+    ensure(t.is_cuda and t.dim() == 3 and t.shape[0] == heads and t.shape[2] == head_dim and t.stride(2) == 1,
+           f"attention arrays are cuda [{heads}][rows][{head_dim}] tensors with contiguous rows")
+    return F.rk_npu_hip_heads(t.data_ptr(), _dtype_code(t), t.stride(0), t.stride(1))
+
+
+def attention_q8(ctx: DeviceContext, cache: KvCacheQ8, q, out, position: int, ws=None, stream=None):
+    """Attention of the rows q [query_heads][rows][head_dim], the first at `position`, over the cache's tokens."""
+    c = cache.config.attention
+    ensure(q.shape == out.shape, "q and out must have the same shape")
+    ws = ws or ctx.attention_workspace(cache)
+    qh, oh = _heads(q, c.query_heads, c.head_dim), _heads(out, c.query_heads, c.head_dim)
+    check(F.lib().rk_npu_hip_attention_q8_device_run(ws.raw, cache.handle.raw, ctypes.byref(qh), q.shape[1], position,
+                                                     ctypes.byref(oh), _stream(stream, q)), "8-bit KV attention")
 
 
 @contextlib.contextmanager

@@ -54,7 +54,7 @@ struct Q8WriteParams {
     __half* open_rows[2];       // where the new open block's rows go (nullptr: none)
     __half* last_rows[2];       // where the last complete block's rows are kept (nullptr: none completes)
     size_t head_bytes;
-    int blocks, fmt;
+    int blocks;
     int length, rows;  // before, and appended
 };
 
@@ -68,34 +68,61 @@ __device__ __forceinline__ float q8_value(unsigned code, int fmt) {
 __device__ __forceinline__ float q8_scale(const float4& s, int which) {
     return which ? ldexpf(s.y, __float_as_int(s.z)) : s.x;
 }
-// 4 quotients 127 x / a (448 x / a) to 4 stored codes.
-__device__ __forceinline__ unsigned q8_codes4(const float (&q)[4], int fmt) {
-    if (fmt == RK_NPU_HIP_KV_I8) {
-        unsigned w = 0;
+// A block's quantisation: quotients most x / a, correctly rounded, and 4 of them
+// as stored codes. The quotient: an approximation, then its exact remainder over a,
+// which with a correctly rounded 1 / a gives the nearest f32 (Markstein's
+// division). most x is exact (7 or 3 bits and fp16's 11), and a border of two codes
+// lies further from any quotient that is not on it than f32 rounds (both are
+// multiples of 1 / (2 a'), a' below 2^11, in the code's binade), so the codes are
+// the definition's. i8: adding 1.5 2^23 + 128 rounds half to even and leaves code
+// + 128 in the low byte.
+struct Q8Quantiser {
+    float a, inv, most;
+    bool poison;
+    template <int FMT>
+    __device__ __forceinline__ unsigned codes4(const _Float16 (&x)[4]) const {
+        float q[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w |= (unsigned)((int)rintf(q[i]) + 128) << (8 * i);
-        return w;
+        for (int i = 0; i < 4; ++i) {
+            const float t = (float)x[i] * most, q0 = t * inv;
+            q[i] = __builtin_fmaf(__builtin_fmaf(-q0, a, t), inv, q0);
+        }
+        if constexpr (FMT == RK_NPU_HIP_KV_I8) {
+            unsigned w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(q[i] + 12583040.0f);
+            const unsigned lo = __builtin_amdgcn_perm(w[1], w[0], 0x0C0C0400u);
+            const unsigned hi = __builtin_amdgcn_perm(w[3], w[2], 0x04000C0Cu);
+            return poison ? 0x80808080u : lo | hi;
+        } else {
+            const int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+            return poison ? 0u : (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
+        }
     }
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
-    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
-}
+};
 
-// Writes appended rows. Block: one token block of one KV head, K (blockIdx.z 0)
-// or V. Its rows meet in LDS as fp16, the old ones from the kept fp16 rows (or,
-// after a deep truncation, from the block's codes). A block that is complete is
-// quantised: a = max |x| as bits; 127 x and 448 x are exact in f32 (11 + 7 and
-// 11 + 3 bits) and the quotient by a, correctly rounded, falls on a border of two
-// codes only where the real one does (the borders are further from the other
-// quotients than its rounding), so the codes are the definition's.
-template <int D, int B>
-__global__ __launch_bounds__(256) void q8_write_kernel(Q8WriteParams P) {
-    constexpr int pitch = D + 8, pieces = D / 8;  // of a row in LDS, 8-value pieces of a row
-    __shared__ __attribute__((aligned(16))) __half rows[B * pitch];
-    __shared__ unsigned red[4];
+// Threads for a block of B x D values: 16 values each, within 256 and 1024.
+constexpr int q8_write_threads(int D, int B) { return B * D <= 4096 ? 256 : B * D >= 16384 ? 1024 : B * D / 16; }
+
+// Writes appended rows. Block: one token block of one KV head, K (blockIdx.z 0) or
+// V. Its rows come as fp16 into registers, every load before the first use, the old
+// ones from the kept rows (or, after a deep truncation, from the block's codes). An
+// open block's go straight to where they are kept. A complete block's meet in LDS,
+// where the largest magnitude is known after one barrier and V is read transposed
+// (ds_read_b64_tr_b16 hands lane l of 16 dim l of 4 keys).
+template <int D, int B, int FMT>
+__global__ __launch_bounds__(q8_write_threads(D, B)) void q8_write_kernel(Q8WriteParams P) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4 lds_s4;
+    constexpr int NT = q8_write_threads(D, B), PT = B * D / 8 / NT;  // 8-value pieces per thread
+    constexpr int pitch = D + 8, pieces = D / 8;                     // of a row in LDS, pieces of a row
+    __shared__ __attribute__((aligned(16))) _Float16 rows[B * pitch];
+    __shared__ unsigned red[NT / 64];
     const int which = blockIdx.z, g = blockIdx.y;
     const int b = P.length / B + blockIdx.x, tid = threadIdx.x;
     const int first = b * B, end = P.length + P.rows;
-    const int have = min(end - first, B);          // rows of the block after the call
+    const int have = min(end - first, B);  // rows of the block after the call
     const int old = max(0, min(P.length - first, B));
     const bool complete = have == B;
     const HeadsView src = which ? P.src[1] : P.src[0];
@@ -103,116 +130,158 @@ __global__ __launch_bounds__(256) void q8_write_kernel(Q8WriteParams P) {
     float4* sc = P.sc + (size_t)g * P.blocks + b;
     const __half* from = which ? P.old_rows[1] : P.old_rows[0];
     const size_t kept = (size_t)g * B * D;
-    const float old_scale = old && !from ? q8_scale(*sc, which) : 0.0f;
-
-    unsigned big = 0;
     // (rows that stay where they are need not be looked at in an open block)
     const int begin = complete || !from ? 0 : old;
-    for (int i = begin * pieces + tid; i < have * pieces; i += 256) {
-        const int j = i / pieces, d = i % pieces * 8, unit = j >> 5, ju = j & 31;
-        unsigned short h[8];
+
+    v4u raw[PT][2];
+#pragma unroll
+    for (int t = 0; t < PT; ++t) {
+        const int i = t * NT + tid, j = i / pieces, d = i % pieces * 8, unit = j >> 5, ju = j & 31;
+        raw[t][0] = raw[t][1] = v4u{0u, 0u, 0u, 0u};
+        if (j >= have || j < begin) continue;
         if (j >= old) {
             const long long at = g * src.head + (long long)(first + j - P.length) * src.row + d;
             if (src.f32) {
                 const float* p = static_cast<const float*>(src.data) + at;
-                const q8_f4a4 x = *reinterpret_cast<const q8_f4a4*>(p), y = *reinterpret_cast<const q8_f4a4*>(p + 4);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    h[k] = __half_as_ushort(__float2half_rn(x[k]));
-                    h[4 + k] = __half_as_ushort(__float2half_rn(y[k]));
-                }
+                raw[t][0] = __builtin_bit_cast(v4u, q8_f4(*reinterpret_cast<const q8_f4a4*>(p)));
+                raw[t][1] = __builtin_bit_cast(v4u, q8_f4(*reinterpret_cast<const q8_f4a4*>(p + 4)));
             } else {
-                const v4u x = v4u(*reinterpret_cast<const q8_u4a2*>(static_cast<const __half*>(src.data) + at));
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    h[2 * k] = (unsigned short)(x[k] & 0xFFFF);
-                    h[2 * k + 1] = (unsigned short)(x[k] >> 16);
-                }
+                raw[t][0] = v4u(*reinterpret_cast<const q8_u4a2*>(static_cast<const __half*>(src.data) + at));
             }
         } else if (from) {
             const __half* p = from + kept + (size_t)unit * 32 * D;
+            if (which == 0) {
+                raw[t][0] = *reinterpret_cast<const v4u*>(p + q8_kt_at(D, ju, d));
+            } else {
+                const unsigned short* u = reinterpret_cast<const unsigned short*>(p);
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                h[k] = __half_as_ushort(p[which ? q8_vt_at(ju, d + k) : q8_kt_at(D, ju, d + k)]);
+                for (int k = 0; k < 4; ++k)
+                    raw[t][0][k] = u[q8_vt_at(ju, d + 2 * k)] | ((unsigned)u[q8_vt_at(ju, d + 2 * k + 1)] << 16);
+            }
         } else {
             const uint8_t* p = codes + (size_t)unit * 32 * D;
+            const float s = q8_scale(*sc, which);
+            q8_h8 h;
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                h[k] = __half_as_ushort(__float2half_rn(
-                    q8_value(p[which ? q8_v_at(ju, d + k) : q8_k_at(D, ju, d + k)], P.fmt) * old_scale));
+                h[k] = (_Float16)(q8_value(p[which ? q8_v_at(ju, d + k) : q8_k_at(D, ju, d + k)], FMT) * s);
+            raw[t][0] = __builtin_bit_cast(v4u, h);
         }
-        v4u w;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = h[2 * k] | ((unsigned)h[2 * k + 1] << 16);
-        *reinterpret_cast<v4u*>(rows + j * pitch + d) = w;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) big = max(big, (unsigned)h[k] & 0x7FFFu);
     }
-    if (complete) {
+    unsigned big = 0;
 #pragma unroll
-        for (int i = 1; i < 64; i <<= 1) big = max(big, (unsigned)__shfl_xor((int)big, i));
-        if ((tid & 63) == 0) red[tid >> 6] = big;
+    for (int t = 0; t < PT; ++t) {
+        const int i = t * NT + tid, j = i / pieces, d = i % pieces * 8;
+        if (j >= have || j < begin) continue;
+        if (src.f32 && j >= old) {
+            const q8_f4 x = __builtin_bit_cast(q8_f4, raw[t][0]), y = __builtin_bit_cast(q8_f4, raw[t][1]);
+            q8_h8 h;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                h[k] = (_Float16)x[k];
+                h[4 + k] = (_Float16)y[k];
+            }
+            raw[t][0] = __builtin_bit_cast(v4u, h);
+        }
+        if (complete) {
+            *reinterpret_cast<v4u*>(rows + j * pitch + d) = raw[t][0];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                big = max(big, max(raw[t][0][k] & 0x7FFFu, (raw[t][0][k] >> 16) & 0x7FFFu));
+        } else {
+            __half* p = (which ? P.open_rows[1] : P.open_rows[0]) + kept + (size_t)(j >> 5) * 32 * D;
+            if (which == 0) {
+                *reinterpret_cast<v4u*>(p + q8_kt_at(D, j & 31, d)) = raw[t][0];
+            } else {
+                unsigned short* u = reinterpret_cast<unsigned short*>(p);
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    u[q8_vt_at(j & 31, d + k)] = (unsigned short)(raw[t][0][k >> 1] >> (16 * (k & 1)));
+            }
+        }
     }
+    if (!complete) return;  // (block-uniform)
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) big = max(big, (unsigned)__shfl_xor((int)big, i));
+    if ((tid & 63) == 0) red[tid >> 6] = big;
     __syncthreads();
-
-    // the fp16 rows that are kept: the open block's new ones, or all of the last
-    // complete block's
-    __half* keep = complete ? (which ? P.last_rows[1] : P.last_rows[0]) : (which ? P.open_rows[1] : P.open_rows[0]);
-    if (complete && (first + 2 * B <= end)) keep = nullptr;  // (a later block is complete too)
-    if (keep) {
-        keep += kept;
-        for (int i = begin * pieces + tid; i < have * pieces; i += 256) {
-            const int j = i / pieces, d = i % pieces * 8, ju = j & 31;
-            __half* p = keep + (size_t)(j >> 5) * 32 * D;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) p[which ? q8_vt_at(ju, d + k) : q8_kt_at(D, ju, d + k)] = rows[j * pitch + d + k];
-        }
-    }
-    if (!complete) return;
+    for (int i = 0; i < NT / 64; ++i) big = max(big, red[i]);
 
-    big = max(max(red[0], red[1]), max(red[2], red[3]));
-    const float a = __half2float(__ushort_as_half((unsigned short)big)), most = P.fmt == RK_NPU_HIP_KV_I8 ? 127.0f : 448.0f;
-    const bool poison = big >= 0x7C00u, zero = big == 0;
+    Q8Quantiser Q;
+    Q.most = FMT == RK_NPU_HIP_KV_I8 ? 127.0f : 448.0f;
+    Q.poison = big >= 0x7C00u;
+    const float a = __half2float(__ushort_as_half((unsigned short)big));
+    Q.a = Q.poison || big == 0 ? 1.0f : a;
+    Q.inv = 1.0f / Q.a;
     if (tid == 0) {
-        const float s = poison ? NAN : zero ? 1.0f : a / most;
+        const float s = Q.poison ? NAN : big == 0 ? 1.0f : a / Q.most;
         if (which == 0) {
             sc->x = s;
         } else {
             // (a / most is a normal number: a >= 2^-24)
-            const int bits = __float_as_int(s), e = poison ? 0 : ((bits >> 23) & 255) - 127;
-            sc->y = poison ? NAN : __int_as_float((bits & 0x7FFFFF) | 0x3F800000);
+            const int bits = __float_as_int(s), e = Q.poison ? 0 : ((bits >> 23) & 255) - 127;
+            sc->y = Q.poison ? NAN : __int_as_float((bits & 0x7FFFFF) | 0x3F800000);
             sc->z = __int_as_float(e);
             sc->w = 1.0f / s;
         }
     }
-    const float div = poison || zero ? 1.0f : a;
-    auto quotient = [&](__half x) { return poison ? 0.0f : __half2float(x) * most / div; };
-    // 16-byte pieces of the codes, in the order they lie in
-    constexpr int unit_pieces = 2 * D;  // of 32 D bytes
-    for (int i = tid; i < (B >> 5) * unit_pieces; i += 256) {
-        const int unit = i / unit_pieces, p = i % unit_pieces, lane = p & 63, lo = lane & 15, hi = lane >> 4;
-        unsigned w[4];
+    // lane (lo, hi)'s dim 16 n + lo of keys 4 hi..+3 of 16 keys from row j0
+    const int lane = tid & 63, lo = lane & 15, hi = lane >> 4;
+    auto transposed = [&](int j0, int n) {
+        const _Float16* p = rows + (j0 + 4 * hi + (lo >> 2)) * pitch + 16 * n + 4 * (lo & 3);
+        return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p));
+    };
+    // the last complete block's fp16 rows are kept too
+    __half* keep = which ? P.last_rows[1] : P.last_rows[0];
+    if (keep && first + 2 * B > end) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int quad = 0; quad < 2; ++quad) {
-                float q[4];
+        for (int t = 0; t < PT; ++t) {
+            const int i = t * NT + tid, unit = i / (4 * D), step = (i >> 6) % (D / 16);
+            q8_h8 h;
+            if (which == 0) {
+                const int at = step % (D / 32) * 32 + 8 * hi, j = unit * 32 + step / (D / 32) * 16 + lo;
+                h = *reinterpret_cast<const q8_h8*>(rows + j * pitch + at);
+            } else {
+                const h4 x = transposed(unit * 32, step), y = transposed(unit * 32 + 16, step);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    int j, d;
-                    if (which == 0) {
-                        const int step = p >> 6;  // [16-key half][64-dim step]
-                        j = step / (D >> 6) * 16 + lo;
-                        d = step % (D >> 6) * 64 + 32 * half + 8 * hi + 4 * quad + k;
-                    } else {
-                        j = 16 * quad + 4 * hi + k;
-                        d = (p >> 6) * 32 + 16 * half + lo;
-                    }
-                    q[k] = quotient(rows[(unit * 32 + j) * pitch + d]);
+                    h[k] = x[k];
+                    h[4 + k] = y[k];
                 }
-                w[2 * half + quad] = q8_codes4(q, P.fmt);
             }
-        *reinterpret_cast<v4u*>(codes + (size_t)i * 16) = v4u{w[0], w[1], w[2], w[3]};
+            *reinterpret_cast<q8_h8*>(keep + kept + (size_t)i * 8) = h;
+        }
+    }
+    // the codes, in the order they lie in
+#pragma unroll
+    for (int t = 0; t < (PT + 1) / 2; ++t) {
+        const int i = t * NT + tid, unit = i / (2 * D), step = (i >> 6) % (D / 32);
+        if (PT == 1 && i >= B * D / 16) break;  // (whole waves)
+        v4u w;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            _Float16 x[4], y[4];
+            if (which == 0) {  // step: [16-key half][64-dim step]
+                const int at = step % (D / 64) * 64 + 32 * half + 8 * hi, j = unit * 32 + step / (D / 64) * 16 + lo;
+                const q8_h8 h = *reinterpret_cast<const q8_h8*>(rows + j * pitch + at);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    x[k] = h[k];
+                    y[k] = h[4 + k];
+                }
+            } else {
+                const h4 h0 = transposed(unit * 32, 2 * step + half), h1 = transposed(unit * 32 + 16, 2 * step + half);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    x[k] = h0[k];
+                    y[k] = h1[k];
+                }
+            }
+            w[2 * half] = Q.template codes4<FMT>(x);
+            w[2 * half + 1] = Q.template codes4<FMT>(y);
+        }
+        *reinterpret_cast<v4u*>(codes + (size_t)i * 16) = w;
     }
 }
 
@@ -482,14 +551,23 @@ static HeadsView view_of(const rk_npu_hip_heads& a) {
     return HeadsView{a.data, a.type == RK_NPU_HIP_F32 ? 1 : 0, (long long)a.head_stride, (long long)a.row_stride};
 }
 
-template <int D>
+template <int D, int FMT>
 static void q8_launch_write(const Q8WriteParams& P, int B, const dim3& grid, hipStream_t s) {
     if (B == 32)
-        hipLaunchKernelGGL((q8_write_kernel<D, 32>), grid, dim3(256), 0, s, P);
+        hipLaunchKernelGGL((q8_write_kernel<D, 32, FMT>), grid, dim3(q8_write_threads(D, 32)), 0, s, P);
     else if (B == 64)
-        hipLaunchKernelGGL((q8_write_kernel<D, 64>), grid, dim3(256), 0, s, P);
+        hipLaunchKernelGGL((q8_write_kernel<D, 64, FMT>), grid, dim3(q8_write_threads(D, 64)), 0, s, P);
     else
-        hipLaunchKernelGGL((q8_write_kernel<D, 128>), grid, dim3(256), 0, s, P);
+        hipLaunchKernelGGL((q8_write_kernel<D, 128, FMT>), grid, dim3(q8_write_threads(D, 128)), 0, s, P);
+}
+template <int FMT>
+static void q8_launch_write(const Q8WriteParams& P, int D, int B, const dim3& grid, hipStream_t s) {
+    if (D == 64)
+        q8_launch_write<64, FMT>(P, B, grid, s);
+    else if (D == 128)
+        q8_launch_write<128, FMT>(P, B, grid, s);
+    else
+        q8_launch_write<256, FMT>(P, B, grid, s);
 }
 
 // Enqueues an append (room and views checked) and advances the bookkeeping.
@@ -508,17 +586,14 @@ static int q8_enqueue_append(Q8Cache* c, const HeadsView& k, const HeadsView& v,
     P.sc = c->sc;
     P.head_bytes = (size_t)c->capacity * D;
     P.blocks = c->capacity / B;
-    P.fmt = c->cfg.format;
     P.length = c->rows.length;
     P.rows = n;
     const int blocks = (c->rows.length + n - 1) / B - c->rows.length / B + 1;
     const dim3 grid(blocks, c->cfg.attention.kv_heads, 2);
-    if (D == 64)
-        q8_launch_write<64>(P, B, grid, s);
-    else if (D == 128)
-        q8_launch_write<128>(P, B, grid, s);
+    if (c->cfg.format == RK_NPU_HIP_KV_I8)
+        q8_launch_write<RK_NPU_HIP_KV_I8>(P, D, B, grid, s);
     else
-        q8_launch_write<256>(P, B, grid, s);
+        q8_launch_write<RK_NPU_HIP_KV_E4M3>(P, D, B, grid, s);
     if (hipGetLastError() != hipSuccess) return RK_NPU_ERR_DEVICE;
     c->rows = st.after;
     return RK_NPU_OK;

@@ -16,12 +16,13 @@ _DT = {}
 
 
 def _dtype_code(t) -> int:
-    import torch
-    if t.dtype == torch.float32:
-        return F.RK_NPU_HIP_F32
-    if t.dtype == torch.float16:
-        return F.RK_NPU_HIP_F16
-    raise NpuError(f"unsupported activation dtype {t.dtype}")
+    if not _DT:
+        import torch
+        _DT.update({torch.float32: F.RK_NPU_HIP_F32, torch.float16: F.RK_NPU_HIP_F16})
+    code = _DT.get(t.dtype)
+    if code is None:
+        raise NpuError(f"unsupported activation dtype {t.dtype}")
+    return code
 
 
 def current_stream():
@@ -159,9 +160,10 @@ def ffn(ctx: DeviceContext, gate_up: DeviceWeights, down: DeviceWeights, x, out,
 
 
 def _stream(stream, t):
-    """`stream`, or torch's current one on the tensor's GPU."""
+    """`stream`, or torch's current one on the tensor's GPU (as a number: a Stream
+    object takes 2 us to make, a third of a call that reads a short cache)."""
     import torch
-    return stream if stream is not None else ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+    return stream if stream is not None else torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 KV_FORMATS = {"i8": F.RK_NPU_HIP_KV_I8, "e4m3": F.RK_NPU_HIP_KV_E4M3}
@@ -235,9 +237,10 @@ class KvCacheQ8:
 
 
 def _heads(t, heads: int, head_dim: int) -> F.rk_npu_hip_heads:
-    ensure(t.is_cuda and t.dim() == 3 and t.shape[0] == heads and t.shape[2] == head_dim and t.stride(2) == 1,
-           f"attention arrays are cuda [{heads}][rows][{head_dim}] tensors with contiguous rows")
-    return F.rk_npu_hip_heads(t.data_ptr(), _dtype_code(t), t.stride(0), t.stride(1))
+    shape, stride = t.shape, t.stride()
+    if not (t.is_cuda and len(shape) == 3 and shape[0] == heads and shape[2] == head_dim and stride[2] == 1):
+        raise NpuError(f"attention arrays are cuda [{heads}][rows][{head_dim}] tensors with contiguous rows")
+    return F.rk_npu_hip_heads(t.data_ptr(), _dtype_code(t), stride[0], stride[1])
 
 
 def attention_q8(ctx: DeviceContext, cache: KvCacheQ8, q, out, position: int, ws=None, stream=None):

@@ -628,8 +628,48 @@ static int q8_enqueue_read(Q8Cache* c, int first, int n, const HeadsView& k, con
     return hipGetLastError() == hipSuccess ? RK_NPU_OK : RK_NPU_ERR_DEVICE;
 }
 
-// Splits: enough that about 512 blocks run, at most what the workspace's partials
-// hold.
+// Rows a block: one when there are many splits or few rows, else as many as leave a
+// row the threads for its dims.
+template <int D>
+static void q8_combine(const AttnQ8Params& P, int R, hipStream_t s) {
+    constexpr int MANY = D == 256 ? 4 : 8;
+    if (P.splits > 16 || R * P.kh < 512)
+        hipLaunchKernelGGL((attn_q8_combine_kernel<D, 1>), dim3(R, P.kh), dim3(256), 0, s, P);
+    else
+        hipLaunchKernelGGL((attn_q8_combine_kernel<D, MANY>), dim3((R + MANY - 1) / MANY, P.kh), dim3(256), 0, s, P);
+}
+
+// The kernel, for R query rows of each KV head: attn_q8_kernel converts a unit's codes
+// in every wave, attn_q8_tile_kernel once a block, which takes rows enough to fill
+// 128- or 256-row blocks and keys enough to fill its stages. Measured, us, either:
+//   head_dim 128, 8 KV heads, f16 output: 512 rows x 8000 keys 34.1 and 45.1, x 16000
+//   56.4 and 56.4, x 32000 98.6 and 89.9; 1024 x 8000 50.0 and 56.2, x 16000 88.7 and
+//   85.9; f32 output 512 x 16000 69.8 and 68.9, 1024 x 8000 63.9 and 67.5;
+//   head_dim 64, 8 KV heads, 512 x 32000: 58.4 and 59.8, f32 80.4 and 76.1;
+//   head_dim 256, 2 KV heads: 1024 x 8000 37.1 and 38.1, x 16000 65.4 and 55.9.
+// They cross near 24 million rows x keys x dims a CU.
+static bool q8_tile(int D, int R, int kv_heads, int units) {
+    const int forced = attention_q8_tile_switch();
+    return forced >= 0 ? forced != 0 : (double)D * R * kv_heads * units * 32 > 24e6 * device_cus();
+}
+
+// Key splits: blocks enough for the CUs, but no more, as a block's rows leave
+// partials: 256 blocks of many rows (512 rows of 8 heads over 4096 keys 21.9 us, 27.6
+// with 512), 128 where a KV head has at most 32, whose blocks are 8 waves that only
+// load (8 rows of 8 heads of 256 over 16001 keys 19.3 us, 20.6 with 256 and 28.2 with
+// 512). A split holds at least a unit for each wave, or two stages.
+static void q8_splits(AttnQ8Params& P, int D, int R, bool tile) {
+    const int rows = q8_block_rows(D, R, tile);
+    P.row_tiles = (R + rows - 1) / rows;
+    P.rows_pad = P.row_tiles * rows;
+    const int base = P.row_tiles * P.kh, least = tile ? 4 : Q8_WAVES, blocks = R > 32 ? 256 : 128;
+    const size_t room = attn_partial_rows(D) / ((size_t)P.rows_pad * P.kh);
+    int want = std::max(1, std::min((blocks + base - 1) / base, (P.units + least - 1) / least));
+    want = (int)std::min<size_t>(want, std::max<size_t>(1, room));
+    P.units_per_split = ((P.units + want - 1) / want + least - 1) / least * least;
+    P.splits = (P.units + P.units_per_split - 1) / P.units_per_split;
+}
+
 static int q8_enqueue_run(AttnWork* w, Q8Cache* c, const HeadsView& q, int rows, int pos, const HeadsView& out,
                           hipStream_t s) {
     const rk_npu_attention_f16_config& cfg = c->cfg.attention;
@@ -665,24 +705,17 @@ static int q8_enqueue_run(AttnWork* w, Q8Cache* c, const HeadsView& q, int rows,
     P.block_values = B * D;
     P.coded = c->rows.coded;
     P.units = ((causal ? std::min(len, pos + rows) : len) + 31) / 32;
-    const int R = cfg.query_heads / cfg.kv_heads * rows, groups = q8_row_groups(D, R), rt = 16 * groups;
-    P.row_tiles = (R + rt - 1) / rt;
-    P.rows_pad = P.row_tiles * rt;
-    const int base = P.row_tiles * cfg.kv_heads;
-    // (a split holds at least a unit for each of the 4 waves)
-    int want = std::max(1, std::min((512 + base - 1) / base, (P.units + 3) / 4));
-    want = std::min<size_t>(want, std::max<size_t>(1, attn_partial_rows(D) / ((size_t)P.rows_pad * cfg.kv_heads)));
-    P.units_per_split = ((P.units + want - 1) / want + 3) / 4 * 4;
-    P.splits = (P.units + P.units_per_split - 1) / P.units_per_split;
-    (c->cfg.format == RK_NPU_HIP_KV_I8 ? launch_attn_q8_i8 : launch_attn_q8_e4m3)(P, D, groups, !P.out_f16, s);
+    const int R = cfg.query_heads / cfg.kv_heads * rows;
+    const bool tile = q8_tile(D, R, cfg.kv_heads, P.units);
+    q8_splits(P, D, R, tile);
+    (c->cfg.format == RK_NPU_HIP_KV_I8 ? launch_attn_q8_i8 : launch_attn_q8_e4m3)(P, D, R, tile, !P.out_f16, s);
     if (P.splits > 1) {
-        const dim3 grid((R + 3) / 4, cfg.kv_heads);
         if (D == 64)
-            hipLaunchKernelGGL(attn_q8_combine_kernel<64>, grid, dim3(256), 0, s, P);
+            q8_combine<64>(P, R, s);
         else if (D == 128)
-            hipLaunchKernelGGL(attn_q8_combine_kernel<128>, grid, dim3(256), 0, s, P);
+            q8_combine<128>(P, R, s);
         else
-            hipLaunchKernelGGL(attn_q8_combine_kernel<256>, grid, dim3(256), 0, s, P);
+            q8_combine<256>(P, R, s);
     }
     return hipGetLastError() == hipSuccess ? RK_NPU_OK : RK_NPU_ERR_DEVICE;
 }

@@ -88,31 +88,26 @@ __device__ __forceinline__ q8_h2 q8_round2(float a, float b) {
     return __builtin_bit_cast(q8_h2, w);
 }
 
-// Max / sum over the 4 lanes of a query row (l % 16 + 16 j), in each of them.
+// Max / sum over the 4 lanes of a query row (l % 16 + 16 j), in each of them: the
+// swaps exchange odd with even 16-lane rows, then the wave's halves.
 __device__ __forceinline__ float q8_rows4_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float q8_rows4_sum(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
-
-// 8 consecutive q values of any alignment, as fp16.
-__device__ __forceinline__ q8_h8 q8_load_q(const AttnQ8Params& P, long long at) {
-    typedef unsigned u16 __attribute__((ext_vector_type(4), aligned(2)));
-    typedef float f16 __attribute__((ext_vector_type(4), aligned(4)));
-    if (!P.q_f32)
-        return __builtin_bit_cast(q8_h8, v4u(*reinterpret_cast<const u16*>(static_cast<const __half*>(P.q) + at)));
-    const float* p = static_cast<const float*>(P.q) + at;
-    const f16 a = *reinterpret_cast<const f16*>(p), b = *reinterpret_cast<const f16*>(p + 4);
-    q8_h8 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        r[i] = (_Float16)a[i];
-        r[4 + i] = (_Float16)b[i];
-    }
-    return r;
+// Min over each 16 lanes, in each of them.
+__device__ __forceinline__ int q8_row_min(int v) {
+    v = min(v, dpp_move<DPP_QUAD_XOR1>(v));
+    v = min(v, dpp_move<DPP_QUAD_XOR2>(v));
+    v = min(v, dpp_move<DPP_ROW_HALF_MIRROR>(v));
+    return min(v, dpp_move<DPP_ROW_MIRROR>(v));
 }
 
 // 4 consecutive outputs of any alignment.
@@ -129,21 +124,21 @@ __device__ __forceinline__ void q8_store4(const AttnQ8Params& P, long long at, q
     }
 }
 
+// A row's maximum before it has seen a key: finite, so that differences are no NaN.
+constexpr float Q8_NONE = -1e30f;
 // The weight 2^d of a partial result whose maximum lies d <= 0 below the row's:
 // never 0, so that an infinite accumulator stays one (0 times it is NaN). What a
 // finite one gains by that is below 2^-100 of the result.
 __device__ __forceinline__ float q8_weight(float m, float top) {
-    return m == -INFINITY ? 0.0f : fmaxf(__builtin_amdgcn_exp2f(m - top), 0x1p-120f);
+    return fmaxf(__builtin_amdgcn_exp2f(m - top), 0x1p-120f);
 }
 
 constexpr float Q8_LAZY = 8.0f;   // a row's maximum moves when a score passes it by this much (powers of 2)
 constexpr float Q8_SHIFT = 6.0f;  // SPLIT: the weights lie this much higher (p below 2^14, p mu below 2^15)
 
-// Attention over codes and tail. Block: 4 waves over one tile of 16 RW query
-// rows of one KV head; wave w takes units w, w + 4, .. of its split, so nothing
-// is shared until the waves' partial (max, sum, accumulators) meet in LDS. A
-// unit's codes go from memory into operand registers; the loads of the next
-// unit are issued as soon as this one's are converted.
+// A wave's query rows, RW groups of 16 (lane l: row l % 16 of each): their key
+// limits, queries, running maxima (less SHIFT), sums and accumulators (lane l:
+// dims 16 n + 4 (l / 16)..+3).
 //
 // With c = scale log2(e) and a block's scales ks and vs = mu 2^e, a key's weight
 // is kept as p = 2^(c ks s + e - m): e in the exponent keeps the products p mu
@@ -152,247 +147,242 @@ constexpr float Q8_SHIFT = 6.0f;  // SPLIT: the weights lie this much higher (p 
 // maximum, a whole number with SPLIT so that e - m is exact.
 //
 // SPLIT (f32 output): p mu goes into the products as two fp16, 22 bits.
-// Otherwise (fp16 output) as one, and the sum adds the rounded weights (p mu
-// times 1 / vs), so that a row whose weight is all on one key is not off.
-//
-// `poison`: a NaN scale makes every score of its block NaN, before the mask.
-template <int D, int RW, int FMT, bool SPLIT>
-__global__ __launch_bounds__(256) void attn_q8_kernel(AttnQ8Params P) {
-    constexpr int KS = D / 32, NB = D / 16, KP = D / 32;  // KP: 16-byte pieces per lane, of K (and V)
-    constexpr int RT = 16 * RW;
-    constexpr float SHIFT = SPLIT ? Q8_SHIFT : 0.0f;
-    __shared__ __attribute__((aligned(16))) float merge[3 * NB * 256];
-    __shared__ float merge_ml[3][2][64];
-    const int split = blockIdx.x, rt = blockIdx.y, g = blockIdx.z;
-    const int G = P.qh / P.kh, R = G * P.m;
-    const int lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const float c = fminf(P.scale * 1.4426950408889634f, 0x1.fffffep127f);
-    const uint8_t* kbase = P.k + (size_t)g * P.head_bytes + lane * 16;
-    const uint8_t* vbase = P.v + (size_t)g * P.head_bytes + lane * 16;
-    const float4* sc = P.sc + (size_t)g * P.blocks;
-    const int coded_units = P.coded >> 5;
-
-    // this lane's query rows: their key limits and fragments
+// Otherwise (fp16 output) as one, and the sum adds the rounded weights (times
+// 1 / vs), so that a row whose weight is all on one key is not off.
+template <int D, int RW, bool SPLIT>
+struct Q8Wave {
+    static constexpr int KS = D / 32, NB = D / 16;
+    static constexpr float SHIFT = SPLIT ? Q8_SHIFT : 0.0f;
     int lim[RW];
+    int open, seen;  // keys below `open` every row sees, from `seen` on none
     q8_h8 qf[RW][KS];
-    int open = 0x7fffffff, seen = 0;  // keys below `open` every row sees, from `seen` on none
-#pragma unroll
-    for (int w = 0; w < RW; ++w) {
-        const int rr = rt * RT + 16 * w + lo;
-        const bool ok = rr < R;
-        const int h = g * G + (ok ? rr / P.m : 0), r = ok ? rr % P.m : 0;
-        lim[w] = ok ? (P.causal ? min(P.len, P.pos + r + 1) : P.len) : 0;
-        if (ok) {
-            open = min(open, lim[w]);
-            seen = max(seen, lim[w]);
-        }
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            qf[w][s] = q8_load_q(P, h * P.q_head + r * P.q_row + 32 * s + 8 * hi);
-            if (!ok) qf[w][s] = q8_h8{};
-        }
-    }
-#pragma unroll
-    for (int i = 1; i < 16; i <<= 1) {
-        open = min(open, __shfl_xor(open, i));
-        seen = max(seen, __shfl_xor(seen, i));
-    }
-    open = __builtin_amdgcn_readfirstlane(open);
-    seen = __builtin_amdgcn_readfirstlane(seen);
-    const int u_end = min(min((split + 1) * P.units_per_split, P.units), (seen + 31) >> 5);
-    const int u_begin = split * P.units_per_split + wave;
-
+    float mrun[RW], lsum[RW];
     q8_f4 o[RW][NB];
-    float mrun[RW], lsum[RW];  // (mrun: the row's maximum less SHIFT)
-#pragma unroll
-    for (int w = 0; w < RW; ++w) {
-        mrun[w] = -INFINITY;
-        lsum[w] = 0.0f;
-#pragma unroll
-        for (int n = 0; n < NB; ++n) o[w][n] = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
 
-    v4u kr[KP], vr[KP];
-    // (the last coded unit's own codes again where there is no further one)
-    auto load_k = [&](int u) {
-        const uint8_t* p = kbase + (size_t)min(u, coded_units - 1) * (32 * D);
+    // Rows r0 + 16 w + lane % 16 of KV head g. Rows from R on are computed as the
+    // head's first row and not written. Every load of the queries comes before the
+    // first use (one memory round trip).
+    __device__ __forceinline__ void start(const AttnQ8Params& P, int g, int r0, int lo, int hi) {
+        typedef unsigned u16 __attribute__((ext_vector_type(4), aligned(2)));
+        typedef float f16 __attribute__((ext_vector_type(4), aligned(4)));
+        const int G = P.qh / P.kh, R = G * P.m;
+        open = 0x7fffffff;
+        seen = 0;
+        long long at[RW];
 #pragma unroll
-        for (int i = 0; i < KP; ++i) kr[i] = *reinterpret_cast<const v4u*>(p + i * 1024);
-    };
-    auto load_v = [&](int u) {
-        const uint8_t* p = vbase + (size_t)min(u, coded_units - 1) * (32 * D);
+        for (int w = 0; w < RW; ++w) {
+            const int rr = r0 + 16 * w + lo;
+            const bool ok = rr < R;
+            const int h = ok ? rr / P.m : 0, r = ok ? rr - h * P.m : 0;
+            at[w] = (long long)(g * G + h) * P.q_head + r * P.q_row + 8 * hi;
+            lim[w] = ok ? (P.causal ? min(P.len, P.pos + r + 1) : P.len) : 0;
+            if (ok) {
+                open = min(open, lim[w]);
+                seen = max(seen, lim[w]);
+            }
+            mrun[w] = Q8_NONE;
+            lsum[w] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < KP; ++i) vr[i] = *reinterpret_cast<const v4u*>(p + i * 1024);
-    };
-    if (u_begin < u_end && coded_units > 0) {
-        load_k(u_begin);
-        load_v(u_begin);
-    }
-    // A unit's scores to weights: s in, ph (and pl) out, the row's sum and, when
-    // its maximum moves, its accumulators updated. `mu` 2^e: V's scale; `inv`: one
-    // over it.
-    auto weigh = [&](int key0, float ks, float mu, float inv, int e, q8_f4 (&s)[RW][2], q8_h8 (&ph)[RW],
-                     q8_h8 (&pl)[RW]) {
-        const bool poison = ks != ks || mu != mu;  // (uniform)
-        const float ef = (float)e, down = __int_as_float((127 - e) << 23);  // 2^-e
-        const float cks = fmaxf(c * ks, 0x1p-120f);
-        if (__builtin_expect(poison, 0)) {
-            mu = inv = 1.0f;
+            for (int n = 0; n < NB; ++n) o[w][n] = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        if (!P.q_f32) {
 #pragma unroll
             for (int w = 0; w < RW; ++w)
 #pragma unroll
-                for (int cb = 0; cb < 2; ++cb) s[w][cb] = q8_f4{NAN, NAN, NAN, NAN};
+                for (int s = 0; s < KS; ++s)
+                    qf[w][s] = __builtin_bit_cast(
+                        q8_h8, v4u(*reinterpret_cast<const u16*>(static_cast<const __half*>(P.q) + at[w] + 32 * s)));
+        } else {
+#pragma unroll
+            for (int w = 0; w < RW; ++w) {
+                f16 x[KS][2];
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        x[s][i] = *reinterpret_cast<const f16*>(static_cast<const float*>(P.q) + at[w] + 32 * s + 4 * i);
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) qf[w][s][i] = (_Float16)x[s][i >> 2][i & 3];
+            }
         }
+        open = __builtin_amdgcn_readfirstlane(q8_row_min(open));
+        seen = -__builtin_amdgcn_readfirstlane(q8_row_min(-seen));
+    }
+
+    // What a unit's weights take from its scales. Without SPLIT, e + log2(mu) goes
+    // into the exponent whole: what its rounding takes is far below fp16's. A NaN
+    // scale (poison) makes cks NaN, so every weight of the block is.
+    struct Unit {
+        float cks, lg, mu, part;  // part: what a weight's sum is multiplied with
+    };
+    static __device__ __forceinline__ Unit unit(float c, float ks, float mu, int e, float inv) {
+        const bool poison = ks != ks || mu != mu;
+        Unit x;
+        x.cks = poison ? NAN : fmaxf(c * ks, 0x1p-120f);
+        x.mu = poison ? 1.0f : mu;
+        x.lg = SPLIT ? (float)e : (float)e + __builtin_amdgcn_logf(x.mu);
+        x.part = SPLIT ? __int_as_float((127 - e) << 23) : poison ? 1.0f : inv;  // 2^-e, 1 / (mu 2^e)
+        return x;
+    }
+    // Masked scores become -inf; where there are some, those of a poisoned block
+    // become NaN here. (`none`: every key is)
+    __device__ __forceinline__ bool masked(int key0, bool none) const { return key0 + 32 > open || none; }
+    __device__ __forceinline__ void mask(Unit& x, int key0, bool none, int hi, q8_f4 (&s)[RW][2]) const {
+        const bool poison = x.cks != x.cks;
+        x.cks = poison ? 1.0f : x.cks;
+#pragma unroll
+        for (int w = 0; w < RW; ++w)
+#pragma unroll
+            for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float y = poison ? NAN : s[w][cb][r];
+                    s[w][cb][r] = none || key0 + 16 * cb + 4 * hi + r >= lim[w] ? -INFINITY : y;
+                }
+    }
+    // The rows' largest scores of a unit, in the maxima's units, and whether one
+    // passes its row's maximum by more than Q8_LAZY.
+    __device__ __forceinline__ bool over(const Unit& x, const q8_f4 (&s)[RW][2], float (&top)[RW]) const {
+        bool any = false;
 #pragma unroll
         for (int w = 0; w < RW; ++w) {
-            if (__builtin_expect(key0 + 32 > open, 0)) {  // (uniform) the unit crosses a mask
-#pragma unroll
-                for (int cb = 0; cb < 2; ++cb)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (key0 + 16 * cb + 4 * hi + r >= lim[w]) s[w][cb][r] = -INFINITY;
-            }
-            float top = __builtin_elementwise_maximum(
+            top[w] = __builtin_elementwise_maximum(
                 __builtin_elementwise_maximum(__builtin_elementwise_maximum(s[w][0][0], s[w][0][1]),
                                               __builtin_elementwise_maximum(s[w][0][2], s[w][0][3])),
                 __builtin_elementwise_maximum(__builtin_elementwise_maximum(s[w][1][0], s[w][1][1]),
                                               __builtin_elementwise_maximum(s[w][1][2], s[w][1][3])));
-            top = __builtin_fmaf(top, cks, ef);
-            if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > mrun[w] + (Q8_LAZY + SHIFT)) != 0, 0)) {
-                float tm = q8_rows4_max(top);
-                if constexpr (SPLIT) tm = __builtin_ceilf(tm) - SHIFT;
-                float alpha = 1.0f;
-                if (tm > mrun[w] + Q8_LAZY) {
-                    alpha = __builtin_amdgcn_exp2f(mrun[w] - tm);  // (0 from -inf)
-                    mrun[w] = tm;
-                }
-                lsum[w] *= alpha;
+            top[w] = __builtin_fmaf(top[w], x.cks, x.lg);
+            any |= top[w] > mrun[w] + (Q8_LAZY + SHIFT);
+        }
+        return any;
+    }
+    __device__ __forceinline__ void raise(const float (&top)[RW]) {
 #pragma unroll
-                for (int n = 0; n < NB; ++n) o[w][n] *= alpha;
+        for (int w = 0; w < RW; ++w) {
+            float tm = q8_rows4_max(top[w]);
+            if constexpr (SPLIT) tm = __builtin_ceilf(tm) - SHIFT;
+            float alpha = 1.0f;
+            if (tm > mrun[w] + Q8_LAZY) {
+                alpha = __builtin_amdgcn_exp2f(mrun[w] - tm);
+                mrun[w] = tm;
             }
-            // (no key seen yet: every score is -inf)
-            const float b = ef - (mrun[w] == -INFINITY ? 0.0f : mrun[w]);
-            float l = 0.0f;
+            lsum[w] *= alpha;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) o[w][n] *= alpha;
+        }
+    }
+    // Scores to weights ph (and pl), and the rows' sums.
+    __device__ __forceinline__ void weigh(const Unit& x, const q8_f4 (&s)[RW][2], q8_h8 (&ph)[RW], q8_h8 (&pl)[RW]) {
+#pragma unroll
+        for (int w = 0; w < RW; ++w) {
+            const float b = x.lg - mrun[w];
+            float l[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
                 for (int r = 0; r < 4; r += 2) {
-                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[w][cb][r], cks, b));
-                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[w][cb][r + 1], cks, b));
-                    const float x0 = p0 * mu, x1 = p1 * mu;
-                    const q8_h2 h = q8_round2(x0, x1);
-                    ph[w][4 * cb + r] = h[0];
-                    ph[w][4 * cb + r + 1] = h[1];
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[w][cb][r], x.cks, b));
+                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[w][cb][r + 1], x.cks, b));
                     if constexpr (SPLIT) {
+                        const float x0 = p0 * x.mu, x1 = p1 * x.mu;
+                        const q8_h2 h = q8_round2(x0, x1);
                         const q8_h2 d = {(_Float16)(x0 - (float)h[0]), (_Float16)(x1 - (float)h[1])};
+                        ph[w][4 * cb + r] = h[0];
+                        ph[w][4 * cb + r + 1] = h[1];
                         pl[w][4 * cb + r] = d[0];
                         pl[w][4 * cb + r + 1] = d[1];
-                        l += p0 + p1;
+                        l[cb] += p0 + p1;
                     } else {
-                        l = __builtin_amdgcn_fdot2(h, q8_h2{(_Float16)1.0f, (_Float16)1.0f}, l, false);
+                        const q8_h2 h = q8_round2(p0, p1);
+                        ph[w][4 * cb + r] = h[0];
+                        ph[w][4 * cb + r + 1] = h[1];
+                        l[cb] = __builtin_amdgcn_fdot2(h, q8_h2{(_Float16)1.0f, (_Float16)1.0f}, l[cb], false);
                     }
                 }
-            lsum[w] = __builtin_fmaf(l, SPLIT ? down : inv, lsum[w]);
+            lsum[w] = __builtin_fmaf(l[0] + l[1], x.part, lsum[w]);
         }
-    };
-    auto product = [&](int n, q8_h8 a, const q8_h8 (&ph)[RW], const q8_h8 (&pl)[RW]) {
+    }
+    __device__ __forceinline__ void product(int n, q8_h8 a, const q8_h8 (&ph)[RW], const q8_h8 (&pl)[RW]) {
 #pragma unroll
         for (int w = 0; w < RW; ++w) {
             o[w][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph[w], o[w][n], 0, 0, 0);
             if constexpr (SPLIT) o[w][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl[w], o[w][n], 0, 0, 0);
         }
-    };
-
-    int u = u_begin;
-    for (; u < min(u_end, coded_units); u += 4) {
-        q8_f4 s[RW][2];
-#pragma unroll
-        for (int w = 0; w < RW; ++w) s[w][0] = s[w][1] = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
-        const float4 x = sc[u >> P.unit_shift];
-#pragma unroll
-        for (int i = 0; i < KP; ++i) {
-            const int cb = i / (D / 64), st = i % (D / 64);
-            const q8_h8 a0 = q8_halves<FMT>(kr[i][0], kr[i][1]), a1 = q8_halves<FMT>(kr[i][2], kr[i][3]);
-#pragma unroll
-            for (int w = 0; w < RW; ++w) {
-                s[w][cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, qf[w][2 * st], s[w][cb], 0, 0, 0);
-                s[w][cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, qf[w][2 * st + 1], s[w][cb], 0, 0, 0);
-            }
-        }
-        load_k(u + 4);
-        q8_h8 ph[RW], pl[RW];
-        weigh(u << 5, x.x, x.y, x.w, __float_as_int(x.z), s, ph, pl);
-#pragma unroll
-        for (int i = 0; i < KP; ++i) {
-            product(2 * i, q8_halves<FMT>(vr[i][0], vr[i][1]), ph, pl);
-            product(2 * i + 1, q8_halves<FMT>(vr[i][2], vr[i][3]), ph, pl);
-        }
-        load_v(u + 4);
     }
 
-    // The tail: fp16 rows in the same order. What is not finite in V stays out of
-    // the products (0 times it is NaN, so masked keys would show); V's exponents
-    // move so that its largest magnitude lies near the codes'.
-    const int u_tail = u;
-    unsigned wild = 0;
-    for (; u < u_end; u += 4) {
-        const size_t at = (size_t)g * P.block_values + (size_t)(u - coded_units) * (32 * D) + lane * 8;
-        q8_f4 s[RW][2];
+    // Units u, u + step, .. below u_end, all of the tail: fp16 rows in the codes'
+    // order. What is not finite in V stays out of the products (0 times it is NaN,
+    // so masked keys would show); V's exponents move so that its largest magnitude
+    // lies near the codes'. Then `wild` units add it to the rows that see it, after
+    // the last change of a maximum (whatever the weights, which are positive).
+    __device__ __forceinline__ void tail(const AttnQ8Params& P, float c, int g, int u, int u_end, int step, int lane) {
+        const int hi = lane >> 4, coded_units = P.coded >> 5, u0 = u;
+        unsigned wild = 0;
+#pragma unroll 1
+        for (; u < u_end; u += step) {
+            const size_t at = (size_t)g * P.block_values + (size_t)(u - coded_units) * (32 * D) + lane * 8;
+            v4u k[2 * KS], v[NB];
+            auto load_v = [&] {
 #pragma unroll
-        for (int w = 0; w < RW; ++w) s[w][0] = s[w][1] = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int n = 0; n < NB; ++n) v[n] = *reinterpret_cast<const v4u*>(P.vt + at + n * 512);
+            };
 #pragma unroll
-        for (int i = 0; i < 2 * KS; ++i) {
-            const q8_h8 a = __builtin_bit_cast(q8_h8, *reinterpret_cast<const v4u*>(P.kt + at + i * 512));
+            for (int i = 0; i < 2 * KS; ++i) k[i] = *reinterpret_cast<const v4u*>(P.kt + at + i * 512);
+            if constexpr (D < 256) load_v();  // (one memory round trip, where the registers allow)
+            q8_f4 s[RW][2];
 #pragma unroll
-            for (int w = 0; w < RW; ++w)
-                s[w][i / KS] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[w][i % KS], s[w][i / KS], 0, 0, 0);
-        }
-        // (what lies behind the last row is not the cache's)
-        unsigned held[4];
+            for (int w = 0; w < RW; ++w) s[w][0] = s[w][1] = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int key = (u << 5) + (i >> 1) * 16 + 4 * hi + (i & 1) * 2;
-            held[i] = (key < P.len ? 0xFFFFu : 0u) | (key + 1 < P.len ? 0xFFFF0000u : 0u);
-        }
-        unsigned big = 0;
-#pragma unroll 2
-        for (int n = 0; n < NB; ++n) {
-            const v4u x = *reinterpret_cast<const v4u*>(P.vt + at + n * 512);
+            for (int i = 0; i < 2 * KS; ++i)
+#pragma unroll
+                for (int w = 0; w < RW; ++w)
+                    s[w][i / KS] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q8_h8, k[i]), qf[w][i % KS],
+                                                                          s[w][i / KS], 0, 0, 0);
+            if constexpr (D == 256) load_v();
+            // (what lies behind the last row is not the cache's)
+            v4u held;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const unsigned y0 = x[i] & held[i] & 0x7FFFu, y1 = ((x[i] & held[i]) >> 16) & 0x7FFFu;
-                wild |= (y0 >= 0x7C00u) | (y1 >= 0x7C00u);
-                big = max(big, max(y0 >= 0x7C00u ? 0u : y0, y1 >= 0x7C00u ? 0u : y1));
+                const int key = (u << 5) + (i >> 1) * 16 + 4 * hi + (i & 1) * 2;
+                held[i] = (key < P.len ? 0xFFFFu : 0u) | (key + 1 < P.len ? 0xFFFF0000u : 0u);
+            }
+            unsigned big = 0;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                v[n] &= held;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    unsigned x = v[n][i];
+                    const unsigned wild0 = (x & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u;
+                    const unsigned wild1 = (x & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u;
+                    wild |= wild0 | wild1;
+                    x &= ~(wild0 | wild1);
+                    v[n][i] = x;
+                    big = max(big, max(x & 0x7FFFu, (x >> 16) & 0x7FFFu));
+                }
+            }
+            const float top = wave_max(__half2float(__ushort_as_half((unsigned short)big)));
+            const int e = top > 0.0f ? ((__float_as_int(top) >> 23) & 255) - 127 - 6 : -30;
+            const float up = __int_as_float((127 - e) << 23);
+            q8_h8 ph[RW], pl[RW];
+            Unit x = unit(c, 1.0f, 1.0f, e, up);
+            if (masked(u << 5, false)) mask(x, u << 5, false, hi, s);  // (uniform)
+            float top1[RW];
+            if (__builtin_amdgcn_ballot_w64(over(x, s, top1)) != 0) raise(top1);
+            weigh(x, s, ph, pl);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                q8_h8 a = __builtin_bit_cast(q8_h8, v[n]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) a[i] = (_Float16)((float)a[i] * up);
+                product(n, a, ph, pl);
             }
         }
-#pragma unroll
-        for (int i = 1; i < 64; i <<= 1) big = max(big, (unsigned)__shfl_xor((int)big, i));
-        const float top = __half2float(__ushort_as_half((unsigned short)__builtin_amdgcn_readfirstlane((int)big)));
-        const int e = top > 0.0f ? ((__float_as_int(top) >> 23) & 255) - 127 - 6 : -30;
-        const float up = __int_as_float((127 - e) << 23);
-        q8_h8 ph[RW], pl[RW];
-        weigh(u << 5, 1.0f, 1.0f, up, e, s, ph, pl);
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            const v4u x = *reinterpret_cast<const v4u*>(P.vt + at + n * 512);
-            q8_h8 a = __builtin_bit_cast(q8_h8, x & v4u{held[0], held[1], held[2], held[3]});
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float y = (float)a[i];
-                a[i] = (_Float16)(fabsf(y) < INFINITY ? y * up : 0.0f);
-            }
-            product(n, a, ph, pl);
-        }
-    }
-#pragma unroll
-    for (int w = 0; w < RW; ++w) lsum[w] = q8_rows4_sum(lsum[w]);
-
-    // The infinite and NaN values of the tail that a row sees: its outputs take
-    // their sum (whatever the weights, which are positive).
-    if (__builtin_amdgcn_ballot_w64(wild != 0) != 0) {
+        if (__builtin_amdgcn_ballot_w64(wild != 0) == 0) return;
 #pragma unroll 1
-        for (u = u_tail; u < u_end; u += 4) {
+        for (u = u0; u < u_end; u += step) {
             const __half* vt = P.vt + (size_t)g * P.block_values + (size_t)(u - coded_units) * (32 * D);
 #pragma unroll 1
             for (int j = 0; j < 32; ++j) {
@@ -409,142 +399,475 @@ __global__ __launch_bounds__(256) void attn_q8_kernel(AttnQ8Params P) {
             }
         }
     }
+};
 
-    // The waves' partials meet: wave w % 4 gathers row group w.
+// Row rr of KV head g, dims 16 (n0 + n) + 4 hi..+3 for n < NB, one of PARTS calls
+// for the row: divided by l and stored, or, with several splits, left as a partial.
+template <int NB, int PARTS>
+__device__ __forceinline__ void q8_finish(const AttnQ8Params& P, int g, int rr, int split, int hi, int n0, float m,
+                                          float l, const q8_f4 (&o)[NB]) {
+    constexpr int D = 16 * NB * PARTS;
+    const int G = P.qh / P.kh;
+    if (P.splits == 1) {
+        const float il = 1.0f / l;
+        const int h = rr / P.m;
+        const long long at = (long long)(g * G + h) * P.o_head + (rr - h * P.m) * P.o_row + 16 * n0 + 4 * hi;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) q8_store4(P, at + 16 * n, o[n] * il);
+        return;
+    }
+    const size_t row = ((size_t)g * P.rows_pad + rr) * P.splits + split;
+    float* acc = P.part + row * D + 16 * n0 + 4 * hi;
+    float* ml = P.part + (size_t)P.kh * P.rows_pad * P.splits * D + row * 2;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) *reinterpret_cast<q8_f4*>(acc + 16 * n) = o[n];
+    if (hi == 0 && n0 == 0) *reinterpret_cast<float2*>(ml) = float2{m, l};
+}
+
+// The NW waves of a row tile meet: each leaves its accumulators in LDS (NW RW NB KiB)
+// and its rows' (max, sum), and takes an NW-th of the tile's (row group, dims) pairs.
+template <int D, int NW, int RW, bool SPLIT>
+__device__ __forceinline__ void q8_meet(const AttnQ8Params& P, const Q8Wave<D, RW, SPLIT>& W, int g, int rt, int split,
+                                        int wave, int lane, uint8_t* smem, float (&ml)[NW][RW][2][16]) {
+    constexpr int NB = D / 16;
+    const int lo = lane & 15, hi = lane >> 4, R = P.qh / P.kh * P.m;
 #pragma unroll
     for (int w = 0; w < RW; ++w) {
-        const int owner = w & 3;
-        if (w) __syncthreads();  // (the previous group's reads are done)
-        if (wave != owner) {
-            const int at = wave < owner ? wave : wave - 1;
 #pragma unroll
-            for (int n = 0; n < NB; ++n) *reinterpret_cast<q8_f4*>(&merge[((at * NB + n) * 64 + lane) * 4]) = o[w][n];
-            merge_ml[at][0][lane] = mrun[w];
-            merge_ml[at][1][lane] = lsum[w];
+        for (int n = 0; n < NB; ++n)
+            *reinterpret_cast<q8_f4*>(smem + ((w * NB + n) * NW + wave) * 1024 + lane * 16) = W.o[w][n];
+        if (hi == 0) {
+            ml[wave][w][0][lo] = W.mrun[w];
+            ml[wave][w][1][lo] = W.lsum[w];
         }
-        __syncthreads();
-        if (wave != owner) continue;
-        float mx[3], top = mrun[w];
+    }
+    __syncthreads();
+    // pairs of a wave, all of one row group (more waves than pairs: the first ones')
+    constexpr int MINE = RW * NB >= NW ? RW * NB / NW : 1;
+    static_assert(RW * NB % MINE == 0 && NB % MINE == 0, "pairs per wave");
+    if (wave * MINE >= RW * NB) return;
+    const int w = wave * MINE / NB, n0 = wave * MINE % NB;
+    float top = Q8_NONE, l = 0.0f, m1[NW];
 #pragma unroll
-        for (int at = 0; at < 3; ++at) {
-            mx[at] = merge_ml[at][0][lane];
-            top = fmaxf(top, mx[at]);
-        }
-        const float a = q8_weight(mrun[w], top);
-        float l = lsum[w] * a;
+    for (int i = 0; i < NW; ++i) {
+        m1[i] = ml[i][w][0][lo];
+        top = fmaxf(top, m1[i]);
+    }
+    q8_f4 sum[MINE];
 #pragma unroll
-        for (int n = 0; n < NB; ++n) o[w][n] *= a;
+    for (int n = 0; n < MINE; ++n) sum[n] = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int at = 0; at < 3; ++at) {
-            // (a wave that saw no key holds zeros; one that saw NaN scores has
-            // maximum -inf and NaN sums)
-            const float b = q8_weight(mx[at], top), l1 = merge_ml[at][1][lane];
-            l += l1 != l1 ? l1 : l1 * b;
+    for (int i = 0; i < NW; ++i) {
+        // (a wave that saw no key holds zeros, one that saw NaN scores a NaN sum)
+        const float b = q8_weight(m1[i], top), l1 = ml[i][w][1][lo];
+        l += l1 != l1 ? l1 : l1 * b;
 #pragma unroll
-            for (int n = 0; n < NB; ++n)
-                o[w][n] += *reinterpret_cast<const q8_f4*>(&merge[((at * NB + n) * 64 + lane) * 4]) * b;
-        }
-        if (lsum[w] != lsum[w]) l = lsum[w];
-        const int rr = rt * RT + 16 * w + lo;
-        if (rr >= R) continue;
-        if (P.splits == 1) {
-            const float il = 1.0f / l;
-            const long long at = (g * G + rr / P.m) * P.o_head + rr % P.m * P.o_row + 4 * hi;
+        for (int n = 0; n < MINE; ++n)
+            sum[n] += *reinterpret_cast<const q8_f4*>(smem + ((w * NB + n0 + n) * NW + i) * 1024 + lane * 16) * b;
+    }
+    const int rr = (rt * RW + w) * 16 + lo;
+    if (rr < R) q8_finish<MINE, NB / MINE>(P, g, rr, split, hi, n0, top, l, sum);
+}
+
+// Few rows. Block: NW waves over one tile of 16 RW query rows of one KV head; wave w
+// takes units w, w + NW, .. of its split, so nothing is shared until the waves'
+// partial (max, sum, accumulators) meet in LDS. A unit's codes go from memory into
+// operand registers; the loads of the next unit are issued as soon as this one's are
+// converted.
+//
+// Measured, the join included: one row of 32 heads over 8 of 128 and 131072 keys
+// (268 MB) e4m3 46.5 us, i8 48: 5.8 and 5.6 TB/s (a large copy reads and writes
+// 4.9). Over 3968 keys (8 MB) 8.0: there it is latency, a unit's load to its
+// products, the waves' meeting and the join's launch. 512 rows over 4096 keys 21.9:
+// conversion and softmax, vector instructions that every 32 rows repeat. The splits
+// joined by their last block, in the same launch, lost to a launch of their own (8.6):
+// 10.0 with the partials through atomics of agent scope, 30 behind a fence, which
+// writes the L2 back. Blocks of 2 or 4 groups of waves with keys of their own and
+// more rows each: 27 to 31 for the 512 rows.
+template <int D, int NW, int RW, int FMT, bool SPLIT>
+__global__ __launch_bounds__(64 * NW) void attn_q8_kernel(AttnQ8Params P) {
+    constexpr int KP = D / 32;  // 16-byte pieces per lane, of K (and V)
+    constexpr int RT = 16 * RW;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[NW * RW * (D / 16) * 1024];
+    __shared__ float ml[NW][RW][2][16];
+    const int g = blockIdx.x, rt = blockIdx.y, split = blockIdx.z;
+    const int lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const float c = fminf(P.scale * 1.4426950408889634f, 0x1.fffffep127f);
+    const uint8_t* kbase = P.k + (size_t)g * P.head_bytes + lane * 16;
+    const uint8_t* vbase = P.v + (size_t)g * P.head_bytes + lane * 16;
+    const float4* sc = P.sc + (size_t)g * P.blocks;
+    const int coded_units = P.coded >> 5;
+    const int u_begin = split * P.units_per_split + wave;
+
+    v4u kr[KP], vr[KP];
+    // (the last coded unit's own codes again where there is no further one)
+    auto load_k = [&](int u) {
+        const uint8_t* p = kbase + (size_t)min(u, coded_units - 1) * (32 * D);
 #pragma unroll
-            for (int n = 0; n < NB; ++n) q8_store4(P, at + 16 * n, o[w][n] * il);
-        } else {
-            const size_t row = ((size_t)g * P.rows_pad + rr) * P.splits + split;
+        for (int i = 0; i < KP; ++i) kr[i] = *reinterpret_cast<const v4u*>(p + i * 1024);
+    };
+    auto load_v = [&](int u) {
+        const uint8_t* p = vbase + (size_t)min(u, coded_units - 1) * (32 * D);
 #pragma unroll
-            for (int n = 0; n < NB; ++n)
-                *reinterpret_cast<q8_f4*>(P.part + row * D + 16 * n + 4 * hi) = o[w][n];
-            if (hi == 0) {
-                float* ml = P.part + (size_t)P.kh * P.rows_pad * P.splits * D + row * 2;
-                ml[0] = top;
-                ml[1] = l;
+        for (int i = 0; i < KP; ++i) vr[i] = *reinterpret_cast<const v4u*>(p + i * 1024);
+    };
+    float4 next = float4{1.0f, 1.0f, 0.0f, 1.0f};  // the next unit's scales
+    if (coded_units > 0) {
+        next = sc[min(u_begin, coded_units - 1) >> P.unit_shift];
+        load_k(u_begin);
+        load_v(u_begin);
+    }
+    Q8Wave<D, RW, SPLIT> W;
+    W.start(P, g, rt * RT, lo, hi);
+    const int u_end = min(min((split + 1) * P.units_per_split, P.units), (W.seen + 31) >> 5);
+    int u = u_begin;
+    for (; u < min(u_end, coded_units); u += NW) {
+        q8_f4 s[RW][2];
+#pragma unroll
+        for (int w = 0; w < RW; ++w) s[w][0] = s[w][1] = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        const float4 x = next;
+        next = sc[min(u + NW, coded_units - 1) >> P.unit_shift];
+#pragma unroll
+        for (int i = 0; i < KP; ++i) {
+            const int cb = i / (D / 64), st = i % (D / 64);
+            const q8_h8 a0 = q8_halves<FMT>(kr[i][0], kr[i][1]), a1 = q8_halves<FMT>(kr[i][2], kr[i][3]);
+#pragma unroll
+            for (int w = 0; w < RW; ++w) {
+                s[w][cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, W.qf[w][2 * st], s[w][cb], 0, 0, 0);
+                s[w][cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, W.qf[w][2 * st + 1], s[w][cb], 0, 0, 0);
             }
         }
+        load_k(u + NW);
+        q8_h8 ph[RW], pl[RW];
+        auto un = W.unit(c, x.x, x.y, __float_as_int(x.z), x.w);
+        if (__builtin_expect(W.masked(u << 5, false), 0)) W.mask(un, u << 5, false, hi, s);  // (uniform)
+        float top[RW];
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(W.over(un, s, top)) != 0, 0)) W.raise(top);
+        W.weigh(un, s, ph, pl);
+#pragma unroll
+        for (int i = 0; i < KP; ++i) {
+            W.product(2 * i, q8_halves<FMT>(vr[i][0], vr[i][1]), ph, pl);
+            W.product(2 * i + 1, q8_halves<FMT>(vr[i][2], vr[i][3]), ph, pl);
+        }
+        load_v(u + NW);
+    }
+    W.tail(P, c, g, u, u_end, NW, lane);
+#pragma unroll
+    for (int w = 0; w < RW; ++w) W.lsum[w] = q8_rows4_sum(W.lsum[w]);
+    q8_meet<D, NW, RW, SPLIT>(P, W, g, rt, split, wave, lane, smem, ml);
+}
+
+// Much work. Block: NW waves with RW groups of 16 rows each over one split; the codes
+// of a stage of U units are converted once, by all threads, into fp16 fragments in
+// LDS that every wave multiplies with its own rows (attn_q8_kernel converts a unit
+// in every wave: 128 of some 250 vector instructions a unit of 32 rows).
+//
+// In step j a wave turns the scores of unit j into weights, computes those of unit
+// j + 1 and multiplies V of unit j - 1: one straight piece of code in which matrix
+// and vector instructions do not depend on each other. In stage t K of stage t + 2
+// and V of stage t + U - 1 (codes in registers since U = 2: stage t - 1, U = 1:
+// t - 2) are converted meanwhile; U + 1 stages of each are in LDS, with one barrier
+// per stage.
+//
+// Measured: 1024 rows of 8 heads of 128 over 32768 keys 149 us with f16 output, 0.92
+// PFLOP/s of a large matrix product's 1.29, 197 with f32 (a third more products: V's
+// with two fp16 for a weight). Matrix cores 42 % busy, vector instructions 54 % of the
+// time: the softmax of 16 scores a lane and unit holds back the products, whose
+// operands come from LDS once for 32 rows. U = 1: 151 to 157. Matrix and vector
+// instructions interleaved by scheduling groups: 162.
+template <int D, int NW, int U, int RW, int FMT, bool SPLIT>
+__global__ __launch_bounds__(64 * NW) void attn_q8_tile_kernel(AttnQ8Params P) {
+    constexpr int KS = D / 32, NB = D / 16, NT = 64 * NW;
+    constexpr int BUFS = U + 1;  // stages in LDS
+    constexpr int UNIT = 64 * D, HALF = UNIT * U;  // bytes of a unit's, a stage's K (or V) fragments
+    constexpr int PIECES = 2 * D * U;       // 16-byte code pieces of a stage's K (and V)
+    constexpr int PT = (2 * PIECES + NT - 1) / NT;  // of both, per thread
+    constexpr bool DEEP = U == 1;  // (codes two stages ahead)
+    static_assert((U == 1 || U == 2) && PIECES % 64 == 0 && 2 * BUFS * HALF <= 144 * 1024, "stage shape");
+    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * BUFS * HALF];
+    __shared__ float4 units[3][U];
+    const int g = blockIdx.x, rt = blockIdx.y, split = blockIdx.z;
+    const int R = P.qh / P.kh * P.m;
+    const int tid = threadIdx.x, lane = tid & 63, lo = lane & 15, hi = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const float c = fminf(P.scale * 1.4426950408889634f, 0x1.fffffep127f);
+    const uint8_t* kbase = P.k + (size_t)g * P.head_bytes;
+    const uint8_t* vbase = P.v + (size_t)g * P.head_bytes;
+    const float4* sc = P.sc + (size_t)g * P.blocks;
+    const int coded_units = P.coded >> 5;
+    const int u_begin = split * P.units_per_split;
+    const int u_last = min((split + 1) * P.units_per_split, P.units);
+    const int u_coded = min(u_last, coded_units);
+    const int stages = (u_coded - u_begin + U - 1) / U;  // (0 or less: only the tail)
+
+    // Pieces 0..PIECES - 1 of a thread's count are K of stage tk, the others V of
+    // stage tv. (a unit past the split's coded ones: the last of these again, not
+    // used)
+    v4u raw[PT], raw1[PT];
+    auto load = [&](v4u (&raw)[PT], int tk, int tv) {
+#pragma unroll
+        for (int i = 0; i < PT; ++i) {
+            const int p = i * NT + tid, q = p % PIECES;
+            const bool k = p < PIECES;  // (whole waves)
+            const int unit = min(u_begin + (k ? tk : tv) * U + q / (2 * D), u_coded - 1);
+            if (2 * PIECES % NT == 0 || p < 2 * PIECES)
+                raw[i] = *reinterpret_cast<const v4u*>((k ? kbase : vbase) + (size_t)unit * (32 * D) + (q % (2 * D)) * 16);
+        }
+    };
+    auto load_scale = [&](int t) {
+        return tid < U ? sc[min(u_begin + t * U + tid, u_coded - 1) >> P.unit_shift] : float4{1.0f, 1.0f, 0.0f, 1.0f};
+    };
+    auto kbuf = [&](int t) { return smem + t % BUFS * HALF; };
+    auto vbuf = [&](int t) { return smem + (BUFS + t % BUFS) * HALF; };
+    // (piece p of 64 lanes: fragments 2 (p / 64) and the next)
+    auto store = [&](const v4u (&raw)[PT], int tk, int tv) {
+#pragma unroll
+        for (int i = 0; i < PT; ++i) {
+            const int p = i * NT + tid, q = p % PIECES;
+            uint8_t* at = (p < PIECES ? kbuf(tk) : vbuf(tv)) + (q >> 6) * 2048 + (q & 63) * 16;
+            if (2 * PIECES % NT == 0 || p < 2 * PIECES) {
+                *reinterpret_cast<q8_h8*>(at) = q8_halves<FMT>(raw[i][0], raw[i][1]);
+                *reinterpret_cast<q8_h8*>(at + 1024) = q8_halves<FMT>(raw[i][2], raw[i][3]);
+            }
+        }
+    };
+
+    typedef Q8Wave<D, RW, SPLIT> Wave;
+    auto store_unit = [&](int t, const float4& s) {
+        const typename Wave::Unit x = Wave::unit(c, s.x, s.y, __float_as_int(s.z), s.w);
+        units[t % 3][tid] = float4{x.cks, x.lg, x.mu, x.part};
+    };
+    Wave W;
+    float4 s0, s1;
+    if (stages > 0) {
+        load(raw, 0, 0);
+        load(raw1, 1, 0);
+        s0 = load_scale(0);
+        s1 = load_scale(1);
+    }
+    W.start(P, g, (rt * NW + wave) * 16 * RW, lo, hi);
+    if (stages > 0) {
+        // (V of stage 0 into the place of stage -1 too: finite, its weights are 0)
+        store(raw, 0, BUFS - 1);
+        store(raw1, 1, 0);
+        if (tid < U) {
+            store_unit(0, s0);
+            store_unit(1, s1);
+        }
+        // In stage t: K of t + 2, and V of the first stage not there.
+        constexpr int VA = U - 1;
+        load(raw, 2, VA);
+        s0 = load_scale(2);
+        if constexpr (DEEP) {
+            load(raw1, 3, 1);
+            s1 = load_scale(3);
+        }
+        __syncthreads();
+        // (unit j: j % U of stage j / U)
+        auto scores = [&](q8_f4 (&s)[RW][2], int j) {
+            const uint8_t* k = kbuf(j / U) + j % U * UNIT + lane * 16;
+#pragma unroll
+            for (int w = 0; w < RW; ++w) s[w][0] = s[w][1] = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < KS; ++i)
+#pragma unroll
+                for (int cb = 0; cb < 2; ++cb) {
+                    const q8_h8 a = *reinterpret_cast<const q8_h8*>(k + (cb * KS + i) * 1024);
+#pragma unroll
+                    for (int w = 0; w < RW; ++w)
+                        s[w][cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, W.qf[w][i], s[w][cb], 0, 0, 0);
+                }
+        };
+        auto products = [&](int j, const q8_h8 (&ph)[RW], const q8_h8 (&pl)[RW]) {
+            const uint8_t* v = (j < 0 ? vbuf(BUFS - 1) : vbuf(j / U) + j % U * UNIT) + lane * 16;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) W.product(n, *reinterpret_cast<const q8_h8*>(v + n * 1024), ph, pl);
+        };
+        auto unit_of = [&](int j) {
+            const float4 x = units[j / U % 3][j % U];
+            return typename Wave::Unit{x.x, x.y, x.z, x.w};
+        };
+        // What a unit's scores need before they are weighed: masks, and whether a
+        // maximum moves.
+        auto look = [&](int j, typename Wave::Unit& x, q8_f4 (&s)[RW][2], float (&top)[RW]) {
+            bool any = W.over(x, s, top);
+            const int u = u_begin + j;
+            if (__builtin_expect(W.masked(u << 5, u >= u_coded), 0)) {  // (uniform)
+                W.mask(x, u << 5, u >= u_coded, hi, s);
+                any = W.over(x, s, top);
+            }
+            return __builtin_amdgcn_ballot_w64(any) != 0;
+        };
+        typename Wave::Unit now = unit_of(0);
+        float top[RW];
+        q8_f4 sa[RW][2], sb[RW][2];
+        q8_h8 pha[RW], pla[RW], phb[RW], plb[RW];
+#pragma unroll
+        for (int w = 0; w < RW; ++w) pha[w] = pla[w] = phb[w] = plb[w] = q8_h8{};
+        scores(sa, 0);
+        bool moves = look(0, now, sa, top);
+        // One unit: s and (ph0, pl0) in, of this unit and the one before; sn and
+        // (ph1, pl1) out, of the next and this one. A stage's first unit waits for
+        // the stage and fills the next one.
+        auto step = [&](int j, bool begins, v4u (&raw)[PT], float4& s0, q8_f4 (&s)[RW][2], q8_h8 (&ph0)[RW],
+                        q8_h8 (&pl0)[RW], q8_f4 (&sn)[RW][2], q8_h8 (&ph1)[RW], q8_h8 (&pl1)[RW]) {
+            if (begins) __syncthreads();
+            if (__builtin_expect(moves, 0)) {  // (uniform)
+                // (what waits to be added has the old maximum)
+                products(j - 1, ph0, pl0);
+#pragma unroll
+                for (int w = 0; w < RW; ++w) ph0[w] = pl0[w] = q8_h8{};
+                W.raise(top);
+            }
+            if (begins) {
+                const int t = j / U;
+                constexpr int AHEAD = DEEP ? 2 : 1;
+                store(raw, t + 2, t + VA);
+                if (tid < U) store_unit(t + 2, s0);
+                load(raw, t + 2 + AHEAD, t + VA + AHEAD);
+                s0 = load_scale(t + 2 + AHEAD);
+            }
+            typename Wave::Unit then = unit_of(j + 1);
+            scores(sn, j + 1);
+            W.weigh(now, s, ph1, pl1);
+            products(j - 1, ph0, pl0);
+            moves = look(j + 1, then, sn, top);
+            now = then;
+        };
+        const int count = stages * U;
+        for (int j = 0; j < count; j += 2) {
+            step(j, true, raw, s0, sa, pha, pla, sb, phb, plb);
+            if (U == 2 || j + 1 < count) {
+                if constexpr (DEEP)
+                    step(j + 1, true, raw1, s1, sb, phb, plb, sa, pha, pla);
+                else
+                    step(j + 1, U == 1, raw, s0, sb, phb, plb, sa, pha, pla);
+            } else {
+#pragma unroll
+                for (int w = 0; w < RW; ++w) {
+                    pha[w] = phb[w];
+                    pla[w] = plb[w];
+                }
+            }
+        }
+        __syncthreads();
+        products(count - 1, pha, pla);
+    }
+    W.tail(P, c, g, max(u_begin, coded_units), min(u_last, (W.seen + 31) >> 5), 1, lane);
+#pragma unroll
+    for (int w = 0; w < RW; ++w) W.lsum[w] = q8_rows4_sum(W.lsum[w]);
+#pragma unroll
+    for (int w = 0; w < RW; ++w) {
+        const int rr = ((rt * NW + wave) * RW + w) * 16 + lo;
+        if (rr < R) q8_finish<NB, 1>(P, g, rr, split, hi, 0, W.mrun[w], W.lsum[w], W.o[w]);
     }
 }
 
 // The splits' partials of one row: out = sum_s w_s acc_s / sum_s w_s l_s with
-// w_s = 2^(m_s - max m). One wave per row, 4 rows a block; lane s holds the
-// weights of splits s, s + 64, ..; the accumulators of 8 splits are in flight.
-template <int D>
+// w_s = 2^(m_s - max m). RPB rows a block, T = 256 / RPB threads each, thread t
+// with 4 dims of every GS-th split (GS = 4 T / D); their loads, 8 at a time, do not
+// wait for the weights, which the row's threads find meanwhile; sums over the GS
+// groups meet in LDS.
+template <int D, int RPB>
 __global__ __launch_bounds__(256) void attn_q8_combine_kernel(AttnQ8Params P) {
-    constexpr int ND = D / 64, B = 8;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = blockIdx.y;
-    const int rr = blockIdx.x * 4 + wave;
+    constexpr int T = 256 / RPB, LD = D / 4, GS = T / LD, B = 8;
+    static_assert(GS >= 1 && T % LD == 0, "threads per row");
+    __shared__ float weight[RPB][256];
+    __shared__ float red[RPB][2][T / 32];
+    __shared__ q8_f4 part[RPB][GS][LD];
+    const int row = threadIdx.x / T, t = threadIdx.x % T, d4 = t % LD, gs = t / LD, g = blockIdx.y;
+    const int rr0 = blockIdx.x * RPB + row;
     const int G = P.qh / P.kh, R = G * P.m, S = P.splits;
-    if (rr >= R) return;  // (wave-uniform; no barrier below)
-    const size_t row = ((size_t)g * P.rows_pad + rr) * S;
-    const float2* ml = reinterpret_cast<const float2*>(P.part + (size_t)P.kh * P.rows_pad * S * D) + row;
+    const int rr = min(rr0, R - 1);  // (threads past the last row: that row again, not written)
+    const size_t at = ((size_t)g * P.rows_pad + rr) * S;
+    const q8_f4* acc = reinterpret_cast<const q8_f4*>(P.part + at * D) + d4;
+    q8_f4 v[B];
+#pragma unroll
+    for (int i = 0; i < B; ++i) v[i] = acc[(size_t)min(gs + i * GS, S - 1) * LD];
+    // weights and denominator, over the row's threads (whole half waves)
+    const float2* ml = reinterpret_cast<const float2*>(P.part + (size_t)P.kh * P.rows_pad * S * D) + at;
+    float2 x[256 / T];
     float top = -INFINITY;
-    for (int s = lane; s < S; s += 64) top = fmaxf(top, ml[s].x);
 #pragma unroll
-    for (int i = 1; i < 64; i <<= 1) top = fmaxf(top, __shfl_xor(top, i));
-    float den = 0.0f, num[ND];
+    for (int i = 0; i < 256 / T; ++i) {
+        x[i] = t + i * T < S ? ml[t + i * T] : float2{-INFINITY, 0.0f};
+        top = fmaxf(top, x[i].x);
+    }
 #pragma unroll
-    for (int d = 0; d < ND; ++d) num[d] = 0.0f;
-    for (int s0 = 0; s0 < S; s0 += 64) {
-        const int mine = s0 + lane;
-        const float2 x = mine < S ? ml[mine] : float2{-INFINITY, 0.0f};
-        const float w = q8_weight(x.x, top);
-        den += x.y != x.y ? x.y : w * x.y;
-        const int count = min(64, S - s0);
-        for (int b = 0; b < count; b += B) {
-            float v[B][ND];
+    for (int i = 1; i < 32; i <<= 1) top = fmaxf(top, __shfl_xor(top, i));
+    if (t % 32 == 0) red[row][0][t / 32] = top;
+    __syncthreads();
 #pragma unroll
-            for (int i = 0; i < B; ++i)
+    for (int i = 0; i < T / 32; ++i) top = fmaxf(top, red[row][0][i]);
+    float den = 0.0f;
 #pragma unroll
-                for (int d = 0; d < ND; ++d)
-                    v[i][d] = P.part[(row + s0 + min(b + i, count - 1)) * D + lane + 64 * d];
+    for (int i = 0; i < 256 / T; ++i) {
+        const float w = q8_weight(x[i].x, top);
+        weight[row][t + i * T] = w;
+        // (a split that saw NaN scores has maximum -inf and a NaN sum)
+        den += x[i].y != x[i].y ? x[i].y : w * x[i].y;
+    }
 #pragma unroll
-            for (int i = 0; i < B; ++i) {
-                const float wi = __shfl(w, min(b + i, count - 1));
+    for (int i = 1; i < 32; i <<= 1) den += __shfl_xor(den, i);
+    if (t % 32 == 0) red[row][1][t / 32] = den;
+    __syncthreads();
+    q8_f4 num = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = gs; s < S; s += B * GS) {
 #pragma unroll
-                for (int d = 0; d < ND; ++d)
-                    num[d] = b + i < count ? __builtin_fmaf(wi, v[i][d], num[d]) : num[d];
-            }
+        for (int i = 0; i < B; ++i) {
+            if (s + i * GS < S) num += v[i] * weight[row][s + i * GS];
+            v[i] = acc[(size_t)min(s + (B + i) * GS, S - 1) * LD];
         }
     }
+    if constexpr (GS > 1) {
+        part[row][gs][d4] = num;
+        __syncthreads();
+        if (gs) return;
 #pragma unroll
-    for (int i = 1; i < 64; i <<= 1) den += __shfl_xor(den, i);
-    const float il = 1.0f / den;
-    const long long at = (g * G + rr / P.m) * P.o_head + rr % P.m * P.o_row + lane;
-#pragma unroll
-    for (int d = 0; d < ND; ++d) {
-        const float y = num[d] * il;
-        if (P.out_f16)
-            static_cast<__half*>(P.out)[at + 64 * d] = __float2half_rn(y);
-        else
-            static_cast<float*>(P.out)[at + 64 * d] = y;
+        for (int i = 1; i < GS; ++i) num += part[row][i][d4];
     }
+    if (rr0 >= R) return;
+    den = red[row][1][0];
+#pragma unroll
+    for (int i = 1; i < T / 32; ++i) den += red[row][1][i];
+    const int h = rr / P.m;
+    q8_store4(P, (long long)(g * G + h) * P.o_head + (rr - h * P.m) * P.o_row + 4 * d4, num * (1.0f / den));
 }
 
-// Row groups (16 rows) per tile for R rows of a KV head.
-inline int q8_row_groups(int head_dim, int R) { return R <= 16 ? 1 : R <= 32 || head_dim == 256 ? 2 : 4; }
+// Row groups (of 16) a wave takes, and rows of a block: attn_q8_kernel's waves share
+// the rows, attn_q8_tile_kernel's have their own.
+constexpr int Q8_WAVES = 8;
+inline int q8_groups(int head_dim, int R) { return R <= 16 || head_dim == 256 ? 1 : 2; }
+inline int q8_block_rows(int head_dim, int R, bool tile) { return 16 * q8_groups(head_dim, R) * (tile ? Q8_WAVES : 1); }
 
-void launch_attn_q8_i8(const AttnQ8Params& P, int head_dim, int row_groups, bool f32_weights, hipStream_t s);
-void launch_attn_q8_e4m3(const AttnQ8Params& P, int head_dim, int row_groups, bool f32_weights, hipStream_t s);
+void launch_attn_q8_i8(const AttnQ8Params& P, int head_dim, int R, bool tile, bool f32_weights, hipStream_t s);
+void launch_attn_q8_e4m3(const AttnQ8Params& P, int head_dim, int R, bool tile, bool f32_weights, hipStream_t s);
 
 template <int D, int FMT, bool SPLIT>
-static void launch_attn_q8_rows(const AttnQ8Params& P, int row_groups, hipStream_t s) {
-    const dim3 grid(P.splits, P.row_tiles, P.kh);
-    if (row_groups == 1)
-        hipLaunchKernelGGL((attn_q8_kernel<D, 1, FMT, SPLIT>), grid, dim3(256), 0, s, P);
-    else if (row_groups == 2)
-        hipLaunchKernelGGL((attn_q8_kernel<D, 2, FMT, SPLIT>), grid, dim3(256), 0, s, P);
-    else if constexpr (D < 256)
-        hipLaunchKernelGGL((attn_q8_kernel<D, 4, FMT, SPLIT>), grid, dim3(256), 0, s, P);
+static void launch_attn_q8_rows(const AttnQ8Params& P, int R, bool tile, hipStream_t s) {
+    // (a row tile's blocks of one KV head are 8 apart where there are 8 heads: the
+    // XCDs take blocks in turn, so each keeps one head's codes in its L2)
+    const dim3 grid(P.kh, P.row_tiles, P.splits), block(64 * Q8_WAVES);
+    if (tile) {
+        if constexpr (D == 256)
+            hipLaunchKernelGGL((attn_q8_tile_kernel<D, Q8_WAVES, 1, 1, FMT, SPLIT>), grid, block, 0, s, P);
+        else
+            hipLaunchKernelGGL((attn_q8_tile_kernel<D, Q8_WAVES, 2, 2, FMT, SPLIT>), grid, block, 0, s, P);
+    } else if (q8_groups(D, R) == 1) {
+        hipLaunchKernelGGL((attn_q8_kernel<D, Q8_WAVES, 1, FMT, SPLIT>), grid, block, 0, s, P);
+    } else if constexpr (D < 256) {
+        hipLaunchKernelGGL((attn_q8_kernel<D, Q8_WAVES, 2, FMT, SPLIT>), grid, block, 0, s, P);
+    }
 }
 
 template <int FMT>
-static void launch_attn_q8(const AttnQ8Params& P, int head_dim, int row_groups, bool f32_weights, hipStream_t s) {
-#define HM_Q8_ROWS(DD)                                       \
-    if (f32_weights)                                         \
-        launch_attn_q8_rows<DD, FMT, true>(P, row_groups, s); \
-    else                                                     \
-        launch_attn_q8_rows<DD, FMT, false>(P, row_groups, s)
+static void launch_attn_q8(const AttnQ8Params& P, int head_dim, int R, bool tile, bool f32_weights, hipStream_t s) {
+#define HM_Q8_ROWS(DD)                                     \
+    if (f32_weights)                                       \
+        launch_attn_q8_rows<DD, FMT, true>(P, R, tile, s); \
+    else                                                   \
+        launch_attn_q8_rows<DD, FMT, false>(P, R, tile, s)
     if (head_dim == 64) {
         HM_Q8_ROWS(64);
     } else if (head_dim == 128) {

@@ -306,7 +306,7 @@ static const int kBN[] = {256, 128, 128, 128, 128, 256};
 // variable, read once when the library first plans a launch; afterwards only
 // rk_npu_hip_set_switch changes it, so no launch reads the environment.
 enum SwitchId { SW_GEMM_VARIANT, SW_SPLITS, SW_FORCE_GEMM, SW_GEMV_QW, SW_GEMV_SPLITS, SW_FFN_FUSED, SW_FFN_SPIN,
-                SW_GEMV_PREQ, SW_HOST_SPIN, SW_GEMV_COMBINE, SW_HOST_FLAG, SW_HOST_POLL, SW_SKINNY,
+                SW_GEMV_PREQ, SW_HOST_SPIN, SW_GEMV_COMBINE, SW_HOST_FLAG, SW_HOST_POLL, SW_SKINNY, SW_Q8_TILE,
                 SW_COUNT };
 struct SwitchDef {
     const char* name;
@@ -316,7 +316,7 @@ static const SwitchDef kSwitches[SW_COUNT] = {
     {"HM_GEMM_VARIANT", -1}, {"HM_SPLITS", 0},         {"HM_FORCE_GEMM", 0}, {"HM_GEMV_QW", -1},
     {"HM_GEMV_SPLITS", 0},   {"HM_FFN_FUSED", 0},      {"HM_FFN_SPIN", 1 << 16}, {"HM_GEMV_PREQ", -1},
     {"HM_HOST_SPIN", 0},     {"HM_GEMV_COMBINE", 1},   {"HM_HOST_FLAG", 1},       {"HM_HOST_POLL", 2000},
-    {"HM_SKINNY", -1}};
+    {"HM_SKINNY", -1},       {"HM_Q8_TILE", -1}};
 
 static std::atomic<int>* switch_table() {
     static std::atomic<int> table[SW_COUNT];
@@ -1197,6 +1197,7 @@ __global__ __launch_bounds__(1024) void host_publish_kernel(const v4u* __restric
     if (threadIdx.x == 0) __hip_atomic_store(done, seq, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 
+int attention_q8_tile_switch() { return switch_value(SW_Q8_TILE); }
 bool host_kernels_enabled() { return switch_value(SW_HOST_FLAG) != 0; }
 
 bool stage_small(const HostStage& st, const void* p, size_t in_bytes, size_t out_bytes) {

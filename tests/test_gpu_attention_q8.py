@@ -232,6 +232,48 @@ def test_attention_row_counts(ctx, d, fmt, dtype):
     p.check_run(33, 0, dtype)
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("length", [33, 64, 100, 129, 300, 1111])
+def test_attention_much_work_kernel(ctx, d, fmt, length):
+    """The kernel for much work, forced onto short contexts: one stage, odd and even
+    counts of them, a tail, several splits, rows past the last block's."""
+    with D.plan_switch("HM_Q8_TILE", 1):
+        for causal, block, dtype in ((True, 32, torch.float32), (False, 64, torch.float16), (True, 128, torch.float16)):
+            p = Pair(ctx, 6, 2, d, fmt, block, causal=causal, capacity=1200, seed=d + length)
+            p.fill(length)
+            for rows in (1, 33, min(90, length)):
+                p.check_run(rows, length - rows if length >= rows else 0, dtype)
+    p.check_run(1, 0, torch.float32)
+
+
+def test_much_work_takes_its_kernel(ctx):
+    """A call large enough for it by itself, 256 rows of 8 heads over 12000 keys of
+    256: the same bits as forced, others than without."""
+    p = Pair(ctx, 8, 1, 256, "i8", 64, capacity=12000, seed=3)
+    p.fill(12000)
+    q = torch.randn(8, 256, 256, device="cuda", dtype=torch.float16)
+    outs = []
+    for value in (-1, 1, 0):
+        with D.plan_switch("HM_Q8_TILE", value):
+            outs.append(torch.empty(8, 256, 256, device="cuda"))
+            D.attention_q8(ctx, p.cache, q, outs[-1], 12000 - 256)
+    assert torch.equal(outs[0], outs[1]) and not torch.equal(outs[0], outs[2])
+    assert torch.allclose(outs[0], outs[2], rtol=0, atol=1e-4)
+    p.compare(q[:, :4].cpu().numpy(), outs[0][:, :4], 12000 - 256)
+
+
+@pytest.mark.parametrize("tile", [0, 1])
+def test_special_values_in_both_kernels(ctx, tile):
+    """Poisoned blocks, infinities of the tail, scales far apart and late maxima, each
+    kernel forced."""
+    with D.plan_switch("HM_Q8_TILE", tile):
+        test_scales_of_all_sizes_share_a_row(ctx)
+        test_not_finite_values(ctx)
+        test_peaked_scores(ctx)
+        test_wide_heads_not_finite_over_splits(ctx)
+
+
 @pytest.mark.parametrize("length", [1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 160, 255, 257])
 def test_attention_lengths(ctx, length):
     """Contexts of one token, of the tail alone, of whole blocks and of both, with

@@ -323,14 +323,17 @@ struct Q8Wave {
 #pragma unroll 1
         for (; u < u_end; u += step) {
             const size_t at = (size_t)g * P.block_values + (size_t)(u - coded_units) * (32 * D) + lane * 8;
-            v4u k[2 * KS], v[NB];
-            auto load_v = [&] {
-#pragma unroll
-                for (int n = 0; n < NB; ++n) v[n] = *reinterpret_cast<const v4u*>(P.vt + at + n * 512);
-            };
+            // One memory round trip for all of K and V, where the registers allow; heads
+            // of 256 take V twice instead, for its magnitude and for the products.
+            constexpr bool KEEP = D < 256;
+            v4u k[2 * KS], v[KEEP ? NB : 1];
+            auto v_at = [&](int n) { return *reinterpret_cast<const v4u*>(P.vt + at + n * 512); };
 #pragma unroll
             for (int i = 0; i < 2 * KS; ++i) k[i] = *reinterpret_cast<const v4u*>(P.kt + at + i * 512);
-            if constexpr (D < 256) load_v();  // (one memory round trip, where the registers allow)
+            if constexpr (KEEP) {
+#pragma unroll
+                for (int n = 0; n < NB; ++n) v[n] = v_at(n);
+            }
             q8_f4 s[RW][2];
 #pragma unroll
             for (int w = 0; w < RW; ++w) s[w][0] = s[w][1] = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -340,7 +343,6 @@ struct Q8Wave {
                 for (int w = 0; w < RW; ++w)
                     s[w][i / KS] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q8_h8, k[i]), qf[w][i % KS],
                                                                           s[w][i / KS], 0, 0, 0);
-            if constexpr (D == 256) load_v();
             // (what lies behind the last row is not the cache's)
             v4u held;
 #pragma unroll
@@ -348,20 +350,24 @@ struct Q8Wave {
                 const int key = (u << 5) + (i >> 1) * 16 + 4 * hi + (i & 1) * 2;
                 held[i] = (key < P.len ? 0xFFFFu : 0u) | (key + 1 < P.len ? 0xFFFF0000u : 0u);
             }
-            unsigned big = 0;
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                v[n] &= held;
+            auto clean = [&](v4u x) {
+                x &= held;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    unsigned x = v[n][i];
-                    const unsigned wild0 = (x & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u;
-                    const unsigned wild1 = (x & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u;
+                    const unsigned wild0 = (x[i] & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u;
+                    const unsigned wild1 = (x[i] & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u;
                     wild |= wild0 | wild1;
-                    x &= ~(wild0 | wild1);
-                    v[n][i] = x;
-                    big = max(big, max(x & 0x7FFFu, (x >> 16) & 0x7FFFu));
+                    x[i] &= ~(wild0 | wild1);
                 }
+                return x;
+            };
+            unsigned big = 0;
+#pragma unroll(KEEP ? NB : 4)
+            for (int n = 0; n < NB; ++n) {
+                const v4u x = clean(KEEP ? v[KEEP ? n : 0] : v_at(n));
+                if constexpr (KEEP) v[n] = x;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) big = max(big, max(x[i] & 0x7FFFu, (x[i] >> 16) & 0x7FFFu));
             }
             const float top = wave_max(__half2float(__ushort_as_half((unsigned short)big)));
             const int e = top > 0.0f ? ((__float_as_int(top) >> 23) & 255) - 127 - 6 : -30;
@@ -374,7 +380,7 @@ struct Q8Wave {
             weigh(x, s, ph, pl);
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                q8_h8 a = __builtin_bit_cast(q8_h8, v[n]);
+                q8_h8 a = __builtin_bit_cast(q8_h8, KEEP ? v[KEEP ? n : 0] : clean(v_at(n)));
 #pragma unroll
                 for (int i = 0; i < 8; ++i) a[i] = (_Float16)((float)a[i] * up);
                 product(n, a, ph, pl);
@@ -386,12 +392,12 @@ struct Q8Wave {
             const __half* vt = P.vt + (size_t)g * P.block_values + (size_t)(u - coded_units) * (32 * D);
 #pragma unroll 1
             for (int j = 0; j < 32; ++j) {
-                const __half* at = vt + ((j >> 2) & 3) * 128 + hi * 32 + (j >> 4) * 4 + (j & 3);
+                const __half* at = vt + ((j >> 2) & 3) * 128 + (j >> 4) * 4 + (j & 3);  // (uniform)
 #pragma unroll
                 for (int n = 0; n < NB; ++n)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float x = __half2float(at[n * 512 + r * 8]);
+                        const float x = __half2float((at + n * 512 + r * 8)[(unsigned)hi * 32]);
                         const float y = fabsf(x) < INFINITY ? 0.0f : x;
 #pragma unroll
                         for (int w = 0; w < RW; ++w) o[w][n][r] += (u << 5) + j < lim[w] ? y : 0.0f;
@@ -521,13 +527,15 @@ __global__ __launch_bounds__(64 * NW) void attn_q8_kernel(AttnQ8Params P) {
     Q8Wave<D, RW, SPLIT> W;
     W.start(P, g, rt * RT, lo, hi);
     const int u_end = min(min((split + 1) * P.units_per_split, P.units), (W.seen + 31) >> 5);
+    const int coded_end = min(u_end, coded_units);
     int u = u_begin;
-    for (; u < min(u_end, coded_units); u += NW) {
+    for (; u < coded_end; u += NW) {
         q8_f4 s[RW][2];
 #pragma unroll
         for (int w = 0; w < RW; ++w) s[w][0] = s[w][1] = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
         const float4 x = next;
-        next = sc[min(u + NW, coded_units - 1) >> P.unit_shift];
+        const bool more = u + NW < coded_end;
+        if (more) next = sc[(u + NW) >> P.unit_shift];
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
             const int cb = i / (D / 64), st = i % (D / 64);
@@ -538,7 +546,7 @@ __global__ __launch_bounds__(64 * NW) void attn_q8_kernel(AttnQ8Params P) {
                 s[w][cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, W.qf[w][2 * st + 1], s[w][cb], 0, 0, 0);
             }
         }
-        load_k(u + NW);
+        if (more) load_k(u + NW);
         q8_h8 ph[RW], pl[RW];
         auto un = W.unit(c, x.x, x.y, __float_as_int(x.z), x.w);
         if (__builtin_expect(W.masked(u << 5, false), 0)) W.mask(un, u << 5, false, hi, s);  // (uniform)
@@ -550,7 +558,7 @@ __global__ __launch_bounds__(64 * NW) void attn_q8_kernel(AttnQ8Params P) {
             W.product(2 * i, q8_halves<FMT>(vr[i][0], vr[i][1]), ph, pl);
             W.product(2 * i + 1, q8_halves<FMT>(vr[i][2], vr[i][3]), ph, pl);
         }
-        load_v(u + NW);
+        if (more) load_v(u + NW);
     }
     W.tail(P, c, g, u, u_end, NW, lane);
 #pragma unroll

@@ -90,6 +90,8 @@ int rk_npu_hip_attention_q8_cache_get_info(const rk_npu_hip_attention_q8_cache* 
                                            rk_npu_attention_f16_cache_info* info);
 
 /* ---- host buffers: [heads][rows][head_dim] fp16 arrays, done on return ------
+ * Calls on one cache from several threads exclude each other, runs on workspaces
+ * of their own excepted; a workspace takes one run at a time (RK_NPU_ERR_BUSY).
  * load replaces the contents (rows == 0: empties the cache, k and v may be
  * NULL); append grows the cache as needed, up to max_capacity; read gives the
  * values of rows first..first + rows - 1 rounded to fp16; run and run_half are
@@ -109,13 +111,25 @@ int rk_npu_hip_attention_q8_run_half(rk_npu_ctx* ctx, rk_npu_attention_f16_works
 
 /* ---- device arrays, on the caller's stream (NULL: the null stream) -----------
  * The arrays lie in the memory of the cache's GPU (RK_NPU_ERR_PARAM otherwise);
- * nothing is synchronized and nothing allocated (append: reserve first). Calls
- * on one cache take effect in the order they are made, so they go to one
- * stream, or the caller orders their streams; runs that only read may overlap
- * on workspaces of their own. A captured call repeats its work on the rows and
- * positions it was captured with: a graph whose appends complete at most one
- * block each call, replayed before the cache moves on, writes the same
- * contents again; the host's length is that of the capture. */
+ * nothing is synchronized and nothing allocated (append: reserve first). An array
+ * that is written overlaps no other of the call. Calls on one cache take effect
+ * in the order they are made, so they go to one stream, or the caller orders
+ * their streams; runs and reads may overlap each other, runs on workspaces of
+ * their own.
+ *
+ * Under stream capture a call is recorded, and the length moves on, as if it had
+ * run: launch the graph before anything else uses what it writes. Each launch does
+ * what was recorded, at the recorded positions:
+ *   - a graph of reads and runs may be launched as long as the rows up to the
+ *     recorded length are the cache's, its storage has not grown, and no later
+ *     append has completed the block that was open (the run read its fp16 rows);
+ *   - a graph of appends may be launched again (with new rows in k and v, to the
+ *     same positions) until another append is made to the cache; several appends
+ *     to one cache in a graph complete one block of it at most, together;
+ *   - an append that continues from codes (after a truncation deeper than the rows
+ *     kept) is refused under capture: RK_NPU_ERR_UNSUPPORTED.
+ * Host-buffer calls wait for device calls made before them; for a graph's launch
+ * the caller waits. */
 int rk_npu_hip_attention_q8_device_append(rk_npu_hip_attention_q8_cache* cache, const rk_npu_hip_heads* k,
                                           const rk_npu_hip_heads* v, int32_t rows, void* stream);
 /* The values of rows first..first + rows - 1 (k or v may be NULL): f32 values,

@@ -71,13 +71,13 @@ class AttentionWork:
 
 
 def _run(backend, work: AttentionWork, cache_raw, q_heads: np.ndarray, m: int, position: int,
-         half: bool) -> np.ndarray:
-    """One rk_npu_attention_f16_run[_half] call on head-major fp16 bits."""
+         half: bool, run=None) -> np.ndarray:
+    """One rk_npu_attention_f16_run[_half] call (or `run`'s) on head-major fp16 bits."""
     cfg = work.config
     L = F.lib()
     out = np.empty((cfg.query_heads, m, cfg.head_dim), np.float16 if half else np.float32)
     q_heads = np.ascontiguousarray(q_heads, np.uint16)
-    run = L.rk_npu_attention_f16_run_half if half else L.rk_npu_attention_f16_run
+    run = run or (L.rk_npu_attention_f16_run_half if half else L.rk_npu_attention_f16_run)
     check(run(backend.ctx, work.workspace.raw, cache_raw, q_heads.ctypes.data, m, position,
               out.ctypes.data, None, None), "native GQA run")
     return out
@@ -133,8 +133,14 @@ class Attention:
         ensure(self.info().length == position, "native KV cache position mismatch")
         kb = np.ascontiguousarray(pack_half(k.reshape(rows, kh, d)).transpose(1, 0, 2))
         vb = np.ascontiguousarray(pack_half(v.reshape(rows, kh, d)).transpose(1, 0, 2))
-        check(F.lib().rk_npu_attention_f16_cache_append(self.backend.ctx, self.cache.raw, kb.ctypes.data,
-                                                        vb.ctypes.data, rows), "append native KV")
+        check(self._append_call(self.backend.ctx, self.cache.raw, kb.ctypes.data, vb.ctypes.data, rows),
+              "append native KV")
+
+    def _append_call(self, *args) -> int:
+        return F.lib().rk_npu_attention_f16_cache_append(*args)
+
+    def _run_call(self, *args) -> int:
+        return F.lib().rk_npu_attention_f16_run(*args)
 
     def run(self, q: np.ndarray, k: np.ndarray, v: np.ndarray, output: np.ndarray, rows: int,
             position: int) -> None:
@@ -155,7 +161,8 @@ class Attention:
             for offset in range(0, rows, step):
                 m = min(step, rows - offset)
                 qb = pack_half(q[offset * qh * d:(offset + m) * qh * d].reshape(m, qh, d)).transpose(1, 0, 2)
-                res = _run(self.backend, work, self.cache.raw, qb, m, position + offset, False)
+                res = _run(self.backend, work, self.cache.raw, qb, m, position + offset, False,
+                           self._run_call)
                 out[offset * qh * d:(offset + m) * qh * d] = res.transpose(1, 0, 2).reshape(-1)
 
 
@@ -204,6 +211,51 @@ class FullAttention:
         output_bits.reshape(-1)[:] = res.view(np.uint16).reshape(-1)
 
 
+class AttentionQ8(Attention):
+    """An Attention whose cache is held in 8 bits, one scale for each block of
+    tokens and KV head (rk_npu_attention_q8.h); no counterpart in the reference.
+    Same calls, same workspace; truncate is exact within the open block and the
+    last complete one."""
+
+    def info(self) -> F.rk_npu_attention_f16_cache_info:
+        info = F.rk_npu_attention_f16_cache_info()
+        check(F.lib().rk_npu_hip_attention_q8_cache_get_info(self.cache.raw, ctypes.byref(info)), "8-bit KV position")
+        return info
+
+    def truncate(self, length: int) -> None:
+        ensure(0 <= length <= 2 ** 31 - 1, "invalid 8-bit KV prefix length")
+        with self._lock:
+            check(F.lib().rk_npu_hip_attention_q8_cache_truncate(self.cache.raw, length), "truncate 8-bit KV cache")
+
+    def reset(self) -> None:
+        with self._lock:
+            check(F.lib().rk_npu_hip_attention_q8_cache_load(self.backend.ctx, self.cache.raw, None, None, 0),
+                  "reset 8-bit KV cache")
+
+    def reserve(self, capacity: int) -> None:
+        ensure(capacity <= self.backend.options.context, "8-bit KV context capacity exceeded")
+        with self._lock:
+            check(F.lib().rk_npu_hip_attention_q8_cache_reserve(self.backend.ctx, self.cache.raw, capacity),
+                  "reserve 8-bit KV cache")
+
+    def read(self, first: int, rows: int):
+        """The values of tokens first.., K and V, each [rows][kv_heads][head_dim] fp16."""
+        kh, d = self.kv_heads, self.dimension
+        ensure(rows > 0, "8-bit KV read of no rows")
+        out = [np.empty((kh, rows, d), np.float16) for _ in range(2)]
+        with self._lock:
+            check(F.lib().rk_npu_hip_attention_q8_cache_read(self.backend.ctx, self.cache.raw, first, rows,
+                                                             out[0].ctypes.data, out[1].ctypes.data),
+                  "read 8-bit KV cache")
+        return tuple(x.transpose(1, 0, 2) for x in out)
+
+    def _append_call(self, *args) -> int:
+        return F.lib().rk_npu_hip_attention_q8_cache_append(*args)
+
+    def _run_call(self, *args) -> int:
+        return F.lib().rk_npu_hip_attention_q8_run(*args)
+
+
 def create_cache(backend, config) -> _Handle:
     raw = ctypes.c_void_p()
     check(F.lib().rk_npu_attention_f16_cache_create(backend.domain, ctypes.byref(config), ctypes.byref(raw)),
@@ -211,9 +263,27 @@ def create_cache(backend, config) -> _Handle:
     return _Handle(raw.value, F.lib().rk_npu_attention_f16_cache_free, "KV cache", keep=backend._shared)
 
 
+KV_FORMATS = {"i8": F.RK_NPU_HIP_KV_I8, "e4m3": F.RK_NPU_HIP_KV_E4M3}
+
+
+def q8_config(attention, fmt: str, block: int) -> F.rk_npu_hip_attention_q8_config:
+    ensure(fmt in KV_FORMATS, f"KV format must be one of {sorted(KV_FORMATS)}")
+    cfg = F.rk_npu_hip_attention_q8_config()
+    F.lib().rk_npu_hip_attention_q8_config_init(ctypes.byref(cfg))
+    cfg.attention, cfg.format, cfg.block = attention, KV_FORMATS[fmt], block
+    return cfg
+
+
+def create_cache_q8(backend, config, fmt: str, block: int) -> _Handle:
+    raw = ctypes.c_void_p()
+    check(F.lib().rk_npu_hip_attention_q8_cache_create(
+        backend.domain, ctypes.byref(q8_config(config, fmt, block)), ctypes.byref(raw)), "create 8-bit KV cache")
+    return _Handle(raw.value, F.lib().rk_npu_hip_attention_q8_cache_free, "8-bit KV cache", keep=backend._shared)
+
+
 def attention_masked(backend, query_heads: int, kv_heads: int, dimension: int, softmax_scale: float,
-                     noncausal: bool) -> Attention:
-    """src/npu.rs:706-760."""
+                     noncausal: bool, q8=None) -> Attention:
+    """src/npu.rs:706-760. q8: (format, block) of an 8-bit cache instead of the fp16 one."""
     ensure(0 < kv_heads <= 32 and query_heads >= kv_heads and query_heads % kv_heads == 0 and dimension > 0 and
            dimension % 32 == 0 and math.isfinite(softmax_scale) and softmax_scale > 0.0,
            "native GQA requires Hq divisible by Hkv, Hkv within 1..32, D divisible by 32 and a positive softmax scale")
@@ -227,8 +297,8 @@ def attention_masked(backend, query_heads: int, kv_heads: int, dimension: int, s
         want = attention_config(backend.options, query_heads, kv_heads, dimension, softmax_scale)
         want.mask_mode = F.RK_NPU_ATTENTION_F16_NO_MASK if noncausal else F.RK_NPU_ATTENTION_F16_CAUSAL
         ensure(_same_geometry(cfg, want), "attention workspace geometry mismatch")
-        cache = create_cache(backend, cfg)
-    return Attention(backend, cache, query_heads, kv_heads, dimension)
+        cache = create_cache(backend, cfg) if q8 is None else create_cache_q8(backend, cfg, *q8)
+    return (Attention if q8 is None else AttentionQ8)(backend, cache, query_heads, kv_heads, dimension)
 
 
 def full_attention(backend, heads: int, dimension: int, rows: int) -> FullAttention:
@@ -242,14 +312,19 @@ def full_attention(backend, heads: int, dimension: int, rows: int) -> FullAttent
     return FullAttention(backend, create_cache(backend, cfg), work)
 
 
-def attention_cache_bytes(options, query_heads: int, kv_heads: int, dimension: int, softmax_scale: float) -> int:
-    """src/npu.rs:442-466."""
+def attention_cache_bytes(options, query_heads: int, kv_heads: int, dimension: int, softmax_scale: float,
+                          q8=None) -> int:
+    """src/npu.rs:442-466. q8: (format, block) of an 8-bit cache."""
     cfg = attention_config(options, query_heads, kv_heads, dimension, softmax_scale)
     sizes = F.rk_npu_attention_f16_sizes()
+    if q8 is not None:
+        check(F.lib().rk_npu_hip_attention_q8_query(ctypes.byref(q8_config(cfg, *q8)), cfg.max_capacity, 1,
+                                                    ctypes.byref(sizes)), "query 8-bit KV memory")
+        return sizes.key_bytes + sizes.value_bytes + sizes.tail_bytes
     check(F.lib().rk_npu_attention_f16_query(ctypes.byref(cfg), cfg.max_capacity, 1, cfg.max_capacity,
                                              ctypes.byref(sizes)), "query native KV memory")
     return sizes.key_bytes + sizes.value_bytes + sizes.tail_bytes
 
 
-__all__ = ["Attention", "FullAttention", "AttentionWork", "attention_config", "attention_masked",
+__all__ = ["Attention", "AttentionQ8", "FullAttention", "AttentionWork", "attention_config", "attention_masked",
            "full_attention", "attention_cache_bytes", "pack_half", "NpuError"]

@@ -10,6 +10,7 @@
 #include <cstring>
 #include <mutex>
 #include <new>
+#include <shared_mutex>
 
 #include "attention.hpp"
 #pragma clang diagnostic push
@@ -366,11 +367,11 @@ struct Q8Rows {
     int block[Q8_SLOTS] = {-1, -1, -1};  // the token block a slot holds the first `rows` rows of
     int rows[Q8_SLOTS] = {0, 0, 0};
 
-    // A slot to write, none of a, b: an empty one, else that of the earliest block.
-    int pick(int a, int b) const {
+    // A slot to write, none of a, b, c: an empty one, else that of the earliest block.
+    int pick(int a, int b, int c) const {
         int best = -1;
         for (int i = 0; i < Q8_SLOTS; ++i)
-            if (i != a && i != b && (best < 0 || block[i] < block[best])) best = i;
+            if (i != a && i != b && i != c && (best < 0 || block[i] < block[best])) best = i;
         return best;
     }
     void forget_from(int b) {  // blocks b and later
@@ -397,30 +398,35 @@ struct Q8Rows {
 // last complete and the new open block go to (-1: none), the bookkeeping after.
 // Kept then: these three. The old rows' slot is written only after them, so the
 // call can be undone, and a captured one repeated.
+// A call in several pieces, all but the last of which end with a block, leaves the
+// rows it began with where they are, and its last complete block: slots `begun` and
+// `done` (-1: none). Pieces behind the first have no old rows, so there is a slot for
+// each of last and open.
 struct Q8Step {
     int from, last, open;
     Q8Rows after;
 };
-static Q8Step q8_step(const Q8Rows& now, int B, int n) {
+static Q8Step q8_step(const Q8Rows& now, int B, int n, int begun, int done) {
     Q8Step s{now.open, -1, -1, now};
     Q8Rows& a = s.after;
     a.length = now.length + n;
     const int b0 = now.length / B, b1 = a.length / B, r = a.length % B;
     if (now.open < 0) a.forget_from(b0);  // (rows of a block that is rewritten from its codes)
     if (b1 > b0) {
-        s.last = b1 - 1 == b0 && s.from >= 0 ? s.from : a.pick(s.from, -1);
+        s.last = b1 - 1 == b0 && s.from >= 0 ? s.from : a.pick(s.from, begun, -1);
+        done = s.last;
         a.block[s.last] = b1 - 1;
         a.rows[s.last] = B;
     }
     if (r > 0) {
-        s.open = b1 == b0 && s.from >= 0 ? s.from : a.pick(s.from, s.last);
+        s.open = b1 == b0 && s.from >= 0 ? s.from : a.pick(s.from, begun, done);
         a.block[s.open] = b1;
         a.rows[s.open] = r;
     }
     a.open = s.open;
     a.coded = b1 * B;
     for (int i = 0; i < Q8_SLOTS; ++i)
-        if (i != s.from && i != s.last && i != s.open) a.block[i] = -1, a.rows[i] = 0;
+        if (i != s.from && i != s.open && i != begun && i != done) a.block[i] = -1, a.rows[i] = 0;
     return s;
 }
 
@@ -435,7 +441,7 @@ struct Q8Cache {
     size_t code_bytes, scale_bytes, kept_bytes;  // of one array each
     uint64_t generation;
     Q8Rows rows;
-    std::mutex mu;   // the fields above against calls from several threads
+    std::shared_mutex mu;  // the fields above against calls from several threads; a host run holds it (shared) to its end
     DevFence fence;  // device-path appends, reads and runs
     hipStream_t stream = nullptr;  // host-buffer appends and reads (created on the first)
     HostStage hs;                  // their pinned staging
@@ -571,9 +577,10 @@ static void q8_launch_write(const Q8WriteParams& P, int D, int B, const dim3& gr
 }
 
 // Enqueues an append (room and views checked) and advances the bookkeeping.
-static int q8_enqueue_append(Q8Cache* c, const HeadsView& k, const HeadsView& v, int n, hipStream_t s) {
+static int q8_enqueue_append(Q8Cache* c, const HeadsView& k, const HeadsView& v, int n, hipStream_t s,
+                             int begun = -1, int* done = nullptr) {
     const int B = c->cfg.block, D = c->cfg.attention.head_dim;
-    const Q8Step st = q8_step(c->rows, B, n);
+    const Q8Step st = q8_step(c->rows, B, n, begun, done ? *done : -1);
     Q8WriteParams P;
     P.src[0] = k;
     P.src[1] = v;
@@ -596,6 +603,7 @@ static int q8_enqueue_append(Q8Cache* c, const HeadsView& k, const HeadsView& v,
         q8_launch_write<RK_NPU_HIP_KV_E4M3>(P, D, B, grid, s);
     if (hipGetLastError() != hipSuccess) return RK_NPU_ERR_DEVICE;
     c->rows = st.after;
+    if (done && st.last >= 0) *done = st.last;
     return RK_NPU_OK;
 }
 
@@ -754,9 +762,11 @@ static int q8_put_host(Q8Cache* c, const uint16_t* k, const uint16_t* v, int row
     const size_t each = (size_t)kh * step * D;
     uint16_t* st = static_cast<uint16_t*>(q8_stage(c, 2 * each * sizeof(uint16_t)));
     if (!st) return RK_NPU_ERR_NOMEM;
-    const int start = c->rows.length;
-    for (int r = 0; r < rows; r += step) {
-        const int n = std::min(step, rows - r);
+    const int start = c->rows.length, begun = c->rows.open;
+    int done = -1;
+    for (int r = 0, n; r < rows; r += n) {
+        n = std::min(step, rows - r);
+        if (r + n < rows) n -= (start + r + n) % c->cfg.block;  // (step is at least 256: the stage holds them)
         for (int g = 0; g < kh; ++g) {
             const size_t at = ((size_t)g * rows + r) * D, to = (size_t)g * n * D;
             std::memcpy(st + to, k + at, (size_t)n * D * sizeof(uint16_t));
@@ -764,7 +774,7 @@ static int q8_put_host(Q8Cache* c, const uint16_t* k, const uint16_t* v, int row
         }
         uint16_t* dev = static_cast<uint16_t*>(c->hs.dev);
         int rc = q8_enqueue_append(c, HeadsView{dev, 0, (long long)n * D, D},
-                                   HeadsView{dev + each, 0, (long long)n * D, D}, n, c->stream);
+                                   HeadsView{dev + each, 0, (long long)n * D, D}, n, c->stream, begun, &done);
         if (rc == RK_NPU_OK && !q8_stage_done(c, st)) rc = RK_NPU_ERR_DEVICE;
         if (rc != RK_NPU_OK) {
             c->rows.truncate(c->cfg.block, start);  // (nothing of a failed call stays)
@@ -785,6 +795,7 @@ static int q8_run_host(rk_npu_attention_f16_workspace* workspace, rk_npu_hip_att
     if (!busy.ok) return RK_NPU_ERR_BUSY;
     DeviceGuard dev(device_of(w->domain));
     if (!dev.ok) return RK_NPU_ERR_DEVICE;
+    std::shared_lock<std::shared_mutex> lock(c->mu);
     const double t0 = now_us();
     const int D = c->cfg.attention.head_dim;
     const size_t n = (size_t)c->cfg.attention.query_heads * rows * D;
@@ -797,11 +808,9 @@ static int q8_run_host(rk_npu_attention_f16_workspace* workspace, rk_npu_hip_att
     if (!stage_upload(w->hs, small, st, &seg, 1, w->stream) || (t && hipStreamSynchronize(w->stream) != hipSuccess))
         rc = RK_NPU_ERR_DEVICE;
     const double t1 = now_us();
-    if (rc == RK_NPU_OK) {
-        std::lock_guard<std::mutex> lock(c->mu);
+    if (rc == RK_NPU_OK)
         rc = q8_enqueue_run(w, c, HeadsView{w->q, 0, (long long)rows * D, D}, rows, pos,
                             HeadsView{w->out, out_f16 ? 0 : 1, (long long)rows * D, D}, w->stream);
-    }
     if (rc == RK_NPU_OK && t && hipStreamSynchronize(w->stream) != hipSuccess) rc = RK_NPU_ERR_DEVICE;
     const double t2 = now_us();
     if (rc == RK_NPU_OK && !stage_download(w->hs, small, st, out, w->out, ob, w->stream)) rc = RK_NPU_ERR_DEVICE;
@@ -896,7 +905,7 @@ void rk_npu_hip_attention_q8_cache_free(rk_npu_hip_attention_q8_cache* cache) {
 int rk_npu_hip_attention_q8_cache_reserve(rk_npu_ctx* ctx, rk_npu_hip_attention_q8_cache* cache, int32_t capacity) {
     Q8Cache* c = as_q8(cache);
     if (!ctx || !c || capacity < 0) return RK_NPU_ERR_PARAM;
-    std::lock_guard<std::mutex> lock(c->mu);
+    std::lock_guard<std::shared_mutex> lock(c->mu);
     DeviceGuard dev(device_of(c->domain));
     if (!dev.ok || c->fence.wait(nullptr) != hipSuccess) return RK_NPU_ERR_DEVICE;
     return q8_grow(c, capacity);
@@ -905,7 +914,7 @@ int rk_npu_hip_attention_q8_cache_reserve(rk_npu_ctx* ctx, rk_npu_hip_attention_
 int rk_npu_hip_attention_q8_cache_truncate(rk_npu_hip_attention_q8_cache* cache, int32_t length) {
     Q8Cache* c = as_q8(cache);
     if (!c) return RK_NPU_ERR_PARAM;
-    std::lock_guard<std::mutex> lock(c->mu);
+    std::lock_guard<std::shared_mutex> lock(c->mu);
     if (length < 0 || length > c->rows.length) return RK_NPU_ERR_PARAM;
     if (length < c->rows.length) c->rows.truncate(c->cfg.block, length);
     return RK_NPU_OK;
@@ -915,7 +924,7 @@ int rk_npu_hip_attention_q8_cache_get_info(const rk_npu_hip_attention_q8_cache* 
                                            rk_npu_attention_f16_cache_info* info) {
     Q8Cache* c = as_q8(cache);
     if (!c || !info) return RK_NPU_ERR_PARAM;
-    std::lock_guard<std::mutex> lock(c->mu);
+    std::shared_lock<std::shared_mutex> lock(c->mu);
     info->length = c->rows.length;
     info->capacity = c->capacity;
     info->max_capacity = q8_max_capacity(c);
@@ -929,7 +938,7 @@ int rk_npu_hip_attention_q8_cache_load(rk_npu_ctx* ctx, rk_npu_hip_attention_q8_
                                        const uint16_t* v, int32_t rows) {
     Q8Cache* c = as_q8(cache);
     if (!ctx || !c || rows < 0 || (rows > 0 && (!k || !v))) return RK_NPU_ERR_PARAM;
-    std::lock_guard<std::mutex> lock(c->mu);
+    std::lock_guard<std::shared_mutex> lock(c->mu);
     if (rows > q8_max_capacity(c)) return RK_NPU_ERR_PARAM;
     DeviceGuard dev(device_of(c->domain));
     if (!dev.ok || c->fence.wait(nullptr) != hipSuccess) return RK_NPU_ERR_DEVICE;
@@ -944,7 +953,7 @@ int rk_npu_hip_attention_q8_cache_append(rk_npu_ctx* ctx, rk_npu_hip_attention_q
                                          const uint16_t* v, int32_t rows) {
     Q8Cache* c = as_q8(cache);
     if (!ctx || !c || rows < 1 || !k || !v) return RK_NPU_ERR_PARAM;
-    std::lock_guard<std::mutex> lock(c->mu);
+    std::lock_guard<std::shared_mutex> lock(c->mu);
     const int most = q8_max_capacity(c);
     if (rows > most - c->rows.length) return RK_NPU_ERR_PARAM;
     DeviceGuard dev(device_of(c->domain));
@@ -961,7 +970,7 @@ int rk_npu_hip_attention_q8_cache_read(rk_npu_ctx* ctx, rk_npu_hip_attention_q8_
                                        int32_t rows, uint16_t* k, uint16_t* v) {
     Q8Cache* c = as_q8(cache);
     if (!ctx || !c || first < 0 || rows < 1 || !k || !v) return RK_NPU_ERR_PARAM;
-    std::lock_guard<std::mutex> lock(c->mu);
+    std::lock_guard<std::shared_mutex> lock(c->mu);
     if (first > c->rows.length - rows) return RK_NPU_ERR_PARAM;
     DeviceGuard dev(device_of(c->domain));
     if (!dev.ok || c->fence.wait(nullptr) != hipSuccess) return RK_NPU_ERR_DEVICE;
@@ -1006,10 +1015,19 @@ int rk_npu_hip_attention_q8_device_append(rk_npu_hip_attention_q8_cache* cache, 
     const int device = device_of(c->domain), kh = c->cfg.attention.kv_heads, D = c->cfg.attention.head_dim;
     if (!valid_heads(k, device, D, false, kh, rows) || !valid_heads(v, device, D, false, kh, rows))
         return RK_NPU_ERR_PARAM;
-    std::lock_guard<std::mutex> lock(c->mu);
+    std::lock_guard<std::shared_mutex> lock(c->mu);
     if (rows > c->capacity - c->rows.length) return RK_NPU_ERR_PARAM;  // (reserve first: no allocation here)
     DeviceGuard dev(device);
     if (!dev.ok) return RK_NPU_ERR_DEVICE;
+    if (c->rows.open < 0 && c->rows.length % c->cfg.block) {
+        // Continues from codes, which it replaces: a captured one could not be repeated.
+        hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(static_cast<hipStream_t>(stream), &st) != hipSuccess ||
+            st != hipStreamCaptureStatusNone) {
+            (void)hipGetLastError();
+            return RK_NPU_ERR_UNSUPPORTED;
+        }
+    }
     const int rc = q8_enqueue_append(c, view_of(*k), view_of(*v), rows, static_cast<hipStream_t>(stream));
     if (rc == RK_NPU_OK) c->fence.note(static_cast<hipStream_t>(stream));
     return rc;
@@ -1022,7 +1040,7 @@ int rk_npu_hip_attention_q8_device_read(rk_npu_hip_attention_q8_cache* cache, in
     const int device = device_of(c->domain), kh = c->cfg.attention.kv_heads, D = c->cfg.attention.head_dim;
     if ((k && !valid_heads(k, device, D, true, kh, rows)) || (v && !valid_heads(v, device, D, true, kh, rows)))
         return RK_NPU_ERR_PARAM;
-    std::lock_guard<std::mutex> lock(c->mu);
+    std::lock_guard<std::shared_mutex> lock(c->mu);
     if (first > c->rows.length - rows) return RK_NPU_ERR_PARAM;
     DeviceGuard dev(device);
     if (!dev.ok) return RK_NPU_ERR_DEVICE;
@@ -1042,7 +1060,7 @@ int rk_npu_hip_attention_q8_device_run(rk_npu_attention_f16_workspace* workspace
     const int device = device_of(c->domain), qh = c->cfg.attention.query_heads, D = c->cfg.attention.head_dim;
     if (!valid_heads(q, device, D, false, qh, rows) || !valid_heads(out, device, D, true, qh, rows))
         return RK_NPU_ERR_PARAM;
-    std::lock_guard<std::mutex> lock(c->mu);
+    std::shared_lock<std::shared_mutex> lock(c->mu);
     DeviceGuard dev(device);
     if (!dev.ok) return RK_NPU_ERR_DEVICE;
     const int rc = q8_enqueue_run(w, c, view_of(*q), rows, position, view_of(*out), static_cast<hipStream_t>(stream));

@@ -10,6 +10,7 @@ import ctypes
 from typing import Dict, List, Optional, Tuple
 
 from . import _ffi as F
+from .attention import KV_FORMATS
 from .npu import NpuError, _Handle, _Shared, check, ensure
 
 _DT = {}
@@ -117,18 +118,21 @@ class DeviceContext:
                                         L.rk_npu_matmul_workspace_free, "W8 workspace", self.shared)
         return self._ws[key]
 
-    def attention_workspace(self, cache: "KvCacheQ8") -> _Handle:
+    def attention_workspace(self, cache: "KvCacheQ8", own: bool = False) -> _Handle:
         """The context's attention workspace for the cache's geometry, created on
-        first use (rk_npu_attention_f16_prepare)."""
+        first use (rk_npu_attention_f16_prepare); own: a new one, for calls that
+        overlap others (a second stream, graphs launched side by side)."""
         c = cache.config.attention
         key = ("attention", c.query_heads, c.kv_heads, c.head_dim, c.softmax_scale, c.mask_mode, c.max_query_rows)
-        if key not in self._ws:
-            raw = ctypes.c_void_p()
-            check(F.lib().rk_npu_attention_f16_prepare(self.domain, ctypes.byref(c), ctypes.byref(raw)),
-                  "prepare attention")
-            self._ws[key] = _Handle(raw.value, F.lib().rk_npu_attention_f16_workspace_free, "attention workspace",
-                                    self.shared)
-        return self._ws[key]
+        if not own and key in self._ws:
+            return self._ws[key]
+        raw = ctypes.c_void_p()
+        check(F.lib().rk_npu_attention_f16_prepare(self.domain, ctypes.byref(c), ctypes.byref(raw)),
+              "prepare attention")
+        ws = _Handle(raw.value, F.lib().rk_npu_attention_f16_workspace_free, "attention workspace", self.shared)
+        if not own:
+            self._ws[key] = ws
+        return ws
 
 
 class DeviceWeights:
@@ -164,9 +168,6 @@ def _stream(stream, t):
     object takes 2 us to make, a third of a call that reads a short cache)."""
     import torch
     return stream if stream is not None else torch._C._cuda_getCurrentRawStream(t.get_device())
-
-
-KV_FORMATS = {"i8": F.RK_NPU_HIP_KV_I8, "e4m3": F.RK_NPU_HIP_KV_E4M3}
 
 
 class KvCacheQ8:
@@ -244,7 +245,9 @@ def _heads(t, heads: int, head_dim: int) -> F.rk_npu_hip_heads:
 
 
 def attention_q8(ctx: DeviceContext, cache: KvCacheQ8, q, out, position: int, ws=None, stream=None):
-    """Attention of the rows q [query_heads][rows][head_dim], the first at `position`, over the cache's tokens."""
+    """Attention of the rows q [query_heads][rows][head_dim], the first at
+    `position`, over the cache's tokens. ws: the context's workspace of this
+    geometry, which calls on one stream share."""
     c = cache.config.attention
     ensure(q.shape == out.shape, "q and out must have the same shape")
     ws = ws or ctx.attention_workspace(cache)

@@ -189,14 +189,24 @@ class Backend:
         from . import attention as A
         return A.attention_masked(self, query_heads, kv_heads, dimension, 1.0 / math.sqrt(dimension), True)
 
+    def attention_q8(self, query_heads: int, kv_heads: int, dimension: int, softmax_scale: float,
+                     fmt: str = "i8", block: int = 32, noncausal: bool = False):
+        """A GQA KV cache held in 8 bits (rk_npu_attention_q8.h): fmt "i8" or "e4m3",
+        one scale for each `block` tokens (32, 64 or 128) and KV head. Shares the
+        backend's attention workspace, so its geometry and mask."""
+        from . import attention as A
+        return A.attention_masked(self, query_heads, kv_heads, dimension, softmax_scale, noncausal, (fmt, block))
+
     def full_attention(self, heads: int, dimension: int, rows: int):
         from . import attention as A
         return A.full_attention(self, heads, dimension, rows)
 
     @staticmethod
-    def attention_cache_bytes(options, query_heads: int, kv_heads: int, dimension: int, softmax_scale: float) -> int:
+    def attention_cache_bytes(options, query_heads: int, kv_heads: int, dimension: int, softmax_scale: float,
+                              q8=None) -> int:
+        """q8: (format, block) of an 8-bit cache."""
         from . import attention as A
-        return A.attention_cache_bytes(options, query_heads, kv_heads, dimension, softmax_scale)
+        return A.attention_cache_bytes(options, query_heads, kv_heads, dimension, softmax_scale, q8)
 
     @property
     def domain(self):

@@ -665,15 +665,22 @@ static bool q8_tile(int D, int R, int kv_heads, int units) {
 // partials: 256 blocks of many rows (512 rows of 8 heads over 4096 keys 21.9 us, 27.6
 // with 512), 128 where a KV head has at most 32, whose blocks are 8 waves that only
 // load (8 rows of 8 heads of 256 over 16001 keys 19.3 us, 20.6 with 256 and 28.2 with
-// 512). A split holds at least a unit for each wave, or two stages.
+// 512). A split holds at least a unit for each wave, or two stages. Few keys are not
+// split: a wave walks its 3 to 5 units in the time of the join's launch, 3 us. One and
+// 16 rows of 32 heads over 8 of 128: 768 keys 6.4 and 8.7 us, split 7.9 and 9.9, 1000
+// keys 8.1 and 11.1, split 8.3 and 11.0; one of 16 over 8 of 64: 1000 keys 6.9, split
+// 8.2, 1500 keys 8.1 and 8.3; one of 16 over 2 of 256: 480 keys 7.8, split 9.3, 768 keys
+// 9.4 and 9.4, 1000 keys 13.3, split 11.0.
 static void q8_splits(AttnQ8Params& P, int D, int R, bool tile) {
     const int rows = q8_block_rows(D, R, tile);
     P.row_tiles = (R + rows - 1) / rows;
     P.rows_pad = P.row_tiles * rows;
     const int base = P.row_tiles * P.kh, least = tile ? 4 : Q8_WAVES, blocks = R > 32 ? 256 : 128;
+    const int few = D == 64 ? 40 : D == 128 ? 32 : 24;
     const size_t room = attn_partial_rows(D) / ((size_t)P.rows_pad * P.kh);
     int want = std::max(1, std::min((blocks + base - 1) / base, (P.units + least - 1) / least));
     want = (int)std::min<size_t>(want, std::max<size_t>(1, room));
+    if (P.units <= few) want = 1;
     P.units_per_split = ((P.units + want - 1) / want + least - 1) / least * least;
     P.splits = (P.units + P.units_per_split - 1) / P.units_per_split;
 }

@@ -182,8 +182,6 @@ struct Q8Wave {
             }
             mrun[w] = Q8_NONE;
             lsum[w] = 0.0f;
-#pragma unroll
-            for (int n = 0; n < NB; ++n) o[w][n] = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
         }
         if (!P.q_f32) {
 #pragma unroll
@@ -209,6 +207,14 @@ struct Q8Wave {
         }
         open = __builtin_amdgcn_readfirstlane(q8_row_min(open));
         seen = -__builtin_amdgcn_readfirstlane(q8_row_min(-seen));
+    }
+
+    // The accumulators: after start(), or by tail<FIRST>.
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int w = 0; w < RW; ++w)
+#pragma unroll
+            for (int n = 0; n < NB; ++n) o[w][n] = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
     // What a unit's weights take from its scales. Without SPLIT, e + log2(mu) goes
@@ -258,6 +264,7 @@ struct Q8Wave {
         }
         return any;
     }
+    template <bool FIRST = false>
     __device__ __forceinline__ void raise(const float (&top)[RW]) {
 #pragma unroll
         for (int w = 0; w < RW; ++w) {
@@ -268,6 +275,7 @@ struct Q8Wave {
                 alpha = __builtin_amdgcn_exp2f(mrun[w] - tm);
                 mrun[w] = tm;
             }
+            if constexpr (FIRST) continue;
             lsum[w] *= alpha;
 #pragma unroll
             for (int n = 0; n < NB; ++n) o[w][n] *= alpha;
@@ -312,83 +320,85 @@ struct Q8Wave {
         }
     }
 
-    // Units u, u + step, .. below u_end, all of the tail: fp16 rows in the codes'
-    // order. What is not finite in V stays out of the products (0 times it is NaN,
-    // so masked keys would show); V's exponents move so that its largest magnitude
-    // lies near the codes'. Then `wild` units add it to the rows that see it, after
-    // the last change of a maximum (whatever the weights, which are positive).
-    __device__ __forceinline__ void tail(const AttnQ8Params& P, float c, int g, int u, int u_end, int step, int lane) {
-        const int hi = lane >> 4, coded_units = P.coded >> 5, u0 = u;
+    // Unit u, one of the tail: fp16 rows in the codes' order. What is not finite in V
+    // stays out of the products (0 times it is NaN, so masked keys would show); V's
+    // exponents move so that its largest magnitude lies near the codes'. Returns
+    // whether there is such a value: wild() then adds them to the rows that see them,
+    // after the last change of a maximum (whatever the weights, which are positive).
+    // FIRST: nothing came before, not clear() either. KEEP: one memory round trip for
+    // all of K and V; heads of 256 whose accumulators are in use have no registers for
+    // it and take V twice, a part at a time, for its magnitude and for the products.
+    template <bool FIRST, bool KEEP>
+    __device__ __forceinline__ bool tail(const AttnQ8Params& P, float c, int g, int u, int lane) {
+        const int hi = lane >> 4;
         unsigned wild = 0;
-#pragma unroll 1
-        for (; u < u_end; u += step) {
-            const size_t at = (size_t)g * P.block_values + (size_t)(u - coded_units) * (32 * D) + lane * 8;
-            // One memory round trip for all of K and V, where the registers allow; heads
-            // of 256 take V twice instead, for its magnitude and for the products.
-            constexpr bool KEEP = D < 256;
-            v4u k[2 * KS], v[KEEP ? NB : 1];
-            auto v_at = [&](int n) { return *reinterpret_cast<const v4u*>(P.vt + at + n * 512); };
+        const size_t at = (size_t)g * P.block_values + (size_t)(u - (P.coded >> 5)) * (32 * D) + lane * 8;
+        v4u k[2 * KS], v[KEEP ? NB : 1];
+        auto v_at = [&](int n) { return *reinterpret_cast<const v4u*>(P.vt + at + n * 512); };
 #pragma unroll
-            for (int i = 0; i < 2 * KS; ++i) k[i] = *reinterpret_cast<const v4u*>(P.kt + at + i * 512);
-            if constexpr (KEEP) {
+        for (int i = 0; i < 2 * KS; ++i) k[i] = *reinterpret_cast<const v4u*>(P.kt + at + i * 512);
+        if constexpr (KEEP) {
 #pragma unroll
-                for (int n = 0; n < NB; ++n) v[n] = v_at(n);
-            }
-            q8_f4 s[RW][2];
+            for (int n = 0; n < NB; ++n) v[n] = v_at(n);
+        }
+        q8_f4 s[RW][2];
 #pragma unroll
-            for (int w = 0; w < RW; ++w) s[w][0] = s[w][1] = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int w = 0; w < RW; ++w) s[w][0] = s[w][1] = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < 2 * KS; ++i)
+        for (int i = 0; i < 2 * KS; ++i)
 #pragma unroll
-                for (int w = 0; w < RW; ++w)
-                    s[w][i / KS] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q8_h8, k[i]), qf[w][i % KS],
-                                                                          s[w][i / KS], 0, 0, 0);
-            // (what lies behind the last row is not the cache's)
-            v4u held;
+            for (int w = 0; w < RW; ++w)
+                s[w][i / KS] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q8_h8, k[i]), qf[w][i % KS],
+                                                                      s[w][i / KS], 0, 0, 0);
+        // (what lies behind the last row is not the cache's)
+        v4u held;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int key = (u << 5) + (i >> 1) * 16 + 4 * hi + (i & 1) * 2;
+            held[i] = (key < P.len ? 0xFFFFu : 0u) | (key + 1 < P.len ? 0xFFFF0000u : 0u);
+        }
+        auto clean = [&](v4u x) {
+            x &= held;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int key = (u << 5) + (i >> 1) * 16 + 4 * hi + (i & 1) * 2;
-                held[i] = (key < P.len ? 0xFFFFu : 0u) | (key + 1 < P.len ? 0xFFFF0000u : 0u);
+                const unsigned wild0 = (x[i] & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u;
+                const unsigned wild1 = (x[i] & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u;
+                wild |= wild0 | wild1;
+                x[i] &= ~(wild0 | wild1);
             }
-            auto clean = [&](v4u x) {
-                x &= held;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const unsigned wild0 = (x[i] & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u;
-                    const unsigned wild1 = (x[i] & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u;
-                    wild |= wild0 | wild1;
-                    x[i] &= ~(wild0 | wild1);
-                }
-                return x;
-            };
-            unsigned big = 0;
+            return x;
+        };
+        unsigned big = 0;
 #pragma unroll(KEEP ? NB : 4)
-            for (int n = 0; n < NB; ++n) {
-                const v4u x = clean(KEEP ? v[KEEP ? n : 0] : v_at(n));
-                if constexpr (KEEP) v[n] = x;
+        for (int n = 0; n < NB; ++n) {
+            const v4u x = clean(KEEP ? v[KEEP ? n : 0] : v_at(n));
+            if constexpr (KEEP) v[n] = x;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) big = max(big, max(x[i] & 0x7FFFu, (x[i] >> 16) & 0x7FFFu));
-            }
-            const float top = wave_max(__half2float(__ushort_as_half((unsigned short)big)));
-            const int e = top > 0.0f ? ((__float_as_int(top) >> 23) & 255) - 127 - 6 : -30;
-            const float up = __int_as_float((127 - e) << 23);
-            q8_h8 ph[RW], pl[RW];
-            Unit x = unit(c, 1.0f, 1.0f, e, up);
-            if (masked(u << 5, false)) mask(x, u << 5, false, hi, s);  // (uniform)
-            float top1[RW];
-            if (__builtin_amdgcn_ballot_w64(over(x, s, top1)) != 0) raise(top1);
-            weigh(x, s, ph, pl);
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                q8_h8 a = __builtin_bit_cast(q8_h8, KEEP ? v[KEEP ? n : 0] : clean(v_at(n)));
-#pragma unroll
-                for (int i = 0; i < 8; ++i) a[i] = (_Float16)((float)a[i] * up);
-                product(n, a, ph, pl);
-            }
+            for (int i = 0; i < 4; ++i) big = max(big, max(x[i] & 0x7FFFu, (x[i] >> 16) & 0x7FFFu));
         }
-        if (__builtin_amdgcn_ballot_w64(wild != 0) == 0) return;
+        const float top = wave_max(__half2float(__ushort_as_half((unsigned short)big)));
+        const int e = top > 0.0f ? ((__float_as_int(top) >> 23) & 255) - 127 - 6 : -30;
+        const float up = __int_as_float((127 - e) << 23);
+        q8_h8 ph[RW], pl[RW];
+        Unit x = unit(c, 1.0f, 1.0f, e, up);
+        if (masked(u << 5, false)) mask(x, u << 5, false, hi, s);  // (uniform)
+        float top1[RW];
+        if (__builtin_amdgcn_ballot_w64(over(x, s, top1)) != 0) raise<FIRST>(top1);
+        weigh(x, s, ph, pl);
+        if constexpr (FIRST) clear();
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            q8_h8 a = __builtin_bit_cast(q8_h8, KEEP ? v[KEEP ? n : 0] : clean(v_at(n)));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a[i] = (_Float16)((float)a[i] * up);
+            product(n, a, ph, pl);
+        }
+        return __builtin_amdgcn_ballot_w64(wild != 0) != 0;
+    }
+    __device__ __forceinline__ void wild(const AttnQ8Params& P, int g, int u, int u_end, int lane) {
+        const int hi = lane >> 4, coded_units = P.coded >> 5;
 #pragma unroll 1
-        for (u = u0; u < u_end; u += step) {
+        for (; u < u_end; ++u) {
             const __half* vt = P.vt + (size_t)g * P.block_values + (size_t)(u - coded_units) * (32 * D);
 #pragma unroll 1
             for (int j = 0; j < 32; ++j) {
@@ -482,10 +492,12 @@ __device__ __forceinline__ void q8_meet(const AttnQ8Params& P, const Q8Wave<D, R
 // converted.
 //
 // Measured, the join included: one row of 32 heads over 8 of 128 and 131072 keys
-// (268 MB) e4m3 46.5 us, i8 48: 5.8 and 5.6 TB/s (a large copy reads and writes
-// 4.9). Over 3968 keys (8 MB) 8.0: there it is latency, a unit's load to its
-// products, the waves' meeting and the join's launch. 512 rows over 4096 keys 21.9:
-// conversion and softmax, vector instructions that every 32 rows repeat. The splits
+// (268 MB) e4m3 46.7 us, i8 50: 5.7 and 5.4 TB/s (a large copy reads and writes
+// 4.9). Over 3968 keys (8 MB) 8.1: there it is latency, a unit's load to its
+// products, the waves' meeting and the join's launch. 512 rows over 4096 keys 21.3:
+// conversion and softmax, vector instructions that every 32 rows repeat. The tail
+// after the coded units, its loads a round trip of their own: one row of 16 heads over
+// 2 of 256, 1000 keys 12.2 instead of 11.0; of 32 over 8 of 128, 3981 keys 8.8 and 8.5. The splits
 // joined by their last block, in the same launch, lost to a launch of their own (8.6):
 // 10.0 with the partials through atomics of agent scope, 30 behind a fence, which
 // writes the L2 back. Blocks of 2 or 4 groups of waves with keys of their own and
@@ -507,29 +519,40 @@ __global__ __launch_bounds__(64 * NW) void attn_q8_kernel(AttnQ8Params P) {
     const int u_begin = split * P.units_per_split + wave;
 
     v4u kr[KP], vr[KP];
-    // (the last coded unit's own codes again where there is no further one)
     auto load_k = [&](int u) {
-        const uint8_t* p = kbase + (size_t)min(u, coded_units - 1) * (32 * D);
+        const uint8_t* p = kbase + (size_t)u * (32 * D);
 #pragma unroll
         for (int i = 0; i < KP; ++i) kr[i] = *reinterpret_cast<const v4u*>(p + i * 1024);
     };
     auto load_v = [&](int u) {
-        const uint8_t* p = vbase + (size_t)min(u, coded_units - 1) * (32 * D);
+        const uint8_t* p = vbase + (size_t)u * (32 * D);
 #pragma unroll
         for (int i = 0; i < KP; ++i) vr[i] = *reinterpret_cast<const v4u*>(p + i * 1024);
     };
     float4 next = float4{1.0f, 1.0f, 0.0f, 1.0f};  // the next unit's scales
-    if (coded_units > 0) {
-        next = sc[min(u_begin, coded_units - 1) >> P.unit_shift];
+    auto first = [&] {
+        if (u_begin >= coded_units) return;
+        next = sc[u_begin >> P.unit_shift];
         load_k(u_begin);
         load_v(u_begin);
-    }
+    };
+    // A wave has one unit of the tail at most (4 units, NW waves). It comes first: its
+    // loads and those of the first coded unit are one memory round trip, for which
+    // heads of 256 have no registers.
+    const int u_tail = u_begin + (max(coded_units - u_begin, 0) + NW - 1) / NW * NW;
+    const bool late = D == 256 && u_tail < min((split + 1) * P.units_per_split, P.units);
+    if (!late) first();
     Q8Wave<D, RW, SPLIT> W;
     W.start(P, g, rt * RT, lo, hi);
     const int u_end = min(min((split + 1) * P.units_per_split, P.units), (W.seen + 31) >> 5);
     const int coded_end = min(u_end, coded_units);
-    int u = u_begin;
-    for (; u < coded_end; u += NW) {
+    bool wild = false;
+    if (u_tail < u_end)
+        wild = W.template tail<true, true>(P, c, g, u_tail, lane);
+    else
+        W.clear();
+    if (late) first();
+    for (int u = u_begin; u < coded_end; u += NW) {
         q8_f4 s[RW][2];
 #pragma unroll
         for (int w = 0; w < RW; ++w) s[w][0] = s[w][1] = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -560,7 +583,7 @@ __global__ __launch_bounds__(64 * NW) void attn_q8_kernel(AttnQ8Params P) {
         }
         if (more) load_v(u + NW);
     }
-    W.tail(P, c, g, u, u_end, NW, lane);
+    if (wild) W.wild(P, g, u_tail, u_tail + 1, lane);
 #pragma unroll
     for (int w = 0; w < RW; ++w) W.lsum[w] = q8_rows4_sum(W.lsum[w]);
     q8_meet<D, NW, RW, SPLIT>(P, W, g, rt, split, wave, lane, smem, ml);
@@ -578,8 +601,8 @@ __global__ __launch_bounds__(64 * NW) void attn_q8_kernel(AttnQ8Params P) {
 // t - 2) are converted meanwhile; U + 1 stages of each are in LDS, with one barrier
 // per stage.
 //
-// Measured: 1024 rows of 8 heads of 128 over 32768 keys 149 us with f16 output, 0.92
-// PFLOP/s of a large matrix product's 1.29, 197 with f32 (a third more products: V's
+// Measured: 1024 rows of 8 heads of 128 over 32768 keys 147 us with f16 output, 0.93
+// PFLOP/s of a large matrix product's 1.29, 194 with f32 (a third more products: V's
 // with two fp16 for a weight). Matrix cores 42 % busy, vector instructions 54 % of the
 // time: the softmax of 16 scores a lane and unit holds back the products, whose
 // operands come from LDS once for 32 rows. U = 1: 151 to 157. Matrix and vector
@@ -655,6 +678,7 @@ __global__ __launch_bounds__(64 * NW) void attn_q8_tile_kernel(AttnQ8Params P) {
         s1 = load_scale(1);
     }
     W.start(P, g, (rt * NW + wave) * 16 * RW, lo, hi);
+    W.clear();
     if (stages > 0) {
         // (V of stage 0 into the place of stage -1 too: finite, its weights are 0)
         store(raw, 0, BUFS - 1);
@@ -762,7 +786,11 @@ __global__ __launch_bounds__(64 * NW) void attn_q8_tile_kernel(AttnQ8Params P) {
         __syncthreads();
         products(count - 1, pha, pla);
     }
-    W.tail(P, c, g, max(u_begin, coded_units), min(u_last, (W.seen + 31) >> 5), 1, lane);
+    const int t_begin = max(u_begin, coded_units), t_end = min(u_last, (W.seen + 31) >> 5);
+    bool wild = false;
+#pragma unroll 1
+    for (int u = t_begin; u < t_end; ++u) wild |= W.template tail<false, (D < 256)>(P, c, g, u, lane);
+    if (wild) W.wild(P, g, t_begin, t_end, lane);
 #pragma unroll
     for (int w = 0; w < RW; ++w) W.lsum[w] = q8_rows4_sum(W.lsum[w]);
 #pragma unroll

@@ -234,13 +234,13 @@ def test_attention_row_counts(ctx, d, fmt, dtype):
 
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("fmt", ["i8", "e4m3"])
-@pytest.mark.parametrize("length", [33, 64, 100, 129, 300, 1111])
+@pytest.mark.parametrize("length", [33, 64, 100, 129, 300, 1111, 1400])
 def test_attention_much_work_kernel(ctx, d, fmt, length):
     """The kernel for much work, forced onto short contexts: one stage, odd and even
     counts of them, a tail, several splits, rows past the last block's."""
     with D.plan_switch("HM_Q8_TILE", 1):
         for causal, block, dtype in ((True, 32, torch.float32), (False, 64, torch.float16), (True, 128, torch.float16)):
-            p = Pair(ctx, 6, 2, d, fmt, block, causal=causal, capacity=1200, seed=d + length)
+            p = Pair(ctx, 6, 2, d, fmt, block, causal=causal, capacity=1500, seed=d + length)
             p.fill(length)
             for rows in (1, 33, min(90, length)):
                 p.check_run(rows, length - rows if length >= rows else 0, dtype)

@@ -173,9 +173,11 @@ int rk_npu_hip_inject_alloc_failures(int count);
  *   HM_HOST_POLL     microseconds a host-buffer call on the kernel path
  *                    polls its completion word before it waits on its
  *                    stream instead (2000; 0: after the first 256 polls)
- *   HM_Q8_TILE       -1 by work; 0 never, 1 always: the attention over an 8-bit
- *                    cache (rk_npu_attention_q8.h) converts codes once a
- *                    block of 128 or 256 query rows instead of in every wave
+ *   HM_Q8_TILE       -1 by work; 1: the attention over an 8-bit cache
+ *                    (rk_npu_attention_q8.h) converts codes once a block of
+ *                    128 or 256 query rows; 0: in every wave, for 16 query
+ *                    rows, or 32 where there are more of head_dim 64 or 128;
+ *                    2: as 0, for 32 of head_dim 256 too
  *   HM_HOST_SPIN     0: a host-buffer call that waits on its stream does so
  *                    in hipStreamSynchronize; 1: by polling its stream
  *                    (slower here)

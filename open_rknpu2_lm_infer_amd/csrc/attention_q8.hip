@@ -656,27 +656,37 @@ static void q8_combine(const AttnQ8Params& P, int R, hipStream_t s) {
 //   head_dim 64, 8 KV heads, 512 x 32000: 58.4 and 59.8, f32 80.4 and 76.1;
 //   head_dim 256, 2 KV heads: 1024 x 8000 37.1 and 38.1, x 16000 65.4 and 55.9.
 // They cross near 24 million rows x keys x dims a CU.
-static bool q8_tile(int D, int R, int kv_heads, int units) {
+//
+// attn_q8_kernel's blocks: one row group, for few rows, on 4 waves (8 on half as many
+// splits: one row of 32 heads over 8 of 128 and 3981 keys 8.5 us instead of 8.0, 64
+// heads over 8 of 256 and 16001 keys 19.4 and 17.0); two share a unit's conversion. Two
+// of 256 dims take every register of a SIMD, and pay over many keys only: i8, 2 KV
+// heads, 512 rows x 16000 keys 43.8 with one and 34.6 with two, x 8000 26.7 and 23.8, x
+// 4000 17.1 and 19.5; 2048 x 4000 34.5 and 34.7 (e4m3, 4 KV heads, 1024 rows 27.5 and
+// 31.7).
+static Q8Plan q8_plan(int D, int R, int kv_heads, int units) {
     const int forced = attention_q8_tile_switch();
-    return forced >= 0 ? forced != 0 : (double)D * R * kv_heads * units * 32 > 24e6 * device_cus();
+    const double work = (double)D * R * kv_heads * units * 32 / device_cus();
+    if (forced == 1 || (forced < 0 && work > 24e6)) return Q8Plan{true, D == 256 ? 1 : 2, 8};
+    if (R <= 16) return Q8Plan{false, 1, 4};
+    if (D < 256) return Q8Plan{false, 2, 8};
+    return Q8Plan{false, forced == 2 || (forced < 0 && work > 10e6 && units > 200) ? 2 : 1, 4};
 }
 
-// Key splits: blocks enough for the CUs, but no more, as a block's rows leave
-// partials: 256 blocks of many rows (512 rows of 8 heads over 4096 keys 21.9 us, 27.6
-// with 512), 128 where a KV head has at most 32, whose blocks are 8 waves that only
-// load (8 rows of 8 heads of 256 over 16001 keys 19.3 us, 20.6 with 256 and 28.2 with
-// 512). A split holds at least a unit for each wave, or two stages. Few keys are not
-// split: a wave walks its 3 to 5 units in the time of the join's launch, 3 us. One and
-// 16 rows of 32 heads over 8 of 128: 768 keys 6.4 and 8.7 us, split 7.9 and 9.9, 1000
-// keys 8.1 and 11.1, split 8.3 and 11.0; one of 16 over 8 of 64: 1000 keys 6.9, split
-// 8.2, 1500 keys 8.1 and 8.3; one of 16 over 2 of 256: 480 keys 7.8, split 9.3, 768 keys
-// 9.4 and 9.4, 1000 keys 13.3, split 11.0.
-static void q8_splits(AttnQ8Params& P, int D, int R, bool tile) {
-    const int rows = q8_block_rows(D, R, tile);
+// Key splits: a block for each CU, but no more, as a block's rows leave partials (512
+// rows of 8 heads over 4096 keys 21.9 us, 27.6 with 512 blocks, 25.5 with 128; one row
+// of 16 heads over 2 of 256 and 20000 keys 11.3, 16.2 with 512). A split holds at least a
+// unit for each wave, or two stages. Few keys are not split: a wave walks its 4 to 6
+// units in the time of the join's launch, 3 us. One row of 32 heads over 8 of 128:
+// 768 keys 6.5, split 7.1, 1000 keys 8.5 and 7.7; of 16 over 2 of 256: 480 keys 7.4 and
+// 7.9, 768 keys 9.3 and 8.2; 64 rows of 32 over 8 of 128 (8 waves): 1000 keys 11.2 and
+// 12.8, 1500 keys 13.7 and 13.5.
+static void q8_splits(AttnQ8Params& P, int D, int R, const Q8Plan& plan) {
+    const int rows = plan.rows();
     P.row_tiles = (R + rows - 1) / rows;
     P.rows_pad = P.row_tiles * rows;
-    const int base = P.row_tiles * P.kh, least = tile ? 4 : Q8_WAVES, blocks = R > 32 ? 256 : 128;
-    const int few = D == 64 ? 40 : D == 128 ? 32 : 24;
+    const int base = P.row_tiles * P.kh, least = plan.tile ? 4 : plan.waves, blocks = 256;
+    const int few = D == 256 ? 16 : plan.waves == 4 ? 24 : 32;
     const size_t room = attn_partial_rows(D) / ((size_t)P.rows_pad * P.kh);
     int want = std::max(1, std::min((blocks + base - 1) / base, (P.units + least - 1) / least));
     want = (int)std::min<size_t>(want, std::max<size_t>(1, room));
@@ -721,9 +731,9 @@ static int q8_enqueue_run(AttnWork* w, Q8Cache* c, const HeadsView& q, int rows,
     P.coded = c->rows.coded;
     P.units = ((causal ? std::min(len, pos + rows) : len) + 31) / 32;
     const int R = cfg.query_heads / cfg.kv_heads * rows;
-    const bool tile = q8_tile(D, R, cfg.kv_heads, P.units);
-    q8_splits(P, D, R, tile);
-    (c->cfg.format == RK_NPU_HIP_KV_I8 ? launch_attn_q8_i8 : launch_attn_q8_e4m3)(P, D, R, tile, !P.out_f16, s);
+    const Q8Plan plan = q8_plan(D, R, cfg.kv_heads, P.units);
+    q8_splits(P, D, R, plan);
+    (c->cfg.format == RK_NPU_HIP_KV_I8 ? launch_attn_q8_i8 : launch_attn_q8_e4m3)(P, D, plan, !P.out_f16, s);
     if (P.splits > 1) {
         if (D == 64)
             q8_combine<64>(P, R, s);

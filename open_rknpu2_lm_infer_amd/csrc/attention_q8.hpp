@@ -492,16 +492,16 @@ __device__ __forceinline__ void q8_meet(const AttnQ8Params& P, const Q8Wave<D, R
 // converted.
 //
 // Measured, the join included: one row of 32 heads over 8 of 128 and 131072 keys
-// (268 MB) e4m3 46.7 us, i8 50: 5.7 and 5.4 TB/s (a large copy reads and writes
-// 4.9). Over 3968 keys (8 MB) 8.1: there it is latency, a unit's load to its
-// products, the waves' meeting and the join's launch. 512 rows over 4096 keys 21.3:
+// (268 MB) e4m3 45.6 us, i8 44.9: 5.9 and 6.0 TB/s (a large copy reads and writes
+// 4.9). Over 3968 keys (8 MB) 7.3: there it is latency, a unit's load to its
+// products, the waves' meeting and the join's launch. 512 rows over 4096 keys 21.7:
 // conversion and softmax, vector instructions that every 32 rows repeat. The tail
 // after the coded units, its loads a round trip of their own: one row of 16 heads over
-// 2 of 256, 1000 keys 12.2 instead of 11.0; of 32 over 8 of 128, 3981 keys 8.8 and 8.5. The splits
-// joined by their last block, in the same launch, lost to a launch of their own (8.6):
-// 10.0 with the partials through atomics of agent scope, 30 behind a fence, which
-// writes the L2 back. Blocks of 2 or 4 groups of waves with keys of their own and
-// more rows each: 27 to 31 for the 512 rows.
+// 2 of 256, 1000 keys 12.2 us instead of 11.0. The splits joined by their last block,
+// in the same launch, lost to a launch of their own (8.6): 10.0 with the partials
+// through atomics of agent scope, 30 behind a fence, which writes the L2 back. Blocks
+// of 2 or 4 groups of waves with keys of their own and more rows each: 27 to 31 for the
+// 512 rows.
 template <int D, int NW, int RW, int FMT, bool SPLIT>
 __global__ __launch_bounds__(64 * NW) void attn_q8_kernel(AttnQ8Params P) {
     constexpr int KP = D / 32;  // 16-byte pieces per lane, of K (and V)
@@ -871,39 +871,38 @@ __global__ __launch_bounds__(256) void attn_q8_combine_kernel(AttnQ8Params P) {
     q8_store4(P, (long long)(g * G + h) * P.o_head + (rr - h * P.m) * P.o_row + 4 * d4, num * (1.0f / den));
 }
 
-// Row groups (of 16) a wave takes, and rows of a block: attn_q8_kernel's waves share
-// the rows, attn_q8_tile_kernel's have their own.
-constexpr int Q8_WAVES = 8;
-inline int q8_groups(int head_dim, int R) { return R <= 16 || head_dim == 256 ? 1 : 2; }
-inline int q8_block_rows(int head_dim, int R, bool tile) { return 16 * q8_groups(head_dim, R) * (tile ? Q8_WAVES : 1); }
+// The kernel of a run: attn_q8_tile_kernel (8 waves with row groups of their own, 2,
+// or 1 of heads of 256) or attn_q8_kernel (waves that share `groups` row groups of 16).
+struct Q8Plan {
+    bool tile;
+    int groups, waves;
+    int rows() const { return 16 * groups * (tile ? waves : 1); }  // of a block
+};
 
-void launch_attn_q8_i8(const AttnQ8Params& P, int head_dim, int R, bool tile, bool f32_weights, hipStream_t s);
-void launch_attn_q8_e4m3(const AttnQ8Params& P, int head_dim, int R, bool tile, bool f32_weights, hipStream_t s);
+void launch_attn_q8_i8(const AttnQ8Params& P, int head_dim, const Q8Plan& plan, bool f32_weights, hipStream_t s);
+void launch_attn_q8_e4m3(const AttnQ8Params& P, int head_dim, const Q8Plan& plan, bool f32_weights, hipStream_t s);
 
 template <int D, int FMT, bool SPLIT>
-static void launch_attn_q8_rows(const AttnQ8Params& P, int R, bool tile, hipStream_t s) {
+static void launch_attn_q8_rows(const AttnQ8Params& P, const Q8Plan& plan, hipStream_t s) {
     // (a row tile's blocks of one KV head are 8 apart where there are 8 heads: the
     // XCDs take blocks in turn, so each keeps one head's codes in its L2)
-    const dim3 grid(P.kh, P.row_tiles, P.splits), block(64 * Q8_WAVES);
-    if (tile) {
-        if constexpr (D == 256)
-            hipLaunchKernelGGL((attn_q8_tile_kernel<D, Q8_WAVES, 1, 1, FMT, SPLIT>), grid, block, 0, s, P);
-        else
-            hipLaunchKernelGGL((attn_q8_tile_kernel<D, Q8_WAVES, 2, 2, FMT, SPLIT>), grid, block, 0, s, P);
-    } else if (q8_groups(D, R) == 1) {
-        hipLaunchKernelGGL((attn_q8_kernel<D, Q8_WAVES, 1, FMT, SPLIT>), grid, block, 0, s, P);
-    } else if constexpr (D < 256) {
-        hipLaunchKernelGGL((attn_q8_kernel<D, Q8_WAVES, 2, FMT, SPLIT>), grid, block, 0, s, P);
-    }
+    const dim3 grid(P.kh, P.row_tiles, P.splits), block(64 * plan.waves);
+    constexpr int G = D == 256 ? 1 : 2;
+    if (plan.tile)
+        hipLaunchKernelGGL((attn_q8_tile_kernel<D, 8, G, G, FMT, SPLIT>), grid, block, 0, s, P);
+    else if (plan.groups == 1)
+        hipLaunchKernelGGL((attn_q8_kernel<D, 4, 1, FMT, SPLIT>), grid, block, 0, s, P);
+    else
+        hipLaunchKernelGGL((attn_q8_kernel<D, D == 256 ? 4 : 8, 2, FMT, SPLIT>), grid, block, 0, s, P);
 }
 
 template <int FMT>
-static void launch_attn_q8(const AttnQ8Params& P, int head_dim, int R, bool tile, bool f32_weights, hipStream_t s) {
+static void launch_attn_q8(const AttnQ8Params& P, int head_dim, const Q8Plan& plan, bool f32_weights, hipStream_t s) {
 #define HM_Q8_ROWS(DD)                                     \
     if (f32_weights)                                       \
-        launch_attn_q8_rows<DD, FMT, true>(P, R, tile, s); \
+        launch_attn_q8_rows<DD, FMT, true>(P, plan, s); \
     else                                                   \
-        launch_attn_q8_rows<DD, FMT, false>(P, R, tile, s)
+        launch_attn_q8_rows<DD, FMT, false>(P, plan, s)
     if (head_dim == 64) {
         HM_Q8_ROWS(64);
     } else if (head_dim == 128) {

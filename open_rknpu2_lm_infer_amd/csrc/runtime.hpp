@@ -197,8 +197,7 @@ struct HostSeg {
     size_t stage_off;  // 256-byte aligned offset of this segment in the stage
 };
 bool stage_small(const HostStage& st, const void* p, size_t in_bytes, size_t out_bytes);
-// HM_Q8_TILE: -1 by work; 0 never, 1 always the attention over the 8-bit cache
-// takes its kernel for much work.
+// HM_Q8_TILE: which kernel the attention over the 8-bit cache takes; -1 by work.
 int attention_q8_tile_switch();
 // HM_HOST_FLAG: host-buffer calls may take the kernel path at all.
 bool host_kernels_enabled();

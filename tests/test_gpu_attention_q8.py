@@ -247,6 +247,32 @@ def test_attention_much_work_kernel(ctx, d, fmt, length):
     p.check_run(1, 0, torch.float32)
 
 
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("length", [40, 100, 129, 600, 1400])
+def test_attention_wide_heads_of_two_row_groups(ctx, fmt, length):
+    """Heads of 256, two row groups a wave, forced onto short contexts."""
+    with D.plan_switch("HM_Q8_TILE", 2):
+        for causal, block, dtype in ((True, 32, torch.float32), (False, 128, torch.float16)):
+            p = Pair(ctx, 6, 2, 256, fmt, block, causal=causal, capacity=1500, seed=length)
+            p.fill(length)
+            for rows in (1, 11, 33):
+                p.check_run(rows, length - rows, dtype)
+
+
+def test_kernels_by_work(ctx):
+    """Calls that take two row groups of 256 by themselves: the same bits as forced."""
+    p = Pair(ctx, 8, 1, 256, "e4m3", 32, capacity=9000, seed=4)
+    p.fill(9000)
+    q = torch.randn(8, 160, 256, device="cuda", dtype=torch.float16)
+    outs = []
+    for value in (-1, 2, 0):
+        with D.plan_switch("HM_Q8_TILE", value):
+            outs.append(torch.empty(8, 160, 256, device="cuda"))
+            D.attention_q8(ctx, p.cache, q, outs[-1], 9000 - 160)
+    assert torch.equal(outs[0], outs[1]) and not torch.equal(outs[0], outs[2])
+    p.compare(q[:, :4].cpu().numpy(), outs[0][:, :4], 9000 - 160)
+
+
 def test_much_work_takes_its_kernel(ctx):
     """A call large enough for it by itself, 256 rows of 8 heads over 12000 keys of
     256: the same bits as forced, others than without."""
@@ -263,7 +289,7 @@ def test_much_work_takes_its_kernel(ctx):
     p.compare(q[:, :4].cpu().numpy(), outs[0][:, :4], 12000 - 256)
 
 
-@pytest.mark.parametrize("tile", [0, 1])
+@pytest.mark.parametrize("tile", [0, 1, 2])
 def test_special_values_in_both_kernels(ctx, tile):
     """Poisoned blocks, infinities of the tail, scales far apart and late maxima, each
     kernel forced."""

@@ -198,6 +198,7 @@ class KvCacheQ8:
               "create the 8-bit KV cache")
         self.handle = _Handle(raw.value, L.rk_npu_hip_attention_q8_cache_free, "8-bit KV cache", ctx.shared)
         self.ctx, self.config = ctx, cfg
+        self._kv, self._query = (kv_heads, head_dim), (query_heads, head_dim)
 
     def info(self) -> F.rk_npu_attention_f16_cache_info:
         info = F.rk_npu_attention_f16_cache_info()
@@ -222,24 +223,26 @@ class KvCacheQ8:
 
     def append(self, k, v, stream=None) -> None:
         """Appends k and v, [kv_heads][rows][head_dim]."""
-        ensure(k.shape == v.shape, "k and v must have the same shape")
-        heads = [_heads(t, self.config.attention.kv_heads, self.config.attention.head_dim) for t in (k, v)]
-        check(F.lib().rk_npu_hip_attention_q8_device_append(self.handle.raw, ctypes.byref(heads[0]),
-                                                            ctypes.byref(heads[1]), k.shape[1], _stream(stream, k)),
+        shape = k.shape
+        ensure(shape == v.shape, "k and v must have the same shape")
+        kh, vh = _heads(k, *self._kv), _heads(v, *self._kv)
+        check(F.lib().rk_npu_hip_attention_q8_device_append(self.handle.raw, ctypes.byref(kh), ctypes.byref(vh),
+                                                            shape[1], _stream(stream, k)),
               "append to the 8-bit KV cache")
 
     def read(self, first: int, k, v, stream=None) -> None:
         """The values of tokens first.. into k and v, [kv_heads][rows][head_dim]."""
-        ensure(k.shape == v.shape, "k and v must have the same shape")
-        heads = [_heads(t, self.config.attention.kv_heads, self.config.attention.head_dim) for t in (k, v)]
-        check(F.lib().rk_npu_hip_attention_q8_device_read(self.handle.raw, first, k.shape[1], ctypes.byref(heads[0]),
-                                                          ctypes.byref(heads[1]), _stream(stream, k)),
+        shape = k.shape
+        ensure(shape == v.shape, "k and v must have the same shape")
+        kh, vh = _heads(k, *self._kv), _heads(v, *self._kv)
+        check(F.lib().rk_npu_hip_attention_q8_device_read(self.handle.raw, first, shape[1], ctypes.byref(kh),
+                                                          ctypes.byref(vh), _stream(stream, k)),
               "read the 8-bit KV cache")
 
 
 def _heads(t, heads: int, head_dim: int) -> F.rk_npu_hip_heads:
     shape, stride = t.shape, t.stride()
-    if not (t.is_cuda and len(shape) == 3 and shape[0] == heads and shape[2] == head_dim and stride[2] == 1):
+    if not (len(shape) == 3 and shape[0] == heads and shape[2] == head_dim and stride[2] == 1 and t.is_cuda):
         raise NpuError(f"attention arrays are cuda [{heads}][rows][{head_dim}] tensors with contiguous rows")
     return F.rk_npu_hip_heads(t.data_ptr(), _dtype_code(t), stride[0], stride[1])
 
@@ -248,11 +251,11 @@ def attention_q8(ctx: DeviceContext, cache: KvCacheQ8, q, out, position: int, ws
     """Attention of the rows q [query_heads][rows][head_dim], the first at
     `position`, over the cache's tokens. ws: the context's workspace of this
     geometry, which calls on one stream share."""
-    c = cache.config.attention
-    ensure(q.shape == out.shape, "q and out must have the same shape")
+    shape = q.shape
+    ensure(shape == out.shape, "q and out must have the same shape")
     ws = ws or ctx.attention_workspace(cache)
-    qh, oh = _heads(q, c.query_heads, c.head_dim), _heads(out, c.query_heads, c.head_dim)
-    check(F.lib().rk_npu_hip_attention_q8_device_run(ws.raw, cache.handle.raw, ctypes.byref(qh), q.shape[1], position,
+    qh, oh = _heads(q, *cache._query), _heads(out, *cache._query)
+    check(F.lib().rk_npu_hip_attention_q8_device_run(ws.raw, cache.handle.raw, ctypes.byref(qh), shape[1], position,
                                                      ctypes.byref(oh), _stream(stream, q)), "8-bit KV attention")
 
 

@@ -801,13 +801,13 @@ __global__ __launch_bounds__(64 * NW) void attn_q8_tile_kernel(AttnQ8Params P) {
 }
 
 // The splits' partials of one row: out = sum_s w_s acc_s / sum_s w_s l_s with
-// w_s = 2^(m_s - max m). RPB rows a block, T = 256 / RPB threads each, thread t
-// with 4 dims of every GS-th split (GS = 4 T / D); their loads, 8 at a time, do not
-// wait for the weights, which the row's threads find meanwhile; sums over the GS
-// groups meet in LDS.
-template <int D, int RPB>
+// w_s = 2^(m_s - max m). Block: DB dims (part blockIdx.z of D) of RPB rows, T = 256 / RPB
+// threads each, thread t with 4 dims of every GS-th split (GS = 4 T / DB); their loads, 8
+// at a time, do not wait for the weights, which the row's threads find meanwhile; sums
+// over the GS groups meet in LDS.
+template <int D, int RPB, int DB>
 __global__ __launch_bounds__(256) void attn_q8_combine_kernel(AttnQ8Params P) {
-    constexpr int T = 256 / RPB, LD = D / 4, GS = T / LD, B = 8;
+    constexpr int T = 256 / RPB, LD = DB / 4, GS = T / LD, B = 8;
     static_assert(GS >= 1 && T % LD == 0, "threads per row");
     __shared__ float weight[RPB][256];
     __shared__ float red[RPB][2][T / 32];
@@ -817,10 +817,10 @@ __global__ __launch_bounds__(256) void attn_q8_combine_kernel(AttnQ8Params P) {
     const int G = P.qh / P.kh, R = G * P.m, S = P.splits;
     const int rr = min(rr0, R - 1);  // (threads past the last row: that row again, not written)
     const size_t at = ((size_t)g * P.rows_pad + rr) * S;
-    const q8_f4* acc = reinterpret_cast<const q8_f4*>(P.part + at * D) + d4;
+    const q8_f4* acc = reinterpret_cast<const q8_f4*>(P.part + at * D) + blockIdx.z * LD + d4;
     q8_f4 v[B];
 #pragma unroll
-    for (int i = 0; i < B; ++i) v[i] = acc[(size_t)min(gs + i * GS, S - 1) * LD];
+    for (int i = 0; i < B; ++i) v[i] = acc[(size_t)min(gs + i * GS, S - 1) * (D / 4)];
     // weights and denominator, over the row's threads (whole half waves)
     const float2* ml = reinterpret_cast<const float2*>(P.part + (size_t)P.kh * P.rows_pad * S * D) + at;
     float2 x[256 / T];
@@ -853,7 +853,7 @@ __global__ __launch_bounds__(256) void attn_q8_combine_kernel(AttnQ8Params P) {
 #pragma unroll
         for (int i = 0; i < B; ++i) {
             if (s + i * GS < S) num += v[i] * weight[row][s + i * GS];
-            v[i] = acc[(size_t)min(s + (B + i) * GS, S - 1) * LD];
+            v[i] = acc[(size_t)min(s + (B + i) * GS, S - 1) * (D / 4)];
         }
     }
     if constexpr (GS > 1) {
@@ -868,7 +868,8 @@ __global__ __launch_bounds__(256) void attn_q8_combine_kernel(AttnQ8Params P) {
 #pragma unroll
     for (int i = 1; i < T / 32; ++i) den += red[row][1][i];
     const int h = rr / P.m;
-    q8_store4(P, (long long)(g * G + h) * P.o_head + (rr - h * P.m) * P.o_row + 4 * d4, num * (1.0f / den));
+    q8_store4(P, (long long)(g * G + h) * P.o_head + (rr - h * P.m) * P.o_row + DB * blockIdx.z + 4 * d4,
+              num * (1.0f / den));
 }
 
 // The kernel of a run: attn_q8_tile_kernel (8 waves with row groups of their own, 2,

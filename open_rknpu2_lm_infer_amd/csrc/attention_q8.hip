@@ -674,30 +674,38 @@ static void q8_combine(const AttnQ8Params& P, int R, hipStream_t s) {
                            P);
 }
 
-// The kernel, for R query rows of each KV head: attn_q8_kernel converts a unit's codes
-// in every wave, attn_q8_tile_kernel once a block, which takes rows enough to fill
-// 128- or 256-row blocks and keys enough to fill its stages. Measured, us, either:
-//   head_dim 128, 8 KV heads, f16 output: 512 rows x 8000 keys 34.1 and 45.1, x 16000
-//   56.4 and 56.4, x 32000 98.6 and 89.9; 1024 x 8000 50.0 and 56.2, x 16000 88.7 and
-//   85.9; f32 output 512 x 16000 69.8 and 68.9, 1024 x 8000 63.9 and 67.5;
-//   head_dim 64, 8 KV heads, 512 x 32000: 58.4 and 59.8, f32 80.4 and 76.1;
-//   head_dim 256, 2 KV heads: 1024 x 8000 37.1 and 38.1, x 16000 65.4 and 55.9.
-// They cross near 24 million rows x keys x dims a CU.
-//
-// attn_q8_kernel's blocks: one row group, for few rows, on 4 waves (8 on half as many
+// The kernel, for R query rows of each KV head. attn_q8_kernel converts a unit's codes
+// in every wave: in blocks of one row group, for few rows, on 4 waves (8 on half as many
 // splits: one row of 32 heads over 8 of 128 and 3981 keys 8.5 us instead of 8.0, 64
-// heads over 8 of 256 and 16001 keys 19.4 and 17.0); two share a unit's conversion. Two
-// of 256 dims take every register of a SIMD, and pay over many keys only: i8, 2 KV
-// heads, 512 rows x 16000 keys 43.8 with one and 34.6 with two, x 8000 26.7 and 23.8, x
-// 4000 17.1 and 19.5; 2048 x 4000 34.5 and 34.7 (e4m3, 4 KV heads, 1024 rows 27.5 and
-// 31.7).
-static Q8Plan q8_plan(int D, int R, int kv_heads, int units) {
+// heads over 8 of 256 and 16001 keys 19.4 and 17.0), or of two, which share a unit's
+// conversion. Two of 256 dims take every register of a SIMD, and pay over many keys
+// only: i8, 2 KV heads, 512 rows x 16000 keys 43.8 with one and 34.6 with two, x 8000
+// 26.7 and 23.8, x 4000 17.1 and 19.5; 2048 x 4000 34.5 and 34.7 (e4m3, 4 KV heads,
+// 1024 rows 27.5 and 31.7).
+//
+// attn_q8_tile_kernel converts once a block, which takes rows enough to fill 128- or
+// 256-row blocks and keys enough to fill its stages; the more, the cheaper the
+// conversion. `cross`: where they do, in million rows x keys x dims a CU. Measured,
+// us, two row groups in every wave and once a block, 8 KV heads (256 dims: 2):
+//   128 dims, i8, f32 output: 1024 rows x 8000 keys (33) 57.4 and 64.8, x 16000 (66) 112
+//   and 106, 256 x 32000 (33) 65.3 and 66.7; e4m3: 1024 x 16000 99.0 and 104, x 32000
+//   195 and 188, f16 output 75.6 and 82.5, 149 and 145; i8, f16 output: x 16000 74.4 and
+//   83.4, x 32000 143 and 147, x 64000 280 and 269;
+//   64 dims, i8, f32: 256 x 32000 (16) 47.7 and 46.7, 1024 x 16000 (33) 76.7 and 78.6, x
+//   32000 149 and 136; e4m3: x 16000 69.1 and 78.6, x 32000 136 and 136, f16 103 and 101;
+//   i8, f16: x 32000 102 and 102, x 64000 204 and 186;
+//   256 dims, i8, f32: 512 x 32000 (33) 68.6 and 69.3, x 64000 122 and 116; e4m3: 110 and
+//   110, f16 87.9 and 90.9, 2048 x 32000 (131) 158 and 152; i8, f16: x 64000 (262) 288
+//   and 295.
+static Q8Plan q8_plan(int D, int R, int kv_heads, int units, bool i8, bool f16) {
+    static const float cross[3][3] = {{28, 45, 33}, {55, 95, 63}, {60, 180, 250}};  // by head_dim 64, 128, 256
     const int forced = attention_q8_tile_switch();
-    const double work = (double)D * R * kv_heads * units * 32 / device_cus();
-    if (forced == 1 || (forced < 0 && work > 24e6)) return Q8Plan{true, D == 256 ? 1 : 2, 8};
+    const double work = 1e-6 * D * R * kv_heads * units * 32 / device_cus();
+    const double most = cross[!i8 ? 1 : f16 ? 2 : 0][D / 128];
+    if (forced == 1 || (forced < 0 && R > 16 && work > most)) return Q8Plan{true, D == 256 ? 1 : 2, 8};
     if (R <= 16) return Q8Plan{false, 1, 4};
     if (D < 256) return Q8Plan{false, 2, 8};
-    return Q8Plan{false, forced == 2 || (forced < 0 && work > 10e6 && units > 200) ? 2 : 1, 4};
+    return Q8Plan{false, forced == 2 || (forced < 0 && work > 10 && units > 200) ? 2 : 1, 4};
 }
 
 // Key splits: a block for each CU, but no more, as a block's rows leave partials (512
@@ -758,7 +766,7 @@ static int q8_enqueue_run(AttnWork* w, Q8Cache* c, const HeadsView& q, int rows,
     P.coded = c->rows.coded;
     P.units = ((causal ? std::min(len, pos + rows) : len) + 31) / 32;
     const int R = cfg.query_heads / cfg.kv_heads * rows;
-    const Q8Plan plan = q8_plan(D, R, cfg.kv_heads, P.units);
+    const Q8Plan plan = q8_plan(D, R, cfg.kv_heads, P.units, c->cfg.format == RK_NPU_HIP_KV_I8, P.out_f16);
     q8_splits(P, D, R, plan);
     (c->cfg.format == RK_NPU_HIP_KV_I8 ? launch_attn_q8_i8 : launch_attn_q8_e4m3)(P, D, plan, !P.out_f16, s);
     if (P.splits > 1) {

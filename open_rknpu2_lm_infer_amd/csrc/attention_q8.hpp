@@ -79,6 +79,20 @@ __device__ __forceinline__ q8_h8 q8_halves(unsigned lo, unsigned hi) {
     return __builtin_bit_cast(q8_h8, v4u{w[0], w[1], w[2], w[3]});
 }
 
+// The same codes of the i8 format as they are stored, u = code + 128, half the
+// instructions: a byte under 0x00 is the fp16 u 2^-24. What that adds, 128 2^-24 times
+// the sum of the other operand, is taken off the sums (Q8Wave, RAW).
+__device__ __forceinline__ q8_h8 q8_bytes(unsigned w0, unsigned w1) {
+    const v4u x = {__builtin_amdgcn_perm(0u, w0, 0x0C010C00u), __builtin_amdgcn_perm(0u, w0, 0x0C030C02u),
+                   __builtin_amdgcn_perm(0u, w1, 0x0C010C00u), __builtin_amdgcn_perm(0u, w1, 0x0C030C02u)};
+    return __builtin_bit_cast(q8_h8, x);
+}
+template <int FMT, bool RAW>
+__device__ __forceinline__ q8_h8 q8_operand(unsigned w0, unsigned w1) {
+    if constexpr (RAW) return q8_bytes(w0, w1);
+    return q8_halves<FMT>(w0, w1);
+}
+
 // Two f32 to fp16, once: without the empty asm the compiler folds the product
 // before a rounding into it in one of the rounding's uses (a single rounding there,
 // two in the others), and the remainder is then that of another value.
@@ -149,14 +163,24 @@ constexpr float Q8_SHIFT = 6.0f;  // SPLIT: the weights lie this much higher (p 
 // SPLIT (f32 output): p mu goes into the products as two fp16, 22 bits.
 // Otherwise (fp16 output) as one, and the sum adds the rounded weights (times
 // 1 / vs), so that a row whose weight is all on one key is not off.
-template <int D, int RW, bool SPLIT>
+//
+// RAW (i8, fp16 output, two row groups a wave): codes come as u 2^-24, u = code + 128,
+// half the instructions of their conversion (512 rows of 8 heads over 8000 keys of 128
+// 28.6 us instead of 34.1; one row group's waves wait for memory). Scores start from
+// -128 2^-24 sum(q); `vsum` adds the weights as they are multiplied, and every 16 units
+// 128 2^-24 of it leaves the accumulators, which else would grow with every key where
+// sums of codes walk: over 44000 keys in one split outputs were 3.2e-4 off instead of
+// 2.9e-4 (relative, fp16's rounding 2.1e-4). The 2^24 goes into cks and e. f32 output
+// has no room for it.
+template <int D, int RW, bool SPLIT, bool RAW = false>
 struct Q8Wave {
+    static_assert(!(SPLIT && RAW), "offset codes are for fp16 output");
     static constexpr int KS = D / 32, NB = D / 16;
     static constexpr float SHIFT = SPLIT ? Q8_SHIFT : 0.0f;
     int lim[RW];
     int open, seen;  // keys below `open` every row sees, from `seen` on none
     q8_h8 qf[RW][KS];
-    float mrun[RW], lsum[RW];
+    float mrun[RW], lsum[RW], vsum[RW], base[RW];
     q8_f4 o[RW][NB];
 
     // Rows r0 + 16 w + lane % 16 of KV head g. Rows from R on are computed as the
@@ -181,7 +205,7 @@ struct Q8Wave {
                 seen = max(seen, lim[w]);
             }
             mrun[w] = Q8_NONE;
-            lsum[w] = 0.0f;
+            lsum[w] = vsum[w] = base[w] = 0.0f;
         }
         if (!P.q_f32) {
 #pragma unroll
@@ -205,6 +229,18 @@ struct Q8Wave {
                     for (int i = 0; i < 8; ++i) qf[w][s][i] = (_Float16)x[s][i >> 2][i & 3];
             }
         }
+        if constexpr (RAW) {
+            q8_h8 off;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) off[i] = (_Float16)-0x1p-17f;
+#pragma unroll
+            for (int w = 0; w < RW; ++w) {
+                q8_f4 sum = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < KS; ++i) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(off, qf[w][i], sum, 0, 0, 0);
+                base[w] = sum[0];
+            }
+        }
         open = __builtin_amdgcn_readfirstlane(q8_row_min(open));
         seen = -__builtin_amdgcn_readfirstlane(q8_row_min(-seen));
     }
@@ -223,13 +259,15 @@ struct Q8Wave {
     struct Unit {
         float cks, lg, mu, part;  // part: what a weight's sum is multiplied with
     };
+    template <bool BYTES = false>
     static __device__ __forceinline__ Unit unit(float c, float ks, float mu, int e, float inv) {
         const bool poison = ks != ks || mu != mu;
         Unit x;
-        x.cks = poison ? NAN : fmaxf(c * ks, 0x1p-120f);
+        x.cks = poison ? NAN : fmaxf(c * ks, 0x1p-120f) * (BYTES ? 0x1p24f : 1.0f);
         x.mu = poison ? 1.0f : mu;
-        x.lg = SPLIT ? (float)e : (float)e + __builtin_amdgcn_logf(x.mu);
+        x.lg = SPLIT ? (float)e : (float)(e + (BYTES ? 24 : 0)) + __builtin_amdgcn_logf(x.mu);
         x.part = SPLIT ? __int_as_float((127 - e) << 23) : poison ? 1.0f : inv;  // 2^-e, 1 / (mu 2^e)
+        if (BYTES) x.part *= 0x1p-24f;
         return x;
     }
     // Masked scores become -inf; where there are some, those of a poisoned block
@@ -277,11 +315,13 @@ struct Q8Wave {
             }
             if constexpr (FIRST) continue;
             lsum[w] *= alpha;
+            vsum[w] *= alpha;
 #pragma unroll
             for (int n = 0; n < NB; ++n) o[w][n] *= alpha;
         }
     }
     // Scores to weights ph (and pl), and the rows' sums.
+    template <bool BYTES = false>
     __device__ __forceinline__ void weigh(const Unit& x, const q8_f4 (&s)[RW][2], q8_h8 (&ph)[RW], q8_h8 (&pl)[RW]) {
 #pragma unroll
         for (int w = 0; w < RW; ++w) {
@@ -310,6 +350,7 @@ struct Q8Wave {
                     }
                 }
             lsum[w] = __builtin_fmaf(l[0] + l[1], x.part, lsum[w]);
+            if constexpr (BYTES) vsum[w] += l[0] + l[1];
         }
     }
     __device__ __forceinline__ void product(int n, q8_h8 a, const q8_h8 (&ph)[RW], const q8_h8 (&pl)[RW]) {
@@ -393,7 +434,33 @@ struct Q8Wave {
             for (int i = 0; i < 8; ++i) a[i] = (_Float16)((float)a[i] * up);
             product(n, a, ph, pl);
         }
+        if constexpr (RAW) {  // (to the units of u 2^-24)
+            static_assert(FIRST || !RAW, "the open block first");
+#pragma unroll
+            for (int w = 0; w < RW; ++w) {
+                mrun[w] += 24.0f;
+                lsum[w] *= 0x1p-24f;
+#pragma unroll
+                for (int n = 0; n < NB; ++n) o[w][n] *= 0x1p-24f;
+            }
+        }
         return __builtin_amdgcn_ballot_w64(wild != 0) != 0;
+    }
+    // RAW: the accumulators of codes.
+    __device__ __forceinline__ void centre() {
+        if constexpr (!RAW) return;
+#pragma unroll
+        for (int w = 0; w < RW; ++w) {
+            const float off = -0x1p-17f * q8_rows4_sum(vsum[w]);
+            vsum[w] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) o[w][n] += off;
+        }
+    }
+    // The sums of a row's 4 lanes.
+    __device__ __forceinline__ void sums() {
+#pragma unroll
+        for (int w = 0; w < RW; ++w) lsum[w] = q8_rows4_sum(lsum[w]);
     }
     __device__ __forceinline__ void wild(const AttnQ8Params& P, int g, int u, int u_end, int lane) {
         const int hi = lane >> 4, coded_units = P.coded >> 5;
@@ -442,8 +509,8 @@ __device__ __forceinline__ void q8_finish(const AttnQ8Params& P, int g, int rr, 
 
 // The NW waves of a row tile meet: each leaves its accumulators in LDS (NW RW NB KiB)
 // and its rows' (max, sum), and takes an NW-th of the tile's (row group, dims) pairs.
-template <int D, int NW, int RW, bool SPLIT>
-__device__ __forceinline__ void q8_meet(const AttnQ8Params& P, const Q8Wave<D, RW, SPLIT>& W, int g, int rt, int split,
+template <int D, int NW, int RW, class Wave>
+__device__ __forceinline__ void q8_meet(const AttnQ8Params& P, const Wave& W, int g, int rt, int split,
                                         int wave, int lane, uint8_t* smem, float (&ml)[NW][RW][2][16]) {
     constexpr int NB = D / 16;
     const int lo = lane & 15, hi = lane >> 4, R = P.qh / P.kh * P.m;
@@ -494,7 +561,7 @@ __device__ __forceinline__ void q8_meet(const AttnQ8Params& P, const Q8Wave<D, R
 // Measured, the join included: one row of 32 heads over 8 of 128 and 131072 keys
 // (268 MB) e4m3 45.6 us, i8 44.9: 5.9 and 6.0 TB/s (a large copy reads and writes
 // 4.9). Over 3968 keys (8 MB) 7.3: there it is latency, a unit's load to its
-// products, the waves' meeting and the join's launch. 512 rows over 4096 keys 21.7:
+// products, the waves' meeting and the join's launch. 512 rows over 4096 keys 20.7:
 // conversion and softmax, vector instructions that every 32 rows repeat. The tail
 // after the coded units, its loads a round trip of their own: one row of 16 heads over
 // 2 of 256, 1000 keys 12.2 us instead of 11.0. The splits joined by their last block,
@@ -542,7 +609,8 @@ __global__ __launch_bounds__(64 * NW) void attn_q8_kernel(AttnQ8Params P) {
     const int u_tail = u_begin + (max(coded_units - u_begin, 0) + NW - 1) / NW * NW;
     const bool late = D == 256 && u_tail < min((split + 1) * P.units_per_split, P.units);
     if (!late) first();
-    Q8Wave<D, RW, SPLIT> W;
+    constexpr bool RAW = FMT == RK_NPU_HIP_KV_I8 && !SPLIT && RW > 1;
+    Q8Wave<D, RW, SPLIT, RAW> W;
     W.start(P, g, rt * RT, lo, hi);
     const int u_end = min(min((split + 1) * P.units_per_split, P.units), (W.seen + 31) >> 5);
     const int coded_end = min(u_end, coded_units);
@@ -555,14 +623,15 @@ __global__ __launch_bounds__(64 * NW) void attn_q8_kernel(AttnQ8Params P) {
     for (int u = u_begin; u < coded_end; u += NW) {
         q8_f4 s[RW][2];
 #pragma unroll
-        for (int w = 0; w < RW; ++w) s[w][0] = s[w][1] = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int w = 0; w < RW; ++w) s[w][0] = s[w][1] = q8_f4{W.base[w], W.base[w], W.base[w], W.base[w]};
         const float4 x = next;
         const bool more = u + NW < coded_end;
         if (more) next = sc[(u + NW) >> P.unit_shift];
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
             const int cb = i / (D / 64), st = i % (D / 64);
-            const q8_h8 a0 = q8_halves<FMT>(kr[i][0], kr[i][1]), a1 = q8_halves<FMT>(kr[i][2], kr[i][3]);
+            const q8_h8 a0 = q8_operand<FMT, RAW>(kr[i][0], kr[i][1]);
+            const q8_h8 a1 = q8_operand<FMT, RAW>(kr[i][2], kr[i][3]);
 #pragma unroll
             for (int w = 0; w < RW; ++w) {
                 s[w][cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, W.qf[w][2 * st], s[w][cb], 0, 0, 0);
@@ -571,22 +640,23 @@ __global__ __launch_bounds__(64 * NW) void attn_q8_kernel(AttnQ8Params P) {
         }
         if (more) load_k(u + NW);
         q8_h8 ph[RW], pl[RW];
-        auto un = W.unit(c, x.x, x.y, __float_as_int(x.z), x.w);
+        auto un = W.template unit<RAW>(c, x.x, x.y, __float_as_int(x.z), x.w);
         if (__builtin_expect(W.masked(u << 5, false), 0)) W.mask(un, u << 5, false, hi, s);  // (uniform)
         float top[RW];
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(W.over(un, s, top)) != 0, 0)) W.raise(top);
-        W.weigh(un, s, ph, pl);
+        W.template weigh<RAW>(un, s, ph, pl);
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
-            W.product(2 * i, q8_halves<FMT>(vr[i][0], vr[i][1]), ph, pl);
-            W.product(2 * i + 1, q8_halves<FMT>(vr[i][2], vr[i][3]), ph, pl);
+            W.product(2 * i, q8_operand<FMT, RAW>(vr[i][0], vr[i][1]), ph, pl);
+            W.product(2 * i + 1, q8_operand<FMT, RAW>(vr[i][2], vr[i][3]), ph, pl);
         }
         if (more) load_v(u + NW);
+        if (RAW && (u - u_begin) % (16 * NW) == 15 * NW) W.centre();
     }
+    W.centre();
+    W.sums();
     if (wild) W.wild(P, g, u_tail, u_tail + 1, lane);
-#pragma unroll
-    for (int w = 0; w < RW; ++w) W.lsum[w] = q8_rows4_sum(W.lsum[w]);
-    q8_meet<D, NW, RW, SPLIT>(P, W, g, rt, split, wave, lane, smem, ml);
+    q8_meet<D, NW, RW>(P, W, g, rt, split, wave, lane, smem, ml);
 }
 
 // Much work. Block: NW waves with RW groups of 16 rows each over one split; the codes
@@ -790,9 +860,8 @@ __global__ __launch_bounds__(64 * NW) void attn_q8_tile_kernel(AttnQ8Params P) {
     bool wild = false;
 #pragma unroll 1
     for (int u = t_begin; u < t_end; ++u) wild |= W.template tail<false, (D < 256)>(P, c, g, u, lane);
+    W.sums();
     if (wild) W.wild(P, g, t_begin, t_end, lane);
-#pragma unroll
-    for (int w = 0; w < RW; ++w) W.lsum[w] = q8_rows4_sum(W.lsum[w]);
 #pragma unroll
     for (int w = 0; w < RW; ++w) {
         const int rr = ((rt * NW + wave) * RW + w) * 16 + lo;

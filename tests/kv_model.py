@@ -112,7 +112,7 @@ def attention(q, k, v, scale, position, causal):
     return out
 
 
-def bound(q, k, v, scale, f16):
+def bound(q, k, v, scale, f16, i8=False):
     """How far f32 arithmetic may be from attention(), per element, relative to
     the largest |value|.
 
@@ -123,10 +123,18 @@ def bound(q, k, v, scale, f16):
     relative error, plus 2^-22 for exp2 and 2^-22 for the two fp16 that stand for
     it (fp16 output: 2^-11 for the one). Numerator and denominator each take it
     once, and add `keys` numbers (2^-24 each, at most). An fp16 output rounds by
-    2^-11 of itself; an f32 one by the quotient's 2 roundings."""
+    2^-11 of itself; an f32 one by the quotient's 2 roundings.
+
+    fp16 output over i8 codes may take the products of u = code + 128 instead and
+    128 times the sum of the other operand off them. u ks is below 2.01 of the
+    block's largest |k|, so a score's d additions add at most 3.02 of it times the
+    sum of |q| (u's and the sum's own); the numerator's of u and of the weights
+    come to 3.02 keys in place of 1."""
     d, keys = q.shape[2], k.shape[1]
     q, k = np.abs(q.astype(np.float64)), np.abs(k.astype(np.float64))
     group = len(q) // len(k)
     s = max(float((q[h] @ k[h // group].T).max()) for h in range(len(q))) * scale * 1.4427
+    more = 3.02 * float(k.max() * q.sum(axis=2).max()) * scale * 1.4427 if f16 and i8 else 0.0
+    s, sums = s + more, 2 if not more else 4.02
     weight = np.log(2.0) * ((d + 3) * 2.0 ** -24 * s + 2.0 ** -15) + 2.0 ** -22 + (2.0 ** -11 if f16 else 2.0 ** -22)
-    return 2 * weight + 2 * keys * 2.0 ** -24 + (2.0 ** -11 if f16 else 2.0 ** -22)
+    return 2 * weight + sums * keys * 2.0 ** -24 + (2.0 ** -11 if f16 else 2.0 ** -22)

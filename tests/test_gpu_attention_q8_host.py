@@ -32,7 +32,7 @@ class HostPair:
         say(f"qh={qh} kh={kh} d={d} {fmt} block={block} noncausal={noncausal} seed={seed}")
         self.be = backend or npu.Backend(npu.ModelOptions(chunk=chunk, context=context))
         self.scale = float(np.float32(d ** -0.5))
-        self.qh, self.kh, self.d, self.noncausal = qh, kh, d, noncausal
+        self.qh, self.kh, self.d, self.noncausal, self.i8 = qh, kh, d, noncausal, fmt == "i8"
         self.att = self.be.attention_q8(qh, kh, d, d ** -0.5, fmt, block, noncausal)
         self.k, self.v = (kv_model.KvModel(kh, d, fmt, block) for _ in range(2))
         self.rng = np.random.default_rng(seed)
@@ -69,7 +69,7 @@ class HostPair:
         """q, out [qh][rows][d]."""
         k, v = self.k.values(), self.v.values()
         want = kv_model.attention(q, k, v, self.scale, position, not self.noncausal)
-        most = kv_model.bound(q, k, v, self.scale, f16) * np.abs(v).max()
+        most = kv_model.bound(q, k, v, self.scale, f16, self.i8) * np.abs(v).max()
         assert np.abs(out.astype(np.float64) - want).max() <= most
 
 

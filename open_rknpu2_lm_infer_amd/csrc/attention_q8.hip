@@ -466,7 +466,7 @@ struct Q8Cache {
     size_t code_bytes, scale_bytes, kept_bytes;  // of one array each
     uint64_t generation;
     Q8Rows rows;
-    std::shared_mutex mu;  // the fields above against calls from several threads; a host run holds it (shared) to its end
+    std::shared_mutex mu;  // the fields above, against calls from several threads; a host run holds it to its end
     DevFence fence;  // device-path appends, reads and runs
     hipStream_t stream = nullptr;  // host-buffer appends and reads (created on the first)
     HostStage hs;                  // their pinned staging
@@ -710,21 +710,25 @@ static Q8Plan q8_plan(int D, int R, int kv_heads, int units, bool i8, bool f16) 
 
 // Key splits: a block for each CU, but no more, as a block's rows leave partials (512
 // rows of 8 heads over 4096 keys 21.9 us, 27.6 with 512 blocks, 25.5 with 128; one row
-// of 16 heads over 2 of 256 and 20000 keys 11.3, 16.2 with 512). A split holds at least a
-// unit for each wave, or two stages. Few keys are not split: a wave walks its 4 to 6
-// units in the time of the join's launch, 3 us. One row of 32 heads over 8 of 128:
-// 768 keys 6.5, split 7.1, 1000 keys 8.5 and 7.7; of 16 over 2 of 256: 480 keys 7.4 and
-// 7.9, 768 keys 9.3 and 8.2; 64 rows of 32 over 8 of 128 (8 waves): 1000 keys 11.2 and
-// 12.8, 1500 keys 13.7 and 13.5.
+// of 16 heads over 2 of 256 and 20000 keys 11.3, 16.2 with 512). 4 waves of 64 dims have
+// too few bytes on their way for a CU, which two blocks make up for once they are long
+// (one row of 16 heads over 8 of 64: 300000 keys 55 us, 76 with 256 blocks, 40000 13.5
+// and 14.5, 20000 9.6 and 9.7; over 2: 131000 12.7 and 12.8, 65000 10.4 and 9.6).
+// A split holds at least a unit for each wave, or two stages. Few keys are not split: a
+// wave walks its 4 to 6 units in the time of the join's launch, 3 us. One row of 32
+// heads over 8 of 128: 768 keys 6.5, split 7.1, 1000 keys 8.5 and 7.7; of 16 over 2 of
+// 256: 480 keys 7.4 and 7.9, 768 keys 9.3 and 8.2; 64 rows of 32 over 8 of 128 (8
+// waves): 1000 keys 11.2 and 12.8, 1500 keys 13.7 and 13.5.
 static void q8_splits(AttnQ8Params& P, int D, int R, const Q8Plan& plan) {
     const int rows = plan.rows();
     P.row_tiles = (R + rows - 1) / rows;
     P.rows_pad = P.row_tiles * rows;
-    const int base = P.row_tiles * P.kh, least = plan.tile ? 4 : plan.waves, blocks = 256;
+    const int base = P.row_tiles * P.kh, least = plan.tile ? 4 : plan.waves;
+    const int blocks = D == 64 && plan.waves == 4 && (long)P.units * base > 32 * 256 ? 512 : 256;
     const int few = D == 256 ? 16 : plan.waves == 4 ? 24 : 32;
     const size_t room = attn_partial_rows(D) / ((size_t)P.rows_pad * P.kh);
     int want = std::max(1, std::min((blocks + base - 1) / base, (P.units + least - 1) / least));
-    want = (int)std::min<size_t>(want, std::max<size_t>(1, room));
+    want = (int)std::min<size_t>(std::min(want, Q8_MAX_SPLITS), std::max<size_t>(1, room));
     if (P.units <= few) want = 1;
     P.units_per_split = ((P.units + want - 1) / want + least - 1) / least * least;
     P.splits = (P.units + P.units_per_split - 1) / P.units_per_split;

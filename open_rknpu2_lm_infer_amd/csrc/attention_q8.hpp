@@ -28,6 +28,7 @@
 namespace hm {
 
 constexpr int Q8_SLOTS = 3;  // fp16 blocks kept
+constexpr int Q8_MAX_SPLITS = 256;  // key splits that a row's join takes
 
 struct AttnQ8Params {
     const void* q;
@@ -876,9 +877,9 @@ __global__ __launch_bounds__(64 * NW) void attn_q8_tile_kernel(AttnQ8Params P) {
 // over the GS groups meet in LDS.
 template <int D, int RPB, int DB>
 __global__ __launch_bounds__(256) void attn_q8_combine_kernel(AttnQ8Params P) {
-    constexpr int T = 256 / RPB, LD = DB / 4, GS = T / LD, B = 8;
+    constexpr int T = 256 / RPB, LD = DB / 4, GS = T / LD, B = 8, W = Q8_MAX_SPLITS / T;
     static_assert(GS >= 1 && T % LD == 0, "threads per row");
-    __shared__ float weight[RPB][256];
+    __shared__ float weight[RPB][Q8_MAX_SPLITS];
     __shared__ float red[RPB][2][T / 32];
     __shared__ q8_f4 part[RPB][GS][LD];
     const int row = threadIdx.x / T, t = threadIdx.x % T, d4 = t % LD, gs = t / LD, g = blockIdx.y;
@@ -892,10 +893,10 @@ __global__ __launch_bounds__(256) void attn_q8_combine_kernel(AttnQ8Params P) {
     for (int i = 0; i < B; ++i) v[i] = acc[(size_t)min(gs + i * GS, S - 1) * (D / 4)];
     // weights and denominator, over the row's threads (whole half waves)
     const float2* ml = reinterpret_cast<const float2*>(P.part + (size_t)P.kh * P.rows_pad * S * D) + at;
-    float2 x[256 / T];
+    float2 x[W];
     float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 256 / T; ++i) {
+    for (int i = 0; i < W; ++i) {
         x[i] = t + i * T < S ? ml[t + i * T] : float2{-INFINITY, 0.0f};
         top = fmaxf(top, x[i].x);
     }
@@ -907,7 +908,7 @@ __global__ __launch_bounds__(256) void attn_q8_combine_kernel(AttnQ8Params P) {
     for (int i = 0; i < T / 32; ++i) top = fmaxf(top, red[row][0][i]);
     float den = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 256 / T; ++i) {
+    for (int i = 0; i < W; ++i) {
         const float w = q8_weight(x[i].x, top);
         weight[row][t + i * T] = w;
         // (a split that saw NaN scores has maximum -inf and a NaN sum)

@@ -511,6 +511,28 @@ def test_captured_step_replays(ctx):
         p.check_contents()
 
 
+@pytest.mark.parametrize("kh,n", [(1, 270001), (8, 33100)])
+def test_narrow_heads_over_many_keys(ctx, kh, n):
+    """Heads of 64 over keys enough for two blocks a CU: 256 splits of one head (the
+    most there are) and 64 of eight; against 64 bits of the values read."""
+    print(f"kh={kh} keys={n}", flush=True)
+    cache = D.KvCacheQ8(ctx, 2 * kh, kh, 64, 0.125, n, fmt="e4m3", max_query_rows=4)
+    x = torch.randn(kh, n, 64, device="cuda", dtype=torch.float16)
+    cache.append(x, torch.randn_like(x))
+    k, v = (torch.empty(kh, n, 64, device="cuda") for _ in range(2))
+    cache.read(0, k, v)
+    q = torch.randn(2 * kh, 4, 64, device="cuda", dtype=torch.float16)
+    out = torch.empty(2 * kh, 4, 64, device="cuda")
+    D.attention_q8(ctx, cache, q, out, n - 4)
+    for h in (0, 2 * kh - 1):
+        for r in (0, 3):
+            seen = n - 3 + r
+            score = (k[h // 2, :seen].double() * q[h, r].double()).sum(1) * 0.125
+            want = (torch.softmax(score, 0)[:, None] * v[h // 2, :seen].double()).sum(0)
+            most = kv_model.bound(q[h:h + 1, r:r + 1].cpu().numpy(), k[h // 2:h // 2 + 1].cpu().numpy(), None, 0.125, False)
+            assert float((out[h, r].double() - want).abs().max()) <= most * float(v.abs().max())
+
+
 @pytest.mark.parametrize("d,kh", [(64, 16), (128, 8), (256, 4)])
 def test_long_averages_of_f16_output(ctx, d, kh):
     """Equal weights over many keys in one split, where sums of offset codes would

@@ -148,26 +148,37 @@ __device__ __forceinline__ float q8_weight(float m, float top) {
     return fmaxf(__builtin_amdgcn_exp2f(m - top), 0x1p-120f);
 }
 
-constexpr float Q8_LAZY = 8.0f;   // a row's maximum moves when a score passes it by this much (powers of 2)
-constexpr float Q8_SHIFT = 6.0f;  // SPLIT: the weights lie this much higher (p below 2^14, p mu below 2^15)
+// A row's maximum moves when a score passes it by LAZY (powers of 2), to SHIFT below
+// the score: weights lie below 2^15, the row's largest above 2^5 (SPLIT) or 2^9. More of
+// fp16's range for the small ones costs more moves: 1024 rows of 8 heads of 128 over
+// 32768 keys, SPLIT with 4 and 10 207 us instead of 198; else with 4 and 11 153 instead
+// of 146, with 8 and 7 145.
+constexpr float q8_lazy(bool split) { return split ? 8.0f : 6.0f; }
+constexpr float q8_shift(bool split) { return split ? 6.0f : 9.0f; }
 
 // A wave's query rows, RW groups of 16 (lane l: row l % 16 of each): their key
 // limits, queries, running maxima (less SHIFT), sums and accumulators (lane l:
 // dims 16 n + 4 (l / 16)..+3).
 //
 // With c = scale log2(e) and a block's scales ks and vs = mu 2^e, a key's weight
-// is kept as p = 2^(c ks s + e - m): e in the exponent keeps the products p mu
-// code of different blocks in one range, whatever their scales, so fp16 holds
-// them. The row's sum adds p 2^-e, its accumulators p mu code; m is the running
-// maximum, a whole number with SPLIT so that e - m is exact.
+// is kept as p = 2^(c ks s + e - m): e in the exponent gives the products p mu code
+// of different blocks one unit, which fp16 operands need. The row's accumulators add
+// p mu code, its sum p 2^-e; m is the running maximum, a whole number with SPLIT so
+// that e - m is exact.
 //
-// SPLIT (f32 output): p mu goes into the products as two fp16, 22 bits.
-// Otherwise (fp16 output) as one, and the sum adds the rounded weights (times
-// 1 / vs), so that a row whose weight is all on one key is not off.
+// p follows V's scale, not only the softmax weight, so a key of small values may be
+// among the row's smallest p and hold the row's largest softmax weight: the sum takes
+// p in f32, before any rounding. (The sum of the fp16 weights lost such keys: 17 % off
+// where half of the weight had 2^-24 of the other half's scale.)
+//
+// SPLIT (f32 output): p mu goes into the products as two fp16, 22 bits. Otherwise
+// (fp16 output) p mu goes in as one, mu in the exponent. fp16 has fewer bits below
+// 2^-14, and 2^-25 is lost: a weight times scale is off by 2^-30 (fp16 output: 2^-34)
+// of the row's largest at most.
 //
 // RAW (i8, fp16 output, two row groups a wave): codes come as u 2^-24, u = code + 128,
 // half the instructions of their conversion (512 rows of 8 heads over 8000 keys of 128
-// 28.6 us instead of 34.1; one row group's waves wait for memory). Scores start from
+// 28.4 us instead of 34.1; one row group's waves wait for memory). Scores start from
 // -128 2^-24 sum(q); `vsum` adds the weights as they are multiplied, and every 16 units
 // 128 2^-24 of it leaves the accumulators, which else would grow with every key where
 // sums of codes walk: over 44000 keys in one split outputs were 3.2e-4 off instead of
@@ -177,7 +188,7 @@ template <int D, int RW, bool SPLIT, bool RAW = false>
 struct Q8Wave {
     static_assert(!(SPLIT && RAW), "offset codes are for fp16 output");
     static constexpr int KS = D / 32, NB = D / 16;
-    static constexpr float SHIFT = SPLIT ? Q8_SHIFT : 0.0f;
+    static constexpr float LAZY = q8_lazy(SPLIT), SHIFT = q8_shift(SPLIT);
     int lim[RW];
     int open, seen;  // keys below `open` every row sees, from `seen` on none
     q8_h8 qf[RW][KS];
@@ -288,7 +299,7 @@ struct Q8Wave {
                 }
     }
     // The rows' largest scores of a unit, in the maxima's units, and whether one
-    // passes its row's maximum by more than Q8_LAZY.
+    // passes its row's maximum by more than LAZY.
     __device__ __forceinline__ bool over(const Unit& x, const q8_f4 (&s)[RW][2], float (&top)[RW]) const {
         bool any = false;
 #pragma unroll
@@ -299,7 +310,7 @@ struct Q8Wave {
                 __builtin_elementwise_maximum(__builtin_elementwise_maximum(s[w][1][0], s[w][1][1]),
                                               __builtin_elementwise_maximum(s[w][1][2], s[w][1][3])));
             top[w] = __builtin_fmaf(top[w], x.cks, x.lg);
-            any |= top[w] > mrun[w] + (Q8_LAZY + SHIFT);
+            any |= top[w] > mrun[w] + (LAZY + SHIFT);
         }
         return any;
     }
@@ -308,9 +319,9 @@ struct Q8Wave {
 #pragma unroll
         for (int w = 0; w < RW; ++w) {
             float tm = q8_rows4_max(top[w]);
-            if constexpr (SPLIT) tm = __builtin_ceilf(tm) - SHIFT;
+            tm = (SPLIT ? __builtin_ceilf(tm) : tm) - SHIFT;
             float alpha = 1.0f;
-            if (tm > mrun[w] + Q8_LAZY) {
+            if (tm > mrun[w] + LAZY) {
                 alpha = __builtin_amdgcn_exp2f(mrun[w] - tm);
                 mrun[w] = tm;
             }
@@ -327,7 +338,7 @@ struct Q8Wave {
 #pragma unroll
         for (int w = 0; w < RW; ++w) {
             const float b = x.lg - mrun[w];
-            float l[2] = {0.0f, 0.0f};
+            float l[2] = {0.0f, 0.0f}, taken[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
@@ -342,16 +353,17 @@ struct Q8Wave {
                         ph[w][4 * cb + r + 1] = h[1];
                         pl[w][4 * cb + r] = d[0];
                         pl[w][4 * cb + r + 1] = d[1];
-                        l[cb] += p0 + p1;
                     } else {
                         const q8_h2 h = q8_round2(p0, p1);
                         ph[w][4 * cb + r] = h[0];
                         ph[w][4 * cb + r + 1] = h[1];
-                        l[cb] = __builtin_amdgcn_fdot2(h, q8_h2{(_Float16)1.0f, (_Float16)1.0f}, l[cb], false);
+                        if constexpr (BYTES)
+                            taken[cb] = __builtin_amdgcn_fdot2(h, q8_h2{(_Float16)1.0f, (_Float16)1.0f}, taken[cb], false);
                     }
+                    l[cb] += p0 + p1;
                 }
             lsum[w] = __builtin_fmaf(l[0] + l[1], x.part, lsum[w]);
-            if constexpr (BYTES) vsum[w] += l[0] + l[1];
+            if constexpr (BYTES) vsum[w] += taken[0] + taken[1];
         }
     }
     __device__ __forceinline__ void product(int n, q8_h8 a, const q8_h8 (&ph)[RW], const q8_h8 (&pl)[RW]) {

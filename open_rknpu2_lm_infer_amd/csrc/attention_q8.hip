@@ -685,23 +685,23 @@ static void q8_combine(const AttnQ8Params& P, int R, hipStream_t s) {
 //
 // attn_q8_tile_kernel converts once a block, which takes rows enough to fill 128- or
 // 256-row blocks and keys enough to fill its stages; the more, the cheaper the
-// conversion. `cross`: where they do, in million rows x keys x dims a CU. Measured,
-// us, two row groups in every wave and once a block, 8 KV heads (256 dims: 2):
-//   128 dims, i8, f32 output: 1024 rows x 8000 keys (33) 57.4 and 64.8, x 16000 (66) 112
-//   and 106, 256 x 32000 (33) 65.3 and 66.7; e4m3: 1024 x 16000 99.0 and 104, x 32000
-//   195 and 188, f16 output 75.6 and 82.5, 149 and 145; i8, f16 output: x 16000 74.4 and
-//   83.4, x 32000 143 and 147, x 64000 280 and 269;
-//   64 dims, i8, f32: 256 x 32000 (16) 47.7 and 46.7, 1024 x 16000 (33) 76.7 and 78.6, x
-//   32000 149 and 136; e4m3: x 16000 69.1 and 78.6, x 32000 136 and 136, f16 103 and 101;
-//   i8, f16: x 32000 102 and 102, x 64000 204 and 186;
-//   256 dims, i8, f32: 512 x 32000 (33) 68.6 and 69.3, x 64000 122 and 116; e4m3: 110 and
-//   110, f16 87.9 and 90.9, 2048 x 32000 (131) 158 and 152; i8, f16: x 64000 (262) 288
-//   and 295.
+// conversion. `cross`: where they do, in million rows x keys x dims a CU; the more rows
+// for the same work the later. Measured, us, in every wave and once a block, 8 KV heads
+// (256 dims: 2), 512 rows:
+//   64 dims, i8: 32000 keys (16) 37.6 and 41.8, 64000 (33) 67.4 and 60.2; f32 output 46.3
+//   and 49.5, 84.6 and 76.3; e4m3: (33) 62.0 and 59.7, (66) 114 and 103, but 1024 rows (33)
+//   54.8 and 62.7, (66) 104 and 103; f32: (33) 77.8 and 74.1, 1024 rows 71.0 and 77.2;
+//   128 dims, i8: 16000 (33) 53.6 and 52.0, 1024 rows 45.2 and 54.6, (66) 88.6 and 83.7;
+//   f32: 65.1 and 63.8, 59.4 and 65.2, 115 and 108; e4m3: (33) 48.7 and 50.6, (66) 84.1 and
+//   80.9, 1024 rows 79.5 and 81.6, (131) 151 and 140; f32: (66) 111 and 106, 102 and 106;
+//   256 dims, 1024 rows, i8: 8000 (16) 35.3 and 37.8, (33) 57.1 and 55.7, (66) 100 and 91;
+//   f32: 40.8 and 43.2, 67.7 and 65.2; e4m3: (33) 50.6 and 54.2, (66) 87.2 and 88.8, (131)
+//   159 and 157; f32: 61.4 and 63.9, 110 and 106.
 static Q8Plan q8_plan(int D, int R, int kv_heads, int units, bool i8, bool f16) {
-    static const float cross[3][3] = {{28, 45, 33}, {55, 95, 63}, {60, 180, 250}};  // by head_dim 64, 128, 256
+    static const float cross[3][3] = {{30, 45, 33}, {45, 70, 60}, {55, 70, 100}};  // by head_dim 64, 128, 256
     const int forced = attention_q8_tile_switch();
     const double work = 1e-6 * D * R * kv_heads * units * 32 / device_cus();
-    const double most = cross[!i8 ? 1 : f16 ? 2 : 0][D / 128];
+    const double most = cross[i8 ? 0 : f16 ? 2 : 1][D / 128];
     if (forced == 1 || (forced < 0 && R > 16 && work > most)) return Q8Plan{true, D == 256 ? 1 : 2, 8};
     if (R <= 16) return Q8Plan{false, 1, 4};
     if (D < 256) return Q8Plan{false, 2, 8};

@@ -59,7 +59,11 @@ typedef _Float16 q8_h2 __attribute__((ext_vector_type(2)));
 typedef float q8_f4 __attribute__((ext_vector_type(4)));
 
 // 8 codes (two words) to 8 fp16, exactly. i8: a byte u = code + 128 under 0x64
-// is the fp16 1024 + u. e4m3: the conversion instruction.
+// is the fp16 1024 + u. e4m3: the conversion instruction. (i8 without the subtraction, a
+// byte under 0x00 as the fp16 u 2^-24 and 128 times the weights' sum taken off at the
+// end: 512 rows of 8 heads over 8000 keys of 128 28.7 us instead of 30.9, but beside that
+// offset the values of light keys are lost. With a key of no value 10 above the others'
+// scores, outputs were 3 % off.)
 template <int FMT>
 __device__ __forceinline__ q8_h8 q8_halves(unsigned lo, unsigned hi) {
     unsigned w[4];
@@ -78,20 +82,6 @@ __device__ __forceinline__ q8_h8 q8_halves(unsigned lo, unsigned hi) {
         w[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true));
     }
     return __builtin_bit_cast(q8_h8, v4u{w[0], w[1], w[2], w[3]});
-}
-
-// The same codes of the i8 format as they are stored, u = code + 128, half the
-// instructions: a byte under 0x00 is the fp16 u 2^-24. What that adds, 128 2^-24 times
-// the sum of the other operand, is taken off the sums (Q8Wave, RAW).
-__device__ __forceinline__ q8_h8 q8_bytes(unsigned w0, unsigned w1) {
-    const v4u x = {__builtin_amdgcn_perm(0u, w0, 0x0C010C00u), __builtin_amdgcn_perm(0u, w0, 0x0C030C02u),
-                   __builtin_amdgcn_perm(0u, w1, 0x0C010C00u), __builtin_amdgcn_perm(0u, w1, 0x0C030C02u)};
-    return __builtin_bit_cast(q8_h8, x);
-}
-template <int FMT, bool RAW>
-__device__ __forceinline__ q8_h8 q8_operand(unsigned w0, unsigned w1) {
-    if constexpr (RAW) return q8_bytes(w0, w1);
-    return q8_halves<FMT>(w0, w1);
 }
 
 // Two f32 to fp16, once: without the empty asm the compiler folds the product
@@ -175,24 +165,14 @@ constexpr float q8_shift(bool split) { return split ? 6.0f : 9.0f; }
 // (fp16 output) p mu goes in as one, mu in the exponent. fp16 has fewer bits below
 // 2^-14, and 2^-25 is lost: a weight times scale is off by 2^-30 (fp16 output: 2^-34)
 // of the row's largest at most.
-//
-// RAW (i8, fp16 output, two row groups a wave): codes come as u 2^-24, u = code + 128,
-// half the instructions of their conversion (512 rows of 8 heads over 8000 keys of 128
-// 28.4 us instead of 34.1; one row group's waves wait for memory). Scores start from
-// -128 2^-24 sum(q); `vsum` adds the weights as they are multiplied, and every 16 units
-// 128 2^-24 of it leaves the accumulators, which else would grow with every key where
-// sums of codes walk: over 44000 keys in one split outputs were 3.2e-4 off instead of
-// 2.9e-4 (relative, fp16's rounding 2.1e-4). The 2^24 goes into cks and e. f32 output
-// has no room for it.
-template <int D, int RW, bool SPLIT, bool RAW = false>
+template <int D, int RW, bool SPLIT>
 struct Q8Wave {
-    static_assert(!(SPLIT && RAW), "offset codes are for fp16 output");
     static constexpr int KS = D / 32, NB = D / 16;
     static constexpr float LAZY = q8_lazy(SPLIT), SHIFT = q8_shift(SPLIT);
     int lim[RW];
     int open, seen;  // keys below `open` every row sees, from `seen` on none
     q8_h8 qf[RW][KS];
-    float mrun[RW], lsum[RW], vsum[RW], base[RW];
+    float mrun[RW], lsum[RW];
     q8_f4 o[RW][NB];
 
     // Rows r0 + 16 w + lane % 16 of KV head g. Rows from R on are computed as the
@@ -217,7 +197,7 @@ struct Q8Wave {
                 seen = max(seen, lim[w]);
             }
             mrun[w] = Q8_NONE;
-            lsum[w] = vsum[w] = base[w] = 0.0f;
+            lsum[w] = 0.0f;
         }
         if (!P.q_f32) {
 #pragma unroll
@@ -241,18 +221,6 @@ struct Q8Wave {
                     for (int i = 0; i < 8; ++i) qf[w][s][i] = (_Float16)x[s][i >> 2][i & 3];
             }
         }
-        if constexpr (RAW) {
-            q8_h8 off;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) off[i] = (_Float16)-0x1p-17f;
-#pragma unroll
-            for (int w = 0; w < RW; ++w) {
-                q8_f4 sum = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int i = 0; i < KS; ++i) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(off, qf[w][i], sum, 0, 0, 0);
-                base[w] = sum[0];
-            }
-        }
         open = __builtin_amdgcn_readfirstlane(q8_row_min(open));
         seen = -__builtin_amdgcn_readfirstlane(q8_row_min(-seen));
     }
@@ -271,15 +239,13 @@ struct Q8Wave {
     struct Unit {
         float cks, lg, mu, part;  // part: what a weight's sum is multiplied with
     };
-    template <bool BYTES = false>
     static __device__ __forceinline__ Unit unit(float c, float ks, float mu, int e, float inv) {
         const bool poison = ks != ks || mu != mu;
         Unit x;
-        x.cks = poison ? NAN : fmaxf(c * ks, 0x1p-120f) * (BYTES ? 0x1p24f : 1.0f);
+        x.cks = poison ? NAN : fmaxf(c * ks, 0x1p-120f);
         x.mu = poison ? 1.0f : mu;
-        x.lg = SPLIT ? (float)e : (float)(e + (BYTES ? 24 : 0)) + __builtin_amdgcn_logf(x.mu);
+        x.lg = SPLIT ? (float)e : (float)e + __builtin_amdgcn_logf(x.mu);
         x.part = SPLIT ? __int_as_float((127 - e) << 23) : poison ? 1.0f : inv;  // 2^-e, 1 / (mu 2^e)
-        if (BYTES) x.part *= 0x1p-24f;
         return x;
     }
     // Masked scores become -inf; where there are some, those of a poisoned block
@@ -327,18 +293,16 @@ struct Q8Wave {
             }
             if constexpr (FIRST) continue;
             lsum[w] *= alpha;
-            vsum[w] *= alpha;
 #pragma unroll
             for (int n = 0; n < NB; ++n) o[w][n] *= alpha;
         }
     }
     // Scores to weights ph (and pl), and the rows' sums.
-    template <bool BYTES = false>
     __device__ __forceinline__ void weigh(const Unit& x, const q8_f4 (&s)[RW][2], q8_h8 (&ph)[RW], q8_h8 (&pl)[RW]) {
 #pragma unroll
         for (int w = 0; w < RW; ++w) {
             const float b = x.lg - mrun[w];
-            float l[2] = {0.0f, 0.0f}, taken[2] = {0.0f, 0.0f};
+            float l[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
@@ -357,13 +321,10 @@ struct Q8Wave {
                         const q8_h2 h = q8_round2(p0, p1);
                         ph[w][4 * cb + r] = h[0];
                         ph[w][4 * cb + r + 1] = h[1];
-                        if constexpr (BYTES)
-                            taken[cb] = __builtin_amdgcn_fdot2(h, q8_h2{(_Float16)1.0f, (_Float16)1.0f}, taken[cb], false);
                     }
                     l[cb] += p0 + p1;
                 }
             lsum[w] = __builtin_fmaf(l[0] + l[1], x.part, lsum[w]);
-            if constexpr (BYTES) vsum[w] += taken[0] + taken[1];
         }
     }
     __device__ __forceinline__ void product(int n, q8_h8 a, const q8_h8 (&ph)[RW], const q8_h8 (&pl)[RW]) {
@@ -447,28 +408,7 @@ struct Q8Wave {
             for (int i = 0; i < 8; ++i) a[i] = (_Float16)((float)a[i] * up);
             product(n, a, ph, pl);
         }
-        if constexpr (RAW) {  // (to the units of u 2^-24)
-            static_assert(FIRST || !RAW, "the open block first");
-#pragma unroll
-            for (int w = 0; w < RW; ++w) {
-                mrun[w] += 24.0f;
-                lsum[w] *= 0x1p-24f;
-#pragma unroll
-                for (int n = 0; n < NB; ++n) o[w][n] *= 0x1p-24f;
-            }
-        }
         return __builtin_amdgcn_ballot_w64(wild != 0) != 0;
-    }
-    // RAW: the accumulators of codes.
-    __device__ __forceinline__ void centre() {
-        if constexpr (!RAW) return;
-#pragma unroll
-        for (int w = 0; w < RW; ++w) {
-            const float off = -0x1p-17f * q8_rows4_sum(vsum[w]);
-            vsum[w] = 0.0f;
-#pragma unroll
-            for (int n = 0; n < NB; ++n) o[w][n] += off;
-        }
     }
     // The sums of a row's 4 lanes.
     __device__ __forceinline__ void sums() {
@@ -622,8 +562,7 @@ __global__ __launch_bounds__(64 * NW) void attn_q8_kernel(AttnQ8Params P) {
     const int u_tail = u_begin + (max(coded_units - u_begin, 0) + NW - 1) / NW * NW;
     const bool late = D == 256 && u_tail < min((split + 1) * P.units_per_split, P.units);
     if (!late) first();
-    constexpr bool RAW = FMT == RK_NPU_HIP_KV_I8 && !SPLIT && RW > 1;
-    Q8Wave<D, RW, SPLIT, RAW> W;
+    Q8Wave<D, RW, SPLIT> W;
     W.start(P, g, rt * RT, lo, hi);
     const int u_end = min(min((split + 1) * P.units_per_split, P.units), (W.seen + 31) >> 5);
     const int coded_end = min(u_end, coded_units);
@@ -636,15 +575,15 @@ __global__ __launch_bounds__(64 * NW) void attn_q8_kernel(AttnQ8Params P) {
     for (int u = u_begin; u < coded_end; u += NW) {
         q8_f4 s[RW][2];
 #pragma unroll
-        for (int w = 0; w < RW; ++w) s[w][0] = s[w][1] = q8_f4{W.base[w], W.base[w], W.base[w], W.base[w]};
+        for (int w = 0; w < RW; ++w) s[w][0] = s[w][1] = q8_f4{0.0f, 0.0f, 0.0f, 0.0f};
         const float4 x = next;
         const bool more = u + NW < coded_end;
         if (more) next = sc[(u + NW) >> P.unit_shift];
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
             const int cb = i / (D / 64), st = i % (D / 64);
-            const q8_h8 a0 = q8_operand<FMT, RAW>(kr[i][0], kr[i][1]);
-            const q8_h8 a1 = q8_operand<FMT, RAW>(kr[i][2], kr[i][3]);
+            const q8_h8 a0 = q8_halves<FMT>(kr[i][0], kr[i][1]);
+            const q8_h8 a1 = q8_halves<FMT>(kr[i][2], kr[i][3]);
 #pragma unroll
             for (int w = 0; w < RW; ++w) {
                 s[w][cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, W.qf[w][2 * st], s[w][cb], 0, 0, 0);
@@ -653,20 +592,18 @@ __global__ __launch_bounds__(64 * NW) void attn_q8_kernel(AttnQ8Params P) {
         }
         if (more) load_k(u + NW);
         q8_h8 ph[RW], pl[RW];
-        auto un = W.template unit<RAW>(c, x.x, x.y, __float_as_int(x.z), x.w);
+        auto un = W.unit(c, x.x, x.y, __float_as_int(x.z), x.w);
         if (__builtin_expect(W.masked(u << 5, false), 0)) W.mask(un, u << 5, false, hi, s);  // (uniform)
         float top[RW];
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(W.over(un, s, top)) != 0, 0)) W.raise(top);
-        W.template weigh<RAW>(un, s, ph, pl);
+        W.weigh(un, s, ph, pl);
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
-            W.product(2 * i, q8_operand<FMT, RAW>(vr[i][0], vr[i][1]), ph, pl);
-            W.product(2 * i + 1, q8_operand<FMT, RAW>(vr[i][2], vr[i][3]), ph, pl);
+            W.product(2 * i, q8_halves<FMT>(vr[i][0], vr[i][1]), ph, pl);
+            W.product(2 * i + 1, q8_halves<FMT>(vr[i][2], vr[i][3]), ph, pl);
         }
         if (more) load_v(u + NW);
-        if (RAW && (u - u_begin) % (16 * NW) == 15 * NW) W.centre();
     }
-    W.centre();
     W.sums();
     if (wild) W.wild(P, g, u_tail, u_tail + 1, lane);
     q8_meet<D, NW, RW>(P, W, g, rt, split, wave, lane, smem, ml);

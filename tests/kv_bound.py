@@ -19,7 +19,7 @@ def steps(model):
     return np.concatenate(parts, axis=1)[:, :model.length]
 
 
-def attention(q, k, v, step, scale, position, causal, f16, i8):
+def attention(q, k, v, step, scale, position, causal, f16):
     """softmax(scale q k) v in float64 and how far each output may be off. q
     [qh][rows][d] fp16, k and v [kh][keys][d] f32, finite; step: steps().
 
@@ -35,10 +35,6 @@ def attention(q, k, v, step, scale, position, causal, f16, i8):
     - what goes into the products is a weight times its V scale, in units that keep
       the row's largest above 2^9 (f32 output: 2^5); below 2^-14 it is off by up to
       2^-25 instead;
-    - i8 codes of fp16 output may be taken as u = code + 128 <= 255, and 128 times the
-      sum of the other operand off their sums: u k's scale is below 2.01 of the
-      largest |k|, and the d additions of u's sum and of its own come to 3.02 of that;
-      the numerator adds 3.02 times `keys` numbers of 128 V scales each;
     - the output: 2^-11 of itself, or 2^-22 for the quotient. Products of two of
       these: 1 % of it all."""
     q, k, v = (x.astype(np.float64) for x in (q, k, v))
@@ -53,8 +49,6 @@ def attention(q, k, v, step, scale, position, causal, f16, i8):
         w = np.exp(s - s.max(axis=1, keepdims=True))
         w /= w.sum(axis=1, keepdims=True)
         size = np.where(seen, np.abs(q[h]) @ np.abs(k[g]).T, 0.0).max(axis=1) * to_bits
-        if f16 and i8:
-            size += 3.02 * np.abs(k[g]).max() * np.abs(q[h]).sum(axis=1) * to_bits
         out[h] = w @ v[g]
         size_v = w @ np.abs(v[g])
         weight = (np.log(2.0) * ((d + 5) * 2.0 ** -24 * size + 2.0 ** -15) + 2.0 ** -21)[:, None]
@@ -62,8 +56,6 @@ def attention(q, k, v, step, scale, position, causal, f16, i8):
         counts = np.divide(np.abs(v[g]), step[g][:, None], where=step[g][:, None] > 0, out=np.zeros_like(v[g]))
         most[h] = (2 * weight + (2.0 ** -11 if f16 else 2.0 ** -22) + 2 * n) * size_v
         most[h] += 2.0 ** (-34 if f16 else -30) * (w * step[g]).max(axis=1, keepdims=True) * (seen @ counts)
-        if f16 and i8:
-            most[h] += 3.02 * n * 128.0 * (w @ step[g])[:, None]
         most[h] += (2.0 ** -11 if f16 else 2.0 ** -22) * np.abs(out[h])
     return out, 1.01 * most + (2.0 ** -25 if f16 else 2.0 ** -149)
 
@@ -74,11 +66,12 @@ def wave(q, k, v, step, scale, f16, unit=32, plant=None):
     largest, f32 sums. plant: a mistake to find. "units": fp16 output's largest is at
     1 first, not at 2^9; "sum": the same, and the sum is that of the rounded weights;
     "zeros": a block of zeros takes part in the reference with scale 1; "drop": one
-    unit is left out."""
+    unit is left out; "offset": codes plus 128 are multiplied, and 128 times the sum of
+    the weights taken off at the end."""
     f32 = np.float32
     s = (k.astype(np.float64) @ q.astype(np.float64)) * scale * np.log2(np.e)
     shift, lazy = (0.0 if plant in ("units", "sum") else 9.0, 6.0) if f16 else (6.0, 8.0)
-    m, den, num = -1e30, 0.0, np.zeros(k.shape[1])
+    m, den, num, taken = -1e30, 0.0, np.zeros(k.shape[1]), 0.0
     for i, u in enumerate(range(0, len(s), unit)):
         if plant == "drop" and i == 1:
             continue
@@ -86,10 +79,15 @@ def wave(q, k, v, step, scale, f16, unit=32, plant=None):
         top = s[u:u + unit].max() + np.log2(vs)
         if top > m + lazy + shift:
             new = np.ceil(top) - shift
-            num, den, m = num * np.exp2(max(m - new, -2000.0)), den * np.exp2(max(m - new, -2000.0)), new
+            alpha = np.exp2(max(m - new, -2000.0))
+            num, den, taken, m = num * alpha, den * alpha, taken * alpha, new
         p = np.exp2(s[u:u + unit] + np.log2(vs) - m).astype(f32)
         high = p.astype(np.float16)
         used = high.astype(np.float64) if f16 else high + (p - high.astype(f32)).astype(np.float16).astype(np.float64)
         den += float((used if plant == "sum" else p.astype(np.float64)).sum()) / vs
-        num += used @ (v[u:u + unit].astype(np.float64) / vs)
-    return num / den
+        codes = v[u:u + unit].astype(np.float64) / vs
+        if plant == "offset":
+            num, taken = (num + used @ (codes + 128.0)).astype(f32).astype(np.float64), taken + used.sum()
+        else:
+            num += used @ codes
+    return (num - 128.0 * taken) / den

@@ -39,7 +39,7 @@ def check(ctx, appends, dtype, fmt="i8", block=32, causal=False, rows=1, qh=2, t
     with D.plan_switch("HM_Q8_TILE", tile):
         D.attention_q8(ctx, cache, torch.from_numpy(q).cuda(), out, n - rows)
     want, most = kv_bound.attention(q, k.values(), v.values(), kv_bound.steps(v), scale, n - rows, causal,
-                                    dtype == F16, fmt == "i8")
+                                    dtype == F16)
     got = out.double().cpu().numpy()
     worst = np.abs(got - want) / most
     assert worst.max() <= 1.0, f"{worst.max()} of the bound at {np.unravel_index(worst.argmax(), worst.shape)}"

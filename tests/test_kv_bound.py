@@ -16,7 +16,7 @@ def check(appends, f16, fmt="i8", d=64, plants=(), q=None):
     q = rng.standard_normal((1, 1, d)).astype(np.float16) if q is None else q[None, None]
     step = kv_bound.steps(v)
     x, y = k.values(), v.values()
-    want, most = kv_bound.attention(q, x, y, step, scale, 0, False, f16, False)
+    want, most = kv_bound.attention(q, x, y, step, scale, 0, False, f16)
 
     def off(plant=None):
         got = kv_bound.wave(q[0, 0], x[0], y[0], step[0], scale, f16, plant=plant)
@@ -52,7 +52,7 @@ def test_blocks_of_zeros(zeros_first, size, f16):
 def test_a_strong_key_of_no_value(gap, f16):
     rng = np.random.default_rng(gap)
     q = rng.standard_normal(64).astype(np.float16)
-    check(kv_cases.strong_key(rng, 1, 64, q, 0.125, gap), f16, q=q, plants=("units",) if f16 and gap >= 14 else ())
+    check(kv_cases.strong_key(rng, 1, 64, q, 0.125, gap), f16, q=q, plants=("units", "offset") if f16 and gap >= 14 else ())
 
 
 @pytest.mark.parametrize("f16", [False, True])

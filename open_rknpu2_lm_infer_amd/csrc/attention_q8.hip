@@ -234,15 +234,17 @@ __global__ __launch_bounds__(q8_write_threads(D, B)) void q8_write_kernel(Q8Writ
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NT / 64; ++i) big = max(big, red[i]);
+    // (zeros only: the smallest scale there is, which lifts no row's maximum)
+    big = max(big, 1u);
 
     Q8Quantiser Q;
     Q.most = FMT == RK_NPU_HIP_KV_I8 ? 127.0f : 448.0f;
     Q.poison = big >= 0x7C00u;
     const float a = __half2float(__ushort_as_half((unsigned short)big));
-    Q.a = Q.poison || big == 0 ? 1.0f : a;
+    Q.a = Q.poison ? 1.0f : a;
     Q.inv = 1.0f / Q.a;
     if (tid == 0) {
-        const float s = Q.poison ? NAN : big == 0 ? 1.0f : a / Q.most;
+        const float s = Q.poison ? NAN : a / Q.most;
         if (which == 0) {
             sc->x = s;
         } else {

@@ -9,8 +9,8 @@
 //      on, 8 keys each: 4 h..4 h + 3 and 16 + 4 h..+3 with h = lane / 16.
 // i8 codes are stored plus 128. The scales are one float4 per block and head:
 // K's scale, and V's as m 2^e with 1 <= m < 2: m, e (an int) and 1 / scale. A
-// block of zeros has scale 1 here; a poisoned one (an infinity or NaN came) has
-// NaN. The tail's fp16 rows lie in the same order with 8 values a lane and step.
+// block of zeros has the smallest scale, of fp16's least value; a poisoned one (an
+// infinity or NaN came) has NaN. The tail's fp16 rows lie in the same order with 8 values a lane and step.
 //
 // Operands of v_mfma_f32_16x16x32_f16: A lane l = row l % 16, k-slots
 // 8 (l / 16)..+7; B lane l = column l % 16, the same slots; C lane l = rows

@@ -37,7 +37,7 @@ def check(ctx, appends, dtype, fmt="i8", block=32, causal=False, rows=1, qh=2, t
     q = rng.standard_normal((qh, rows, d)).astype(np.float16) if q is None else np.broadcast_to(q, (qh, rows, d)).copy()
     out = torch.full((qh, rows, d), 77.0, dtype=dtype, device="cuda")
     with D.plan_switch("HM_Q8_TILE", tile):
-        D.attention_q8(ctx, cache, torch.from_numpy(q).cuda(), out, n - rows)
+        D.attention_q8(ctx, cache, torch.from_numpy(q).cuda(), out, max(n - rows, 0))
     want, most = kv_bound.attention(q, k.values(), v.values(), kv_bound.steps(v), scale, n - rows, causal,
                                     dtype == F16)
     got = out.double().cpu().numpy()
@@ -77,6 +77,28 @@ def test_a_strong_key_of_no_value(ctx, gap, dtype):
             rng = np.random.default_rng(gap)
             q = rng.standard_normal(64).astype(np.float16)
             check(ctx, kv_cases.strong_key(rng, 1, 64, q, 0.125, gap), dtype, fmt, rows=rows // 2, tile=tile, q=q)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("fmt,block", [("i8", 32), ("i8", 128), ("e4m3", 64)])
+@pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** -14, 1.0, 2000.0])
+@pytest.mark.parametrize("zeros_first", [True, False])
+def test_blocks_of_zeros(ctx, zeros_first, size, fmt, block, dtype):
+    """Half of the keys, and the tail, have values of zero: they take their share of
+    the weight and leave the others' values all of their bits, however small."""
+    for rows, tile in KERNELS[:3]:
+        rng = np.random.default_rng(3)
+        check(ctx, kv_cases.zeros(rng, 1, 64, size, zeros_first, tail=20), dtype, fmt, block, rows=rows // 2, tile=tile)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_only_zeros(ctx, dtype):
+    """No value anywhere: outputs of zero, exactly."""
+    for n in (20, 32, 300):
+        for rows, tile in KERNELS[:3]:
+            got = check(ctx, [(np.ones((1, n, 64), np.float16), np.zeros((1, n, 64), np.float16))], dtype,
+                        rows=rows // 2, tile=tile)
+            assert not got.any()
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])

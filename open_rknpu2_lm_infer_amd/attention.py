@@ -18,7 +18,7 @@ from typing import Optional
 import numpy as np
 
 from . import _ffi as F
-from .npu import NpuError, _Handle, check, ensure
+from .npu import NpuError, _Handle, check, ensure, int32
 
 
 def pack_half(values: np.ndarray) -> np.ndarray:
@@ -235,13 +235,15 @@ class AttentionQ8(Attention):
     def reserve(self, capacity: int) -> None:
         ensure(capacity <= self.backend.options.context, "8-bit KV context capacity exceeded")
         with self._lock:
-            check(F.lib().rk_npu_hip_attention_q8_cache_reserve(self.backend.ctx, self.cache.raw, capacity),
+            check(F.lib().rk_npu_hip_attention_q8_cache_reserve(self.backend.ctx, self.cache.raw,
+                                                                int32(capacity, "capacity")),
                   "reserve 8-bit KV cache")
 
     def read(self, first: int, rows: int):
         """The values of tokens first.., K and V, each [rows][kv_heads][head_dim] fp16."""
         kh, d = self.kv_heads, self.dimension
-        ensure(rows > 0, "8-bit KV read of no rows")
+        ensure(int32(rows, "rows") > 0, "8-bit KV read of no rows")
+        int32(first, "first")
         out = [np.empty((kh, rows, d), np.float16) for _ in range(2)]
         with self._lock:
             check(F.lib().rk_npu_hip_attention_q8_cache_read(self.backend.ctx, self.cache.raw, first, rows,
@@ -270,7 +272,7 @@ def q8_config(attention, fmt: str, block: int) -> F.rk_npu_hip_attention_q8_conf
     ensure(fmt in KV_FORMATS, f"KV format must be one of {sorted(KV_FORMATS)}")
     cfg = F.rk_npu_hip_attention_q8_config()
     F.lib().rk_npu_hip_attention_q8_config_init(ctypes.byref(cfg))
-    cfg.attention, cfg.format, cfg.block = attention, KV_FORMATS[fmt], block
+    cfg.attention, cfg.format, cfg.block = attention, KV_FORMATS[fmt], int32(block, "block")
     return cfg
 
 

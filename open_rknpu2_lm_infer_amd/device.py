@@ -11,7 +11,7 @@ from typing import Dict, List, Optional, Tuple
 
 from . import _ffi as F
 from .attention import KV_FORMATS
-from .npu import NpuError, _Handle, _Shared, check, ensure
+from .npu import NpuError, _Handle, _Shared, check, ensure, int32
 
 _DT = {}
 
@@ -184,13 +184,18 @@ class KvCacheQ8:
                  capacity: int, fmt: str = "i8", block: int = 32, causal: bool = True, max_query_rows: int = 128,
                  initial_capacity: Optional[int] = None):
         ensure(fmt in KV_FORMATS, f"KV format must be one of {sorted(KV_FORMATS)}")
+        initial = capacity if initial_capacity is None else initial_capacity
+        for name, value in (("query_heads", query_heads), ("kv_heads", kv_heads), ("head_dim", head_dim),
+                            ("capacity", capacity), ("max_query_rows", max_query_rows), ("initial_capacity", initial),
+                            ("block", block)):
+            int32(value, name)
         L = F.lib()
         cfg = F.rk_npu_hip_attention_q8_config()
         L.rk_npu_hip_attention_q8_config_init(ctypes.byref(cfg))
         a = cfg.attention
         a.query_heads, a.kv_heads, a.head_dim, a.softmax_scale = query_heads, kv_heads, head_dim, softmax_scale
         a.max_query_rows, a.max_capacity = max_query_rows, capacity
-        a.initial_capacity = capacity if initial_capacity is None else initial_capacity
+        a.initial_capacity = initial
         a.mask_mode = F.RK_NPU_ATTENTION_F16_CAUSAL if causal else F.RK_NPU_ATTENTION_F16_NO_MASK
         cfg.format, cfg.block = KV_FORMATS[fmt], block
         raw = ctypes.c_void_p()
@@ -214,12 +219,14 @@ class KvCacheQ8:
         return info.key_bytes + info.value_bytes + info.tail_bytes
 
     def reserve(self, capacity: int) -> None:
-        check(F.lib().rk_npu_hip_attention_q8_cache_reserve(self.ctx.shared.ctx.raw, self.handle.raw, capacity),
+        check(F.lib().rk_npu_hip_attention_q8_cache_reserve(self.ctx.shared.ctx.raw, self.handle.raw,
+                                                           int32(capacity, "capacity")),
               "reserve the 8-bit KV cache")
 
     def truncate(self, length: int) -> None:
         """Keeps the first `length` tokens; exact within the open block and the last complete one."""
-        check(F.lib().rk_npu_hip_attention_q8_cache_truncate(self.handle.raw, length), "truncate the 8-bit KV cache")
+        check(F.lib().rk_npu_hip_attention_q8_cache_truncate(self.handle.raw, int32(length, "length")),
+              "truncate the 8-bit KV cache")
 
     def append(self, k, v, stream=None) -> None:
         """Appends k and v, [kv_heads][rows][head_dim]."""
@@ -235,8 +242,8 @@ class KvCacheQ8:
         shape = k.shape
         ensure(shape == v.shape, "k and v must have the same shape")
         kh, vh = _heads(k, *self._kv), _heads(v, *self._kv)
-        check(F.lib().rk_npu_hip_attention_q8_device_read(self.handle.raw, first, shape[1], ctypes.byref(kh),
-                                                          ctypes.byref(vh), _stream(stream, k)),
+        check(F.lib().rk_npu_hip_attention_q8_device_read(self.handle.raw, int32(first, "first"), shape[1],
+                                                          ctypes.byref(kh), ctypes.byref(vh), _stream(stream, k)),
               "read the 8-bit KV cache")
 
 
@@ -244,6 +251,7 @@ def _heads(t, heads: int, head_dim: int) -> F.rk_npu_hip_heads:
     shape, stride = t.shape, t.stride()
     if not (len(shape) == 3 and shape[0] == heads and shape[2] == head_dim and stride[2] == 1 and t.is_cuda):
         raise NpuError(f"attention arrays are cuda [{heads}][rows][{head_dim}] tensors with contiguous rows")
+    int32(shape[1], "rows")
     return F.rk_npu_hip_heads(t.data_ptr(), _dtype_code(t), stride[0], stride[1])
 
 
@@ -255,8 +263,9 @@ def attention_q8(ctx: DeviceContext, cache: KvCacheQ8, q, out, position: int, ws
     ensure(shape == out.shape, "q and out must have the same shape")
     ws = ws or ctx.attention_workspace(cache)
     qh, oh = _heads(q, *cache._query), _heads(out, *cache._query)
-    check(F.lib().rk_npu_hip_attention_q8_device_run(ws.raw, cache.handle.raw, ctypes.byref(qh), shape[1], position,
-                                                     ctypes.byref(oh), _stream(stream, q)), "8-bit KV attention")
+    check(F.lib().rk_npu_hip_attention_q8_device_run(ws.raw, cache.handle.raw, ctypes.byref(qh), shape[1],
+                                                     int32(position, "position"), ctypes.byref(oh),
+                                                     _stream(stream, q)), "8-bit KV attention")
 
 
 @contextlib.contextmanager

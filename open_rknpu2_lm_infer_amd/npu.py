@@ -35,6 +35,13 @@ def ensure(cond: bool, msg: str) -> None:
         raise NpuError(msg)
 
 
+def int32(value: int, name: str) -> int:
+    """`value`, which the library takes as 32 bits (ctypes keeps the low ones)."""
+    if not -2 ** 31 <= value < 2 ** 31:
+        raise NpuError(f"{name} {value} does not fit 32 bits")
+    return value
+
+
 def bucket(rows: int) -> int:
     """src/npu.rs:201-211."""
     ensure(1 <= rows <= 256, "linear batch must be within 1..256")

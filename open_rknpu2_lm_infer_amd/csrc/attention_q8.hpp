@@ -139,12 +139,12 @@ __device__ __forceinline__ float q8_weight(float m, float top) {
 }
 
 // A row's maximum moves when a score passes it by LAZY (powers of 2), to SHIFT below
-// the score: weights lie below 2^15, the row's largest above 2^5 (SPLIT) or 2^9. More of
-// fp16's range for the small ones costs more moves: 1024 rows of 8 heads of 128 over
-// 32768 keys, SPLIT with 4 and 10 207 us instead of 198; else with 4 and 11 153 instead
-// of 146, with 8 and 7 145.
-constexpr float q8_lazy(bool split) { return split ? 8.0f : 6.0f; }
-constexpr float q8_shift(bool split) { return split ? 6.0f : 9.0f; }
+// the score: weights lie below 2^15, the row's largest above 2^(SHIFT - 1) (SPLIT) or
+// 2^SHIFT. More of fp16's range for the small ones costs more moves, which show where
+// waves do not wait for memory: 1024 rows of 8 heads of 128 over 32768 keys, SPLIT with
+// LAZY 8 198 us, with 4 207; one fp16 a weight with 8 145, with 6 146, with 4 153.
+constexpr float q8_lazy(bool split, bool few) { return few ? 4.0f : split ? 8.0f : 6.0f; }
+constexpr float q8_shift(bool split, bool few) { return (split ? 14.0f : 15.0f) - q8_lazy(split, few); }
 
 // A wave's query rows, RW groups of 16 (lane l: row l % 16 of each): their key
 // limits, queries, running maxima (less SHIFT), sums and accumulators (lane l:
@@ -161,14 +161,13 @@ constexpr float q8_shift(bool split) { return split ? 6.0f : 9.0f; }
 // p in f32, before any rounding. (The sum of the fp16 weights lost such keys: 17 % off
 // where half of the weight had 2^-24 of the other half's scale.)
 //
-// SPLIT (f32 output): p mu goes into the products as two fp16, 22 bits. Otherwise
-// (fp16 output) p mu goes in as one, mu in the exponent. fp16 has fewer bits below
-// 2^-14, and 2^-25 is lost: a weight times scale is off by 2^-30 (fp16 output: 2^-34)
-// of the row's largest at most.
-template <int D, int RW, bool SPLIT>
+// SPLIT: p mu goes into the products as two fp16, 22 bits. Otherwise p mu goes in as
+// one, mu in the exponent. fp16 has fewer bits below 2^-14, and 2^-25 is lost: a weight
+// times scale is off by 2^-30 (FEW, or one fp16: 2^-34) of the row's largest at most.
+template <int D, int RW, bool SPLIT, bool FEW = false>
 struct Q8Wave {
     static constexpr int KS = D / 32, NB = D / 16;
-    static constexpr float LAZY = q8_lazy(SPLIT), SHIFT = q8_shift(SPLIT);
+    static constexpr float LAZY = q8_lazy(SPLIT, FEW), SHIFT = q8_shift(SPLIT, FEW);
     int lim[RW];
     int open, seen;  // keys below `open` every row sees, from `seen` on none
     q8_h8 qf[RW][KS];
@@ -562,7 +561,7 @@ __global__ __launch_bounds__(64 * NW) void attn_q8_kernel(AttnQ8Params P) {
     const int u_tail = u_begin + (max(coded_units - u_begin, 0) + NW - 1) / NW * NW;
     const bool late = D == 256 && u_tail < min((split + 1) * P.units_per_split, P.units);
     if (!late) first();
-    Q8Wave<D, RW, SPLIT> W;
+    Q8Wave<D, RW, SPLIT, RW == 1> W;
     W.start(P, g, rt * RT, lo, hi);
     const int u_end = min(min((split + 1) * P.units_per_split, P.units), (W.seen + 31) >> 5);
     const int coded_end = min(u_end, coded_units);
@@ -899,8 +898,8 @@ struct Q8Plan {
     int rows() const { return 16 * groups * (tile ? waves : 1); }  // of a block
 };
 
-void launch_attn_q8_i8(const AttnQ8Params& P, int head_dim, const Q8Plan& plan, bool f32_weights, hipStream_t s);
-void launch_attn_q8_e4m3(const AttnQ8Params& P, int head_dim, const Q8Plan& plan, bool f32_weights, hipStream_t s);
+void launch_attn_q8_i8(const AttnQ8Params& P, int head_dim, const Q8Plan& plan, bool two, hipStream_t s);
+void launch_attn_q8_e4m3(const AttnQ8Params& P, int head_dim, const Q8Plan& plan, bool two, hipStream_t s);
 
 template <int D, int FMT, bool SPLIT>
 static void launch_attn_q8_rows(const AttnQ8Params& P, const Q8Plan& plan, hipStream_t s) {
@@ -910,16 +909,16 @@ static void launch_attn_q8_rows(const AttnQ8Params& P, const Q8Plan& plan, hipSt
     constexpr int G = D == 256 ? 1 : 2;
     if (plan.tile)
         hipLaunchKernelGGL((attn_q8_tile_kernel<D, 8, G, G, FMT, SPLIT>), grid, block, 0, s, P);
-    else if (plan.groups == 1)
-        hipLaunchKernelGGL((attn_q8_kernel<D, 4, 1, FMT, SPLIT>), grid, block, 0, s, P);
+    else if (plan.groups == 1)  // (narrow heads: up to 16 rows, whose weights are two fp16)
+        hipLaunchKernelGGL((attn_q8_kernel<D, 4, 1, FMT, SPLIT || D != 256>), grid, block, 0, s, P);
     else
         hipLaunchKernelGGL((attn_q8_kernel<D, D == 256 ? 4 : 8, 2, FMT, SPLIT>), grid, block, 0, s, P);
 }
 
 template <int FMT>
-static void launch_attn_q8(const AttnQ8Params& P, int head_dim, const Q8Plan& plan, bool f32_weights, hipStream_t s) {
+static void launch_attn_q8(const AttnQ8Params& P, int head_dim, const Q8Plan& plan, bool two, hipStream_t s) {
 #define HM_Q8_ROWS(DD)                                     \
-    if (f32_weights)                                       \
+    if (two)                                               \
         launch_attn_q8_rows<DD, FMT, true>(P, plan, s); \
     else                                                   \
         launch_attn_q8_rows<DD, FMT, false>(P, plan, s)

@@ -6,8 +6,8 @@
 
 namespace hm {
 
-void launch_attn_q8_i8(const AttnQ8Params& P, int head_dim, const Q8Plan& plan, bool f32_weights, hipStream_t s) {
-    launch_attn_q8<RK_NPU_HIP_KV_I8>(P, head_dim, plan, f32_weights, s);
+void launch_attn_q8_i8(const AttnQ8Params& P, int head_dim, const Q8Plan& plan, bool two, hipStream_t s) {
+    launch_attn_q8<RK_NPU_HIP_KV_I8>(P, head_dim, plan, two, s);
 }
 
 }  // namespace hm

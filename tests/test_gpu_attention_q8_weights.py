@@ -122,3 +122,20 @@ def test_every_unit_counts(ctx, qh, kh, d, rows, keys, fmt, dtype):
     rng = np.random.default_rng(keys)
     for tile in ((0, 1, 2) if qh // kh * rows > 16 else (0,)):
         check(ctx, kv_cases.marks(rng, kh, d, keys), dtype, fmt, rows=rows, qh=qh, tile=tile, causal=rows > 1, d=d)
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("qh,kh,d,rows,keys", [(32, 8, 128, 1, 3980), (16, 8, 64, 8, 2000), (16, 2, 256, 2, 5000),
+                                               (1, 1, 64, 1, 1), (4, 2, 128, 3, 45)])
+def test_few_rows_of_f16_output_are_rounded_once(ctx, qh, kh, d, rows, keys, fmt):
+    """Up to 16 query rows per KV head: fp16 outputs are the f32 ones, rounded."""
+    print(f"{fmt} qh={qh} kh={kh} d={d} rows={rows} keys={keys}", flush=True)
+    cache = D.KvCacheQ8(ctx, qh, kh, d, d ** -0.5, keys, fmt=fmt, max_query_rows=rows)
+    g = torch.Generator("cuda").manual_seed(keys)
+    k, v = (torch.randn(kh, keys, d, device="cuda", generator=g) for _ in range(2))
+    cache.append(k, v)
+    q = torch.randn(qh, rows, d, device="cuda", generator=g)
+    outs = [torch.empty(qh, rows, d, device="cuda", dtype=t) for t in (F32, F16)]
+    for o in outs:
+        D.attention_q8(ctx, cache, q, o, keys - rows)
+    assert torch.equal(outs[0].half(), outs[1])

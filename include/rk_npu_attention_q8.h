@@ -28,13 +28,13 @@
  * the next append continues from their values rounded to fp16.
  *
  * Attention is rk_npu_attention_f16.h's formula over the cache's values: f32
- * scores (scale q k below 2^24), weights and sums. Into the products with V a weight
- * goes times its block's V scale, as two fp16 (22 bits), or as one (11 bits) where the
- * output is fp16 and there are more than 16 query rows per KV head (rows x query heads
- * / KV heads). Either is off by 2^-30 of the row's largest such product at most where
- * fp16 has fewer bits: values of keys that light are lost, their weights are not. A
- * value of the tail that is infinite or NaN counts for the query rows that see its
- * token and for no other.
+ * scores, weights and sums, for |scale q k| up to 10^7 (beyond, a row may come out as
+ * NaN). Into the products with V a weight goes times its block's V scale, as two fp16
+ * (22 bits), or as one (11 bits) where the output is fp16 and there are more than 16
+ * query rows per KV head (rows x query heads / KV heads). Where fp16 has fewer bits it
+ * is off by up to 2^-30 of the row's largest such product: the values of keys that
+ * light are lost, their weights are not. A value of the tail that is infinite or NaN
+ * counts for the query rows that see its token and for no other.
  *
  * Workspaces are rk_npu_attention_f16_workspace of the same geometry
  * (rk_npu_attention_f16_prepare with &config.attention).

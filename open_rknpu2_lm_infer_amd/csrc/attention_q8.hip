@@ -681,9 +681,8 @@ static void q8_combine(const AttnQ8Params& P, int R, hipStream_t s) {
 // splits: one row of 32 heads over 8 of 128 and 3981 keys 8.5 us instead of 8.0, 64
 // heads over 8 of 256 and 16001 keys 19.4 and 17.0), or of two, which share a unit's
 // conversion. Two of 256 dims take every register of a SIMD, and pay over many keys
-// only: i8, 2 KV heads, 512 rows x 16000 keys 43.8 with one and 34.6 with two, x 8000
-// 26.7 and 23.8, x 4000 17.1 and 19.5; 2048 x 4000 34.5 and 34.7 (e4m3, 4 KV heads,
-// 1024 rows 27.5 and 31.7).
+// only: i8, 2 KV heads, 512 rows x 16000 keys 45.4 with one and 35.5 with two, x 8000
+// 27.5 and 24.6, x 4000 17.7 and 20.0; 2048 x 4000 35.9 and 35.6 (e4m3 27.8 and 32.1).
 //
 // attn_q8_tile_kernel converts once a block, which takes rows enough to fill 128- or
 // 256-row blocks and keys enough to fill its stages; the more, the cheaper the
@@ -726,7 +725,8 @@ static void q8_splits(AttnQ8Params& P, int D, int R, const Q8Plan& plan) {
     P.row_tiles = (R + rows - 1) / rows;
     P.rows_pad = P.row_tiles * rows;
     const int base = P.row_tiles * P.kh, least = plan.tile ? 4 : plan.waves;
-    const int blocks = D == 64 && plan.waves == 4 && (long)P.units * base > 32 * 256 ? 512 : 256;
+    const int cus = device_cus();
+    const int blocks = D == 64 && plan.waves == 4 && (long)P.units * base > 32 * cus ? 2 * cus : cus;
     const int few = D == 256 ? 16 : plan.waves == 4 ? 24 : 32;
     const size_t room = attn_partial_rows(D) / ((size_t)P.rows_pad * P.kh);
     int want = std::max(1, std::min((blocks + base - 1) / base, (P.units + least - 1) / least));

@@ -132,8 +132,9 @@ __device__ __forceinline__ void q8_store4(const AttnQ8Params& P, long long at, q
 // A row's maximum before it has seen a key: finite, so that differences are no NaN.
 constexpr float Q8_NONE = -1e30f;
 // The weight 2^d of a partial result whose maximum lies d <= 0 below the row's:
-// never 0, so that an infinite accumulator stays one (0 times it is NaN). What a
-// finite one gains by that is below 2^-100 of the result.
+// never 0, so that an infinite accumulator stays one (0 times it is NaN). A finite sum
+// gains by that 2^-72 a key at most (2^15 the weight, 2^33 for the least V scale),
+// where the row's is above 2^-5.
 __device__ __forceinline__ float q8_weight(float m, float top) {
     return fmaxf(__builtin_amdgcn_exp2f(m - top), 0x1p-120f);
 }
@@ -511,10 +512,12 @@ __device__ __forceinline__ void q8_meet(const AttnQ8Params& P, const Wave& W, in
 // converted.
 //
 // Measured, the join included: one row of 32 heads over 8 of 128 and 131072 keys
-// (268 MB) e4m3 45.6 us, i8 44.9: 5.9 and 6.0 TB/s (a large copy reads and writes
-// 4.9). Over 3968 keys (8 MB) 7.3: there it is latency, a unit's load to its
-// products, the waves' meeting and the join's launch. 512 rows over 4096 keys 20.7:
-// conversion and softmax, vector instructions that every 32 rows repeat. The tail
+// (268 MB) e4m3 45.8 us, i8 45.3: 5.9 TB/s (a large copy reads and writes 4.9). Over
+// 3968 keys (8 MB) 7.5: there it is latency, a unit's load to its products, the waves'
+// meeting and the join's launch. 512 rows of 8 heads over 4096 keys, fp16 output, 21.1:
+// conversion and softmax, vector instructions that every 32 rows repeat, take a SIMD 64 %
+// of its time and the products 24 %, mostly one after the other; 1024 rows of 2 heads of
+// 256 over 2048 keys 16.6: 37 and 22 %, one wave a SIMD waits for its loads. The tail
 // after the coded units, its loads a round trip of their own: one row of 16 heads over
 // 2 of 256, 1000 keys 12.2 us instead of 11.0. The splits joined by their last block,
 // in the same launch, lost to a launch of their own (8.6): 10.0 with the partials
@@ -620,11 +623,11 @@ __global__ __launch_bounds__(64 * NW) void attn_q8_kernel(AttnQ8Params P) {
 // t - 2) are converted meanwhile; U + 1 stages of each are in LDS, with one barrier
 // per stage.
 //
-// Measured: 1024 rows of 8 heads of 128 over 32768 keys 147 us with f16 output, 0.93
-// PFLOP/s of a large matrix product's 1.29, 194 with f32 (a third more products: V's
-// with two fp16 for a weight). Matrix cores 42 % busy, vector instructions 54 % of the
-// time: the softmax of 16 scores a lane and unit holds back the products, whose
-// operands come from LDS once for 32 rows. U = 1: 151 to 157. Matrix and vector
+// Measured: 1024 rows of 8 heads of 128 over 32768 keys 148 us with f16 output, 0.92
+// PFLOP/s of a large matrix product's 1.29, 196 with f32 (half as many products more:
+// V's with two fp16 for a weight). Matrix cores 43 % busy (f32 48), vector instructions
+// 57 % of the time (59): the softmax of 16 scores a lane and unit holds back the products,
+// whose operands come from LDS once for 32 rows. U = 1: 151 to 157. Matrix and vector
 // instructions interleaved by scheduling groups: 162.
 template <int D, int NW, int U, int RW, int FMT, bool SPLIT>
 __global__ __launch_bounds__(64 * NW) void attn_q8_tile_kernel(AttnQ8Params P) {
@@ -859,7 +862,7 @@ __global__ __launch_bounds__(256) void attn_q8_combine_kernel(AttnQ8Params P) {
     for (int i = 0; i < W; ++i) {
         const float w = q8_weight(x[i].x, top);
         weight[row][t + i * T] = w;
-        // (a split that saw NaN scores has maximum -inf and a NaN sum)
+        // (a split that saw NaN scores has a NaN sum)
         den += x[i].y != x[i].y ? x[i].y : w * x[i].y;
     }
 #pragma unroll

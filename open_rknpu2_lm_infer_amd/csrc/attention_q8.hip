@@ -777,7 +777,7 @@ static int q8_enqueue_run(AttnWork* w, Q8Cache* c, const HeadsView& q, int rows,
     // Weights as two fp16: always for f32 output, and for fp16 output where it costs
     // little, so that the output's rounding is all that is lost: one row of 32 heads over 8
     // of 128, 4000 keys 7.9 us (one fp16 7.8), 16000 10.8 (10.4), 131000 45.4 (44.5).
-    const bool two = !P.out_f16 || R <= 16;
+    const bool two = !P.out_f16 || (!plan.tile && R <= 16);
     (c->cfg.format == RK_NPU_HIP_KV_I8 ? launch_attn_q8_i8 : launch_attn_q8_e4m3)(P, D, plan, two, s);
     if (P.splits > 1) {
         if (D == 64)

@@ -7,14 +7,16 @@ from tests import kv_model
 
 
 def steps(model):
-    """[kh][length]: the scale each key's values of V are multiples of. The tail's
-    units of 32 tokens take 2^e, their largest magnitude within 64..128 of it."""
-    parts = [np.repeat(np.where(np.any(codes, axis=(1, 2)), scales, 0.0)[:, None], model.B, 1)
+    """[kh][length]: the scale each key's values of V are multiples of; a block of zeros
+    has that of fp16's least value. The tail's units of 32 tokens take 2^e, their largest
+    magnitude within 64..128 of it, or 2^-30."""
+    least = 2.0 ** -24 / kv_model.TOP[model.fmt]
+    parts = [np.repeat(np.where(np.any(codes, axis=(1, 2)), scales, least)[:, None], model.B, 1)
              for codes, scales in model.blocks]
     tail = np.abs(model.tail.astype(np.float64))
     for u in range(0, tail.shape[1], 32):
         top = tail[:, u:u + 32].max(axis=(1, 2))
-        e = np.where(top > 0, np.exp2(np.floor(np.log2(np.where(top > 0, top, 1.0))) - 6), 0.0)
+        e = np.where(top > 0, np.exp2(np.floor(np.log2(np.where(top > 0, top, 1.0))) - 6), 2.0 ** -30)
         parts.append(np.repeat(e[:, None], tail[:, u:u + 32].shape[1], 1))
     return np.concatenate(parts, axis=1)[:, :model.length]
 
@@ -53,7 +55,7 @@ def attention(q, k, v, step, scale, position, causal, f16):
         size_v = w @ np.abs(v[g])
         weight = (np.log(2.0) * ((d + 5) * 2.0 ** -24 * size + 2.0 ** -15) + 2.0 ** -21)[:, None]
         n = seen.sum(axis=1)[:, None] * 2.0 ** -24
-        counts = np.divide(np.abs(v[g]), step[g][:, None], where=step[g][:, None] > 0, out=np.zeros_like(v[g]))
+        counts = np.abs(v[g]) / step[g][:, None]
         most[h] = (2 * weight + (2.0 ** -11 if f16 else 2.0 ** -22) + 2 * n) * size_v
         most[h] += 2.0 ** (-34 if f16 else -30) * (w * step[g]).max(axis=1, keepdims=True) * (seen @ counts)
         most[h] += (2.0 ** -11 if f16 else 2.0 ** -22) * np.abs(out[h])
@@ -75,7 +77,7 @@ def wave(q, k, v, step, scale, f16, unit=32, plant=None):
     for i, u in enumerate(range(0, len(s), unit)):
         if plant == "drop" and i == 1:
             continue
-        vs = float(step[u]) or (1.0 if plant == "zeros" else 2.0 ** -31)
+        vs = 1.0 if plant == "zeros" and not v[u:u + unit].any() else float(step[u])
         top = s[u:u + unit].max() + np.log2(vs)
         if top > m + lazy + shift:
             new = np.ceil(top) - shift

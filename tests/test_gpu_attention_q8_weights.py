@@ -73,7 +73,7 @@ def test_a_strong_key_of_no_value(ctx, gap, dtype):
     """Nearly all of a row's weight on a key whose V is zero, in a block of larger
     values: the output is the other keys', each of a weight e^-gap."""
     for fmt in ("i8", "e4m3"):
-        for rows, tile in KERNELS[:3]:
+        for rows, tile in KERNELS[:3] + [(2, 1)]:
             rng = np.random.default_rng(gap)
             q = rng.standard_normal(64).astype(np.float16)
             check(ctx, kv_cases.strong_key(rng, 1, 64, q, 0.125, gap), dtype, fmt, rows=rows // 2, tile=tile, q=q)

@@ -191,6 +191,23 @@ class rk_npu_hip_heads(Structure):
     _fields_ = [("data", c_void_p), ("type", c_int32), ("head_stride", c_int64), ("row_stride", c_int64)]
 
 
+# rk_npu_attention_paged.h
+RK_NPU_HIP_PAGED_MAX_SEQUENCES = 1024
+RK_NPU_HIP_PAGED_MAX_ROWS = 1 << 23
+RK_NPU_HIP_PAGED_MAX_QUERIES = 1 << 26
+
+
+class rk_npu_hip_attention_paged_config(Structure):
+    _fields_ = [("attention", rk_npu_attention_f16_config), ("page", c_int32), ("pages", c_int32),
+                ("rotary_dim", c_int32), ("interleaved", c_int32), ("rope_theta", c_double),
+                ("frequencies", POINTER(c_double))]
+
+
+class rk_npu_hip_paged_batch(Structure):
+    _fields_ = [("sequences", c_int32), ("rows", c_int32), ("max_rows", c_int32), ("max_tokens", c_int32),
+                ("lengths", c_void_p), ("row_offsets", c_void_p), ("table", c_void_p), ("table_stride", c_int32)]
+
+
 P = POINTER
 i8p = P(c_int8)
 f32p = P(c_float)
@@ -383,6 +400,18 @@ SIGNATURES = {
                                                     P(rk_npu_hip_heads), c_void_p]),
     "rk_npu_hip_attention_q8_device_run": (c_int, [c_void_p, c_void_p, P(rk_npu_hip_heads), c_int32, c_int32,
                                                    P(rk_npu_hip_heads), c_void_p]),
+    "rk_npu_hip_attention_paged_config_init": (None, [P(rk_npu_hip_attention_paged_config)]),
+    "rk_npu_hip_attention_paged_query": (c_int, [P(rk_npu_hip_attention_paged_config), P(rk_npu_attention_f16_sizes)]),
+    "rk_npu_hip_attention_paged_pool_create": (c_int, [c_void_p, P(rk_npu_hip_attention_paged_config), P(c_void_p)]),
+    "rk_npu_hip_attention_paged_pool_free": (None, [c_void_p]),
+    "rk_npu_hip_attention_paged_status": (c_int, [c_void_p]),
+    "rk_npu_hip_attention_paged_append": (c_int, [c_void_p, P(rk_npu_hip_paged_batch), P(rk_npu_hip_heads),
+                                                  P(rk_npu_hip_heads), c_void_p, P(rk_npu_hip_heads),
+                                                  P(rk_npu_hip_heads), c_void_p]),
+    "rk_npu_hip_attention_paged_read": (c_int, [c_void_p, P(rk_npu_hip_paged_batch), P(rk_npu_hip_heads),
+                                                P(rk_npu_hip_heads), c_void_p]),
+    "rk_npu_hip_attention_paged_run": (c_int, [c_void_p, c_void_p, P(rk_npu_hip_paged_batch), P(rk_npu_hip_heads),
+                                               P(rk_npu_hip_heads), c_void_p]),
 }
 
 # Measurement-only library (libhip_probes.so, csrc/probes.hip): the roofline

@@ -1,6 +1,6 @@
 // What the attention families share: the run workspace and its fences, the
 // geometry checks, caller-memory checks (attention.hip: the fp16 cache;
-// attention_q8.hip: the 8-bit cache).
+// attention_q8.hip: the 8-bit cache; attention_paged.hip: the paged cache).
 #pragma once
 
 #include <hip/hip_fp16.h>
@@ -10,6 +10,7 @@
 #include <mutex>
 
 #include "../../include/rk_npu_attention_f16.h"
+#include "../../include/rk_npu_attention_q8.h"
 #include "runtime.hpp"
 
 namespace hm {
@@ -154,6 +155,46 @@ inline bool kernel_readable(const void* p, int device) {
         return false;
     }
     return a.type == hipMemoryTypeDevice && a.device == device;
+}
+
+// The calls leave the calling thread's current device as it was.
+struct DeviceGuard {
+    int before = -1;
+    bool ok;
+    explicit DeviceGuard(int device) {
+        if (hipGetDevice(&before) != hipSuccess) before = -1;
+        ok = before == device || hipSetDevice(device) == hipSuccess;
+        if (before == device) before = -1;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+struct HeadsView {  // rk_npu_hip_heads in a kernel's arguments
+    void* data;
+    int f32;
+    long long head, row;
+};
+
+inline bool valid_heads(const rk_npu_hip_heads* a, int device, int head_dim, bool written, int heads, int rows) {
+    if (!a || !a->data || (a->type != RK_NPU_HIP_F16 && a->type != RK_NPU_HIP_F32) || a->head_stride < 0 ||
+        a->row_stride < 0)
+        return false;
+    const uintptr_t element = a->type == RK_NPU_HIP_F16 ? 2 : 4;
+    if (reinterpret_cast<uintptr_t>(a->data) % element) return false;
+    if (a->head_stride > ((int64_t)1 << 46) || a->row_stride > ((int64_t)1 << 40)) return false;
+    if (written) {
+        // rows of head_dim values must not overlap, in a head or over the heads
+        const int64_t hs = a->head_stride, rs = a->row_stride;
+        const bool by_head = (rows == 1 || rs >= head_dim) && (heads == 1 || hs >= (int64_t)(rows - 1) * rs + head_dim);
+        const bool by_row = (heads == 1 || hs >= head_dim) && (rows == 1 || rs >= (int64_t)(heads - 1) * hs + head_dim);
+        if (!by_head && !by_row) return false;
+    }
+    return kernel_readable(a->data, device);
+}
+inline HeadsView view_of(const rk_npu_hip_heads& a) {
+    return HeadsView{a.data, a.type == RK_NPU_HIP_F32 ? 1 : 0, (long long)a.head_stride, (long long)a.row_stride};
 }
 
 }  // namespace hm

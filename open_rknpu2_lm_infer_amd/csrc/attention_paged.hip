@@ -1,0 +1,518 @@
+// The paged KV cache: its C ABI (include/rk_npu_attention_paged.h), and the kernels
+// that write and read its pages. The attention over it: attention_paged.hpp, which
+// also gives the layout.
+
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <cstring>
+#include <new>
+#include <vector>
+
+#include "attention.hpp"
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Wunused-function"  // (the headers' other kernels)
+#include "attention_paged.hpp"
+#pragma clang diagnostic pop
+#include "launch.hpp"
+
+namespace hm {
+
+constexpr uint32_t MAGIC_PAGED_POOL = 0x47504841u;
+
+// 8 values of a row in f32, and 8 as fp16 or f32, of any alignment.
+__device__ __forceinline__ void pg_get8(const HeadsView& a, long long at, float (&x)[8]) {
+    if (a.f32) {
+        const float* p = static_cast<const float*>(a.data) + at;
+        const pg_f4a4 u = *reinterpret_cast<const pg_f4a4*>(p), v = *reinterpret_cast<const pg_f4a4*>(p + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = u[i];
+            x[4 + i] = v[i];
+        }
+    } else {
+        const pg_h8 u = __builtin_bit_cast(
+            pg_h8, v4u(*reinterpret_cast<const pg_u4a2*>(static_cast<const __half*>(a.data) + at)));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = (float)u[i];
+    }
+}
+__device__ __forceinline__ v4u pg_halves(const float (&x)[8]) {
+    pg_h8 h;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = (_Float16)x[i];
+    return __builtin_bit_cast(v4u, h);
+}
+__device__ __forceinline__ void pg_put8(const HeadsView& a, long long at, const float (&x)[8]) {
+    if (a.f32) {
+        float* p = static_cast<float*>(a.data) + at;
+        *reinterpret_cast<pg_f4a4*>(p) = pg_f4a4{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<pg_f4a4*>(p + 4) = pg_f4a4{x[4], x[5], x[6], x[7]};
+    } else {
+        *reinterpret_cast<pg_u4a2*>(static_cast<__half*>(a.data) + at) = pg_u4a2(pg_halves(x));
+    }
+}
+
+struct PagedRowsParams {
+    PagedBatch b;
+    HeadsView k, v, q, q_out;   // (data nullptr: none)
+    const int* positions;
+    const double* turns;        // frequencies in turns (radians / 2 pi) per position
+    int D, qh, rotary, interleaved;
+    int rows_per_block, heads_per_block;
+};
+
+// The sequences and tokens of a block's rows row0..row0 + n - 1, by all its threads:
+// seq[i] and token[i] (-1: no token), dest[i] (the row's place in the pool in tokens of
+// a head, page * kh * page + place; -1: none).
+template <int RB>
+__device__ __forceinline__ void pg_block_rows(const PagedBatch& B, int row0, int n, int (&seq)[RB], int (&token)[RB],
+                                              int (&page)[RB]) {
+    const int tid = threadIdx.x;
+    if (tid < RB) {
+        seq[tid] = B.offsets ? -1 : row0 + tid < B.sequences ? row0 + tid : -1;
+        token[tid] = -1;
+        page[tid] = -1;
+    }
+    __syncthreads();
+    if (B.offsets) {
+        for (int s = tid; s < B.sequences; s += blockDim.x) {
+            const int a = B.offsets[s], b = B.offsets[s + 1];
+            if (a < 0 || b < a || b > B.rows || b - a > B.max_rows) {
+                pg_flaw(B);
+                continue;
+            }
+            for (int r = max(a, row0); r < min(b, row0 + n); ++r) seq[r - row0] = s;
+        }
+        __syncthreads();
+    }
+    if (tid < n && seq[tid] >= 0) {
+        const int s = seq[tid];
+        const PagedSeq q = pg_seq(B, s);
+        const int t = q.len - q.n + (row0 + tid - q.row);
+        // (another thread may have found the row in a sequence of overlapping offsets)
+        if (q.n > 0 && t >= 0 && t < q.len) {
+            token[tid] = t;
+            page[tid] = pg_page(B, s, t);
+        }
+    }
+    __syncthreads();
+}
+
+// Append. Block: `rows_per_block` rows of `heads_per_block` of the heads, counted q
+// heads, K heads, V heads. A thread takes 16 values of a row at a time, the two pieces
+// of 8 dims that turn into each other.
+template <int RB>
+__global__ __launch_bounds__(256) void paged_append_kernel(PagedRowsParams P) {
+    __shared__ int seq[RB], token[RB], page[RB];
+    __shared__ float2 turn[RB * 128];
+    const PagedBatch& B = P.b;
+    const int tid = threadIdx.x, row0 = blockIdx.x * RB, n = min(RB, B.rows - row0);
+    pg_block_rows<RB>(B, row0, n, seq, token, page);
+    const int pairs = P.rotary >> 1;
+    for (int i = tid; i < n * pairs; i += 256) {
+        const int r = i / pairs, j = i - r * pairs;
+        if (token[r] < 0) continue;
+        const double at = (double)(P.positions ? P.positions[row0 + r] : token[r]) * P.turns[j];
+        float s, c;
+        sincospif(2.0f * (float)(at - __builtin_rint(at)), &s, &c);
+        turn[i] = float2{c, s};
+    }
+    __syncthreads();
+    const int per_head = P.D >> 4, heads = P.qh + 2 * B.kh, qh = P.qh;
+    const int h0 = blockIdx.y * P.heads_per_block, hn = min(P.heads_per_block, heads - h0);
+    const int page_mask = (1 << B.page_shift) - 1;
+    for (int i = tid; i < n * hn * per_head; i += 256) {
+        const int unit = i % per_head, h = h0 + i / per_head % hn, r = i / per_head / hn;
+        if (token[r] < 0) continue;
+        const int kind = h < qh ? 0 : h < qh + B.kh ? 1 : 2, g = kind == 0 ? h : h - qh - (kind - 1) * B.kh;
+        const HeadsView& src = kind == 0 ? P.q : kind == 1 ? P.k : P.v;
+        if (!src.data) continue;
+        const bool turned = unit < P.rotary >> 4 && kind != 2;
+        // pieces of 8 dims: a pair's two, or neighbours
+        const int rest = unit - (P.rotary >> 4);
+        const int a = turned && !P.interleaved ? unit : unit < P.rotary >> 4 ? 2 * unit : (P.rotary >> 3) + 2 * rest;
+        const int b = turned && !P.interleaved ? unit + (P.rotary >> 4) : a + 1;
+        const long long at = (long long)g * src.head + (long long)(row0 + r) * src.row;
+        float x[8], y[8];
+        pg_get8(src, at + 8 * a, x);
+        pg_get8(src, at + 8 * b, y);
+        if (turned) {
+            const float2* t = turn + r * pairs + 8 * unit;
+            if (!P.interleaved) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float u = x[k], v = y[k];
+                    x[k] = u * t[k].x - v * t[k].y;
+                    y[k] = v * t[k].x + u * t[k].y;
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float u = x[2 * k], v = x[2 * k + 1], w = y[2 * k], z = y[2 * k + 1];
+                    x[2 * k] = u * t[k].x - v * t[k].y;
+                    x[2 * k + 1] = v * t[k].x + u * t[k].y;
+                    y[2 * k] = w * t[4 + k].x - z * t[4 + k].y;
+                    y[2 * k + 1] = z * t[4 + k].x + w * t[4 + k].y;
+                }
+            }
+        }
+        if (kind == 0) {
+            const long long to = (long long)g * P.q_out.head + (long long)(row0 + r) * P.q_out.row;
+            pg_put8(P.q_out, to + 8 * a, x);
+            pg_put8(P.q_out, to + 8 * b, y);
+        } else if (page[r] >= 0) {
+            const int place = token[r] & page_mask, j = place & 15;
+            __half* to = (kind == 1 ? B.k : B.v) +
+                         (((size_t)page[r] * B.kh + g) << B.page_shift) * P.D + (size_t)(place & ~15) * P.D;
+            const int pa = kind == 1 ? pg_k_place(P.D, j, a) : pg_v_place(P.D, j, a);
+            const int pb = kind == 1 ? pg_k_place(P.D, j, b) : pg_v_place(P.D, j, b);
+            *reinterpret_cast<v4u*>(to + pa * 8) = pg_halves(x);
+            *reinterpret_cast<v4u*>(to + pb * 8) = pg_halves(y);
+        }
+    }
+}
+
+// Read. Block: as the append's, over K heads then V heads; a thread takes a piece of 8
+// dims at a time.
+template <int RB>
+__global__ __launch_bounds__(256) void paged_read_kernel(PagedRowsParams P) {
+    __shared__ int seq[RB], token[RB], page[RB];
+    const PagedBatch& B = P.b;
+    const int tid = threadIdx.x, row0 = blockIdx.x * RB, n = min(RB, B.rows - row0);
+    pg_block_rows<RB>(B, row0, n, seq, token, page);
+    const int per_head = P.D >> 3, h0 = blockIdx.y * P.heads_per_block, hn = min(P.heads_per_block, 2 * B.kh - h0);
+    const int page_mask = (1 << B.page_shift) - 1;
+    for (int i = tid; i < n * hn * per_head; i += 256) {
+        const int piece = i % per_head, h = h0 + i / per_head % hn, r = i / per_head / hn;
+        const int which = h < B.kh ? 0 : 1, g = h - which * B.kh;
+        const HeadsView& dst = which ? P.v : P.k;
+        if (page[r] < 0 || !dst.data) continue;
+        const int place = token[r] & page_mask, j = place & 15;
+        const __half* from = (which ? B.v : B.k) + (((size_t)page[r] * B.kh + g) << B.page_shift) * P.D +
+                             (size_t)(place & ~15) * P.D;
+        const pg_h8 u = __builtin_bit_cast(
+            pg_h8, *reinterpret_cast<const v4u*>(from + (which ? pg_v_place(P.D, j, piece) : pg_k_place(P.D, j, piece)) * 8));
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = (float)u[k];
+        pg_put8(dst, (long long)g * dst.head + (long long)(row0 + r) * dst.row + 8 * piece, x);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------
+struct PagedPool {
+    uint32_t magic;
+    Domain* domain;
+    rk_npu_hip_attention_paged_config cfg;
+    __half* kv[2];
+    double* turns;  // [rotary / 2], or nullptr
+    int* flaw;
+    size_t kv_bytes, turn_bytes;  // of one array each
+    DevFence fence;               // device calls that note flaws
+};
+
+constexpr size_t PAGED_FLAW_BYTES = 256;
+
+static PagedPool* as_pool(const void* p) {
+    PagedPool* c = static_cast<PagedPool*>(const_cast<void*>(p));
+    return (c && c->magic == MAGIC_PAGED_POOL) ? c : nullptr;
+}
+
+static bool valid_paged(const rk_npu_hip_attention_paged_config* c) {
+    if (!c || !valid_config(&c->attention)) return false;
+    if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128 && c->page != 256) return false;
+    if (c->rotary_dim < 0 || c->rotary_dim > c->attention.head_dim || c->rotary_dim % 16) return false;
+    if (c->interleaved != 0 && c->interleaved != 1) return false;
+    if (c->rotary_dim > 0 && !c->frequencies && !(std::isfinite(c->rope_theta) && c->rope_theta > 0.0)) return false;
+    if (c->rotary_dim > 0 && c->frequencies)
+        for (int i = 0; i < c->rotary_dim / 2; ++i)
+            if (!std::isfinite(c->frequencies[i])) return false;
+    // (kernels count the pool's 16-token tiles in 32 bits)
+    return c->pages >= 1 && (int64_t)c->pages * c->attention.kv_heads * (c->page / 16) <= INT_MAX &&
+           c->attention.max_capacity <= INT_MAX - 255;
+}
+static size_t paged_kv_bytes(const rk_npu_hip_attention_paged_config& c) {
+    return (size_t)c.pages * c.page * c.attention.kv_heads * c.attention.head_dim * sizeof(__half);
+}
+
+// A batch a call may plan by; the arrays on the device are the kernels' to check.
+static bool valid_batch(const PagedPool* c, const rk_npu_hip_paged_batch* b) {
+    if (!b || b->sequences < 1 || b->sequences > RK_NPU_HIP_PAGED_MAX_SEQUENCES || b->rows < 1 ||
+        b->rows > RK_NPU_HIP_PAGED_MAX_ROWS)
+        return false;
+    if (b->max_rows < 1 || b->max_rows > b->rows || b->table_stride < 1 || b->max_tokens < 1) return false;
+    if (!b->row_offsets && (b->max_rows != 1 || b->rows < b->sequences)) return false;
+    if (b->max_tokens > (int64_t)b->table_stride * c->cfg.page || b->max_tokens > c->cfg.attention.max_capacity)
+        return false;
+    const int device = device_of(c->domain);
+    auto ints = [&](const int32_t* p) {
+        return p && reinterpret_cast<uintptr_t>(p) % sizeof(int32_t) == 0 && kernel_readable(p, device);
+    };
+    return ints(b->lengths) && ints(b->table) && (!b->row_offsets || ints(b->row_offsets));
+}
+
+static PagedBatch batch_of(const PagedPool* c, const rk_npu_hip_paged_batch* b) {
+    PagedBatch B;
+    B.lengths = b->lengths;
+    B.offsets = b->row_offsets;
+    B.table = b->table;
+    B.flaw = c->flaw;
+    B.k = c->kv[0];
+    B.v = c->kv[1];
+    B.sequences = b->sequences;
+    B.rows = b->rows;
+    B.max_rows = b->max_rows;
+    B.max_tokens = b->max_tokens;
+    B.table_stride = b->table_stride;
+    B.kh = c->cfg.attention.kv_heads;
+    B.pages = c->cfg.pages;
+    B.page_shift = __builtin_ctz(c->cfg.page);
+    return B;
+}
+
+static PagedRowsParams rows_params(const PagedPool* c, const rk_npu_hip_paged_batch* b) {
+    PagedRowsParams P{};
+    P.b = batch_of(c, b);
+    P.turns = c->turns;
+    P.D = c->cfg.attention.head_dim;
+    P.rotary = c->cfg.rotary_dim;
+    P.interleaved = c->cfg.interleaved;
+    return P;
+}
+
+static bool paged_same_geometry(const AttnWork* w, const PagedPool* c) {
+    const rk_npu_attention_f16_config &a = w->cfg, &b = c->cfg.attention;
+    return a.query_heads == b.query_heads && a.kv_heads == b.kv_heads && a.head_dim == b.head_dim &&
+           a.mask_mode == b.mask_mode && a.softmax_scale == b.softmax_scale &&
+           device_of(w->domain) == device_of(c->domain);
+}
+
+// Row tiles, and the blocks that splits aim at.
+static void paged_plan(AttnPagedParams& P, int D) {
+    const PagedBatch& B = P.b;
+    const int G = P.qh / B.kh;
+    P.tile_rows = (int64_t)B.max_rows * G <= 8 ? 8 : 16;
+    // (each sequence ends a tile of its own)
+    const int64_t tiles = std::min<int64_t>((int64_t)B.sequences * (((int64_t)B.max_rows * G + P.tile_rows - 1) / P.tile_rows),
+                                            (int64_t)B.rows * G / P.tile_rows + B.sequences);
+    P.tiles = (int)std::min<int64_t>(tiles, INT_MAX / 2);
+    P.least = 8;
+    P.target = 0;
+    const int units = (B.max_tokens + 31) / 32, want = std::max(1, 2 * device_cus() / B.kh);
+    const int64_t items = (int64_t)P.tiles + want;
+    // (units are added up in 32 bits)
+    if (units > 16 && P.tiles < want && (int64_t)P.tiles * units < (1 << 30) &&
+        (size_t)(items * B.kh * P.tile_rows) <= attn_partial_rows(D))
+        P.target = want;
+    P.items = P.target ? (int)items : P.tiles;
+}
+
+template <int D>
+static void launch_paged(const AttnPagedParams& P, hipStream_t s) {
+    const dim3 grid(P.b.kh * P.items);
+    if (P.tile_rows == 8)
+        hipLaunchKernelGGL((attn_paged_rows_kernel<D, 4, true>), grid, dim3(256), 0, s, P);
+    else
+        hipLaunchKernelGGL((attn_paged_rows_kernel<D, 4, false>), grid, dim3(256), 0, s, P);
+    if (P.target)
+        hipLaunchKernelGGL((attn_paged_join_kernel<D>), dim3(P.b.kh, P.tiles, P.tile_rows), dim3(256), 0, s, P);
+}
+
+}  // namespace hm
+
+using namespace hm;
+
+extern "C" {
+
+void rk_npu_hip_attention_paged_config_init(rk_npu_hip_attention_paged_config* c) {
+    if (!c) return;
+    std::memset(c, 0, sizeof(*c));
+    rk_npu_attention_f16_config_init(&c->attention);
+    c->page = 64;
+    c->rope_theta = 10000.0;
+}
+
+int rk_npu_hip_attention_paged_query(const rk_npu_hip_attention_paged_config* c, rk_npu_attention_f16_sizes* sizes) {
+    if (!valid_paged(c) || !sizes) return RK_NPU_ERR_PARAM;
+    const int rc = rk_npu_attention_f16_query(&c->attention, 0, 1, 0, sizes);
+    if (rc != RK_NPU_OK) return rc;
+    sizes->key_bytes = sizes->value_bytes = paged_kv_bytes(*c);
+    sizes->tail_bytes = 0;
+    return RK_NPU_OK;
+}
+
+int rk_npu_hip_attention_paged_pool_create(rk_npu_iommu_domain* domain,
+                                           const rk_npu_hip_attention_paged_config* config,
+                                           rk_npu_hip_attention_paged_pool** out) {
+    if (out) *out = nullptr;
+    Domain* d = static_cast<Domain*>(domain);
+    if (!d || !out || !valid_paged(config)) return RK_NPU_ERR_PARAM;
+    if (!supported_dim(config->attention.head_dim)) return RK_NPU_ERR_UNSUPPORTED;
+    DeviceGuard dev(device_of(d));
+    if (!dev.ok) return RK_NPU_ERR_DEVICE;
+    PagedPool* c = new (std::nothrow) PagedPool();
+    if (!c) return RK_NPU_ERR_NOMEM;
+    c->magic = MAGIC_PAGED_POOL;
+    c->domain = d;
+    c->cfg = *config;
+    c->cfg.frequencies = nullptr;
+    c->kv_bytes = paged_kv_bytes(*config);
+    const int pairs = config->rotary_dim / 2;
+    c->turn_bytes = std::max<size_t>(1, pairs) * sizeof(double);
+    double turns[128];
+    const double around = 6.283185307179586476925286766559;
+    for (int j = 0; j < pairs; ++j)
+        turns[j] = (config->frequencies ? config->frequencies[j] : std::pow(config->rope_theta, -(double)j / pairs)) / around;
+    auto* raw = reinterpret_cast<rk_npu_hip_attention_paged_pool*>(c);
+    c->flaw = static_cast<int*>(domain_alloc(d, PAGED_FLAW_BYTES));
+    c->turns = c->flaw ? static_cast<double*>(domain_alloc(d, c->turn_bytes)) : nullptr;
+    c->kv[0] = c->turns ? static_cast<__half*>(domain_alloc(d, c->kv_bytes)) : nullptr;
+    c->kv[1] = c->kv[0] ? static_cast<__half*>(domain_alloc(d, c->kv_bytes)) : nullptr;
+    if (!c->kv[1]) {
+        rk_npu_hip_attention_paged_pool_free(raw);
+        return RK_NPU_ERR_NOMEM;
+    }
+    const int zero = 0;
+    if (hipMemcpy(c->flaw, &zero, sizeof(zero), hipMemcpyHostToDevice) != hipSuccess ||
+        (pairs && hipMemcpy(c->turns, turns, pairs * sizeof(double), hipMemcpyHostToDevice) != hipSuccess)) {
+        (void)hipGetLastError();
+        rk_npu_hip_attention_paged_pool_free(raw);
+        return RK_NPU_ERR_DEVICE;
+    }
+    *out = raw;
+    return RK_NPU_OK;
+}
+
+void rk_npu_hip_attention_paged_pool_free(rk_npu_hip_attention_paged_pool* pool) {
+    PagedPool* c = as_pool(pool);
+    if (!c) return;
+    DeviceGuard dev(device_of(c->domain));
+    (void)c->fence.wait(nullptr);
+    c->fence.destroy();
+    for (int i = 0; i < 2; ++i) domain_free(c->domain, c->kv[i], c->kv_bytes);
+    domain_free(c->domain, c->turns, c->turn_bytes);
+    domain_free(c->domain, c->flaw, PAGED_FLAW_BYTES);
+    c->magic = 0;
+    delete c;
+}
+
+int rk_npu_hip_attention_paged_status(rk_npu_hip_attention_paged_pool* pool) {
+    PagedPool* c = as_pool(pool);
+    if (!c) return RK_NPU_ERR_PARAM;
+    DeviceGuard dev(device_of(c->domain));
+    if (!dev.ok || c->fence.wait(nullptr) != hipSuccess) return RK_NPU_ERR_DEVICE;
+    int flaw = 0;
+    const int zero = 0;
+    if (hipMemcpy(&flaw, c->flaw, sizeof(flaw), hipMemcpyDeviceToHost) != hipSuccess) return RK_NPU_ERR_DEVICE;
+    if (flaw && hipMemcpy(c->flaw, &zero, sizeof(zero), hipMemcpyHostToDevice) != hipSuccess) return RK_NPU_ERR_DEVICE;
+    return flaw ? RK_NPU_ERR_PARAM : RK_NPU_OK;
+}
+
+int rk_npu_hip_attention_paged_append(rk_npu_hip_attention_paged_pool* pool, const rk_npu_hip_paged_batch* batch,
+                                      const rk_npu_hip_heads* k, const rk_npu_hip_heads* v, const int32_t* positions,
+                                      const rk_npu_hip_heads* q, const rk_npu_hip_heads* q_out, void* stream) {
+    PagedPool* c = as_pool(pool);
+    if (!c || !valid_batch(c, batch) || !q != !q_out) return RK_NPU_ERR_PARAM;
+    const int device = device_of(c->domain), kh = c->cfg.attention.kv_heads, qh = c->cfg.attention.query_heads;
+    const int D = c->cfg.attention.head_dim, rows = batch->rows;
+    if (!valid_heads(k, device, D, false, kh, rows) || !valid_heads(v, device, D, false, kh, rows))
+        return RK_NPU_ERR_PARAM;
+    if (q && (!valid_heads(q, device, D, false, qh, rows) || !valid_heads(q_out, device, D, true, qh, rows)))
+        return RK_NPU_ERR_PARAM;
+    // (in place: each thread writes what it alone has read)
+    if (q && q->data == q_out->data &&
+        (q->type != q_out->type || q->head_stride != q_out->head_stride || q->row_stride != q_out->row_stride))
+        return RK_NPU_ERR_PARAM;
+    if (positions && (reinterpret_cast<uintptr_t>(positions) % sizeof(int32_t) || !kernel_readable(positions, device)))
+        return RK_NPU_ERR_PARAM;
+    DeviceGuard dev(device);
+    if (!dev.ok) return RK_NPU_ERR_DEVICE;
+    PagedRowsParams P = rows_params(c, batch);
+    P.k = view_of(*k);
+    P.v = view_of(*v);
+    if (q) {
+        P.q = view_of(*q);
+        P.q_out = view_of(*q_out);
+        P.qh = qh;
+    }
+    P.positions = positions;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int heads = P.qh + 2 * kh;
+    P.rows_per_block = 1;
+    P.heads_per_block = heads;
+    hipLaunchKernelGGL(paged_append_kernel<1>, dim3(rows, 1), dim3(256), 0, s, P);
+    if (hipGetLastError() != hipSuccess) return RK_NPU_ERR_DEVICE;
+    c->fence.note(s);
+    return RK_NPU_OK;
+}
+
+int rk_npu_hip_attention_paged_read(rk_npu_hip_attention_paged_pool* pool, const rk_npu_hip_paged_batch* batch,
+                                    const rk_npu_hip_heads* k, const rk_npu_hip_heads* v, void* stream) {
+    PagedPool* c = as_pool(pool);
+    if (!c || !valid_batch(c, batch) || (!k && !v)) return RK_NPU_ERR_PARAM;
+    const int device = device_of(c->domain), kh = c->cfg.attention.kv_heads, D = c->cfg.attention.head_dim;
+    if ((k && !valid_heads(k, device, D, true, kh, batch->rows)) || (v && !valid_heads(v, device, D, true, kh, batch->rows)))
+        return RK_NPU_ERR_PARAM;
+    DeviceGuard dev(device);
+    if (!dev.ok) return RK_NPU_ERR_DEVICE;
+    PagedRowsParams P = rows_params(c, batch);
+    if (k) P.k = view_of(*k);
+    if (v) P.v = view_of(*v);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    P.rows_per_block = 1;
+    P.heads_per_block = 2 * kh;
+    hipLaunchKernelGGL(paged_read_kernel<1>, dim3(batch->rows, 1), dim3(256), 0, s, P);
+    if (hipGetLastError() != hipSuccess) return RK_NPU_ERR_DEVICE;
+    c->fence.note(s);
+    return RK_NPU_OK;
+}
+
+int rk_npu_hip_attention_paged_run(rk_npu_attention_f16_workspace* workspace, rk_npu_hip_attention_paged_pool* pool,
+                                   const rk_npu_hip_paged_batch* batch, const rk_npu_hip_heads* q,
+                                   const rk_npu_hip_heads* out, void* stream) {
+    AttnWork* w = as_attn_work(workspace);
+    PagedPool* c = as_pool(pool);
+    if (!w || !c || !paged_same_geometry(w, c) || !valid_batch(c, batch)) return RK_NPU_ERR_PARAM;
+    const rk_npu_attention_f16_config& cfg = c->cfg.attention;
+    const int device = device_of(c->domain), D = cfg.head_dim;
+    if ((int64_t)batch->rows * cfg.query_heads > RK_NPU_HIP_PAGED_MAX_QUERIES) return RK_NPU_ERR_PARAM;
+    if (!valid_heads(q, device, D, false, cfg.query_heads, batch->rows) ||
+        !valid_heads(out, device, D, true, cfg.query_heads, batch->rows))
+        return RK_NPU_ERR_PARAM;
+    DeviceGuard dev(device);
+    if (!dev.ok) return RK_NPU_ERR_DEVICE;
+    AttnPagedParams P;
+    P.b = batch_of(c, batch);
+    P.q = q->data;
+    P.q_f32 = q->type == RK_NPU_HIP_F32;
+    P.q_head = q->head_stride;
+    P.q_row = q->row_stride;
+    P.out = out->data;
+    P.out_f16 = out->type == RK_NPU_HIP_F16;
+    P.o_head = out->head_stride;
+    P.o_row = out->row_stride;
+    P.part = w->part;
+    P.qh = cfg.query_heads;
+    P.causal = cfg.mask_mode == RK_NPU_ATTENTION_F16_CAUSAL ? 1 : 0;
+    P.scale = cfg.softmax_scale;
+    paged_plan(P, D);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (D == 64)
+        launch_paged<64>(P, s);
+    else if (D == 128)
+        launch_paged<128>(P, s);
+    else
+        launch_paged<256>(P, s);
+    if (hipGetLastError() != hipSuccess) return RK_NPU_ERR_DEVICE;
+    c->fence.note(s);
+    w->fence.note(s);
+    return RK_NPU_OK;
+}
+
+}  // extern "C"

@@ -41,12 +41,6 @@ __device__ __forceinline__ int q8_vt_at(int j, int d) {
     return ((d >> 4) * 64 + ((j >> 2) & 3) * 16 + (d & 15)) * 8 + (j >> 4) * 4 + (j & 3);
 }
 
-struct HeadsView {  // rk_npu_hip_heads in a kernel's arguments
-    void* data;
-    int f32;
-    long long head, row;
-};
-
 struct Q8WriteParams {
     HeadsView src[2];  // K, V: the appended rows
     uint8_t* codes[2];
@@ -479,20 +473,6 @@ static Q8Cache* as_q8(const void* p) {
     return (c && c->magic == MAGIC_Q8_CACHE) ? c : nullptr;
 }
 
-// The calls leave the calling thread's current device as it was.
-struct DeviceGuard {
-    int before = -1;
-    bool ok;
-    explicit DeviceGuard(int device) {
-        if (hipGetDevice(&before) != hipSuccess) before = -1;
-        ok = before == device || hipSetDevice(device) == hipSuccess;
-        if (before == device) before = -1;
-    }
-    ~DeviceGuard() {
-        if (before >= 0) (void)hipSetDevice(before);
-    }
-};
-
 static bool valid_q8(const rk_npu_hip_attention_q8_config* c) {
     return c && valid_config(&c->attention) && (c->format == RK_NPU_HIP_KV_I8 || c->format == RK_NPU_HIP_KV_E4M3) &&
            (c->block == 32 || c->block == 64 || c->block == 128) && c->attention.max_capacity <= INT_MAX - 255;
@@ -562,26 +542,6 @@ static int q8_grow(Q8Cache* c, int capacity) {
     c->scale_bytes = sb;
     c->generation += 1;
     return RK_NPU_OK;
-}
-
-static bool valid_heads(const rk_npu_hip_heads* a, int device, int head_dim, bool written, int heads, int rows) {
-    if (!a || !a->data || (a->type != RK_NPU_HIP_F16 && a->type != RK_NPU_HIP_F32) || a->head_stride < 0 ||
-        a->row_stride < 0)
-        return false;
-    const uintptr_t element = a->type == RK_NPU_HIP_F16 ? 2 : 4;
-    if (reinterpret_cast<uintptr_t>(a->data) % element) return false;
-    if (a->head_stride > ((int64_t)1 << 46) || a->row_stride > ((int64_t)1 << 40)) return false;
-    if (written) {
-        // rows of head_dim values must not overlap, in a head or over the heads
-        const int64_t hs = a->head_stride, rs = a->row_stride;
-        const bool by_head = (rows == 1 || rs >= head_dim) && (heads == 1 || hs >= (int64_t)(rows - 1) * rs + head_dim);
-        const bool by_row = (heads == 1 || hs >= head_dim) && (rows == 1 || rs >= (int64_t)(heads - 1) * hs + head_dim);
-        if (!by_head && !by_row) return false;
-    }
-    return kernel_readable(a->data, device);
-}
-static HeadsView view_of(const rk_npu_hip_heads& a) {
-    return HeadsView{a.data, a.type == RK_NPU_HIP_F32 ? 1 : 0, (long long)a.head_stride, (long long)a.row_stride};
 }
 
 template <int D, int FMT>

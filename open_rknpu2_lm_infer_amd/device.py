@@ -118,8 +118,8 @@ class DeviceContext:
                                         L.rk_npu_matmul_workspace_free, "W8 workspace", self.shared)
         return self._ws[key]
 
-    def attention_workspace(self, cache: "KvCacheQ8", own: bool = False) -> _Handle:
-        """The context's attention workspace for the cache's geometry, created on
+    def attention_workspace(self, cache, own: bool = False) -> _Handle:
+        """The context's attention workspace for the geometry of a cache (KvCacheQ8 or KvPages), created on
         first use (rk_npu_attention_f16_prepare); own: a new one, for calls that
         overlap others (a second stream, graphs launched side by side)."""
         c = cache.config.attention
@@ -266,6 +266,132 @@ def attention_q8(ctx: DeviceContext, cache: KvCacheQ8, q, out, position: int, ws
     check(F.lib().rk_npu_hip_attention_q8_device_run(ws.raw, cache.handle.raw, ctypes.byref(qh), shape[1],
                                                      int32(position, "position"), ctypes.byref(oh),
                                                      _stream(stream, q)), "8-bit KV attention")
+
+
+def _ints(t, name: str, shape) -> int:
+    """The address of a cuda int32 tensor of this shape, its last dimension contiguous."""
+    import torch
+    if not (t.is_cuda and t.dtype == torch.int32 and tuple(t.shape) == tuple(shape) and
+            (t.shape[-1] <= 1 or t.stride(-1) == 1)):
+        raise NpuError(f"{name} is a cuda int32 tensor {list(shape)}, contiguous")
+    return t.data_ptr()
+
+
+class PagedBatch:
+    """The sequences of a call on a KvPages (rk_npu_attention_paged.h), in cuda int32
+    tensors that are read when the work runs: table [sequences][pages], the page of
+    token t being table[s][t // page]; lengths [sequences], the call's rows among
+    them; row_offsets [sequences + 1], sequence s having rows row_offsets[s] to
+    row_offsets[s + 1], or None: row s. No sequence has more than max_rows rows or
+    max_tokens tokens (default: what the table holds)."""
+
+    def __init__(self, table, lengths, row_offsets=None, max_rows: int = 1, max_tokens: Optional[int] = None):
+        ensure(len(table.shape) == 2 and len(lengths.shape) == 1, "a table is [sequences][pages], lengths [sequences]")
+        n = lengths.shape[0]
+        self.table, self.lengths, self.row_offsets = table, lengths, row_offsets
+        self.sequences, self.max_rows, self.max_tokens = n, int32(max_rows, "max_rows"), max_tokens
+        if max_tokens is not None:
+            int32(max_tokens, "max_tokens")
+        self._stride = int32(table.shape[1] if n <= 1 else table.stride(0), "the table's stride")
+        ensure(n <= 1 or self._stride >= table.shape[1], "the table's rows overlap")
+        self._at = (_ints(lengths, "lengths", (n,)),
+                    None if row_offsets is None else _ints(row_offsets, "row_offsets", (n + 1,)),
+                    _ints(table, "table", (n, table.shape[1])))
+
+    def _raw(self, rows: int, page: int) -> F.rk_npu_hip_paged_batch:
+        most = self.table.shape[1] * page
+        tokens = min(most, 2 ** 31 - 1) if self.max_tokens is None else self.max_tokens
+        if tokens > most:
+            raise NpuError(f"the table holds {most} tokens a sequence, max_tokens is {tokens}")
+        lengths, offsets, table = self._at
+        return F.rk_npu_hip_paged_batch(self.sequences, int32(rows, "rows"), self.max_rows, tokens, lengths, offsets,
+                                        table, self._stride)
+
+
+class KvPages:
+    """A pool of `pages` pages of `page` tokens (16 to 256) of fp16 K and V for many
+    sequences (rk_npu_attention_paged.h), none longer than `capacity` tokens (default:
+    the pool's). append rotates the first rotary_dim dims of K and query rows by
+    positions times rope_theta^(-2j / rotary_dim), or times frequencies[j] (a
+    sequence of rotary_dim / 2 floats), pairs (j, j + rotary_dim / 2) or, interleaved,
+    (2j, 2j + 1).
+
+    Arrays are cuda tensors [heads][rows][head_dim], f16 or f32, any strides of
+    heads and rows."""
+
+    def __init__(self, ctx: DeviceContext, query_heads: int, kv_heads: int, head_dim: int, softmax_scale: float,
+                 pages: int, page: int = 64, capacity: Optional[int] = None, causal: bool = True, rotary_dim: int = 0,
+                 rope_theta: float = 10000.0, interleaved: bool = False, frequencies=None):
+        capacity = min(pages * page, 2 ** 31 - 256) if capacity is None else capacity
+        for name, value in (("query_heads", query_heads), ("kv_heads", kv_heads), ("head_dim", head_dim),
+                            ("pages", pages), ("page", page), ("capacity", capacity), ("rotary_dim", rotary_dim)):
+            int32(value, name)
+        L = F.lib()
+        cfg = F.rk_npu_hip_attention_paged_config()
+        L.rk_npu_hip_attention_paged_config_init(ctypes.byref(cfg))
+        a = cfg.attention
+        a.query_heads, a.kv_heads, a.head_dim, a.softmax_scale = query_heads, kv_heads, head_dim, softmax_scale
+        a.max_query_rows, a.max_capacity, a.initial_capacity = 1, capacity, 0
+        a.mask_mode = F.RK_NPU_ATTENTION_F16_CAUSAL if causal else F.RK_NPU_ATTENTION_F16_NO_MASK
+        cfg.page, cfg.pages, cfg.rotary_dim, cfg.interleaved, cfg.rope_theta = page, pages, rotary_dim, interleaved, rope_theta
+        if frequencies is not None:
+            frequencies = [float(f) for f in frequencies]
+            ensure(2 * len(frequencies) == rotary_dim, "there are rotary_dim / 2 frequencies")
+            if frequencies:
+                cfg.frequencies = (ctypes.c_double * len(frequencies))(*frequencies)
+        raw = ctypes.c_void_p()
+        check(L.rk_npu_hip_attention_paged_pool_create(ctx.domain, ctypes.byref(cfg), ctypes.byref(raw)),
+              "create the KV pages")
+        self.handle = _Handle(raw.value, L.rk_npu_hip_attention_paged_pool_free, "KV pages", ctx.shared)
+        self.ctx, self.config, self.page = ctx, cfg, page
+        self._kv, self._query = (kv_heads, head_dim), (query_heads, head_dim)
+
+    def bytes(self) -> int:
+        sizes = F.rk_npu_attention_f16_sizes()
+        check(F.lib().rk_npu_hip_attention_paged_query(ctypes.byref(self.config), ctypes.byref(sizes)), "KV pages' sizes")
+        return sizes.key_bytes + sizes.value_bytes
+
+    def check(self) -> None:
+        """Waits for the calls made and raises where the device found a wrong length, offset or page since the last check."""
+        check(F.lib().rk_npu_hip_attention_paged_status(self.handle.raw), "a length, row offset or page out of range")
+
+    def append(self, batch: PagedBatch, k, v, q=None, q_out=None, positions=None, stream=None) -> None:
+        """Puts the batch's rows k and v, [kv_heads][rows][head_dim], into their pages, k
+        rotated, and the query rows q, rotated, into q_out (q itself, or another array).
+        positions: cuda int32 [rows], by default the rows' tokens."""
+        rows = k.shape[1]
+        ensure(k.shape == v.shape, "k and v must have the same shape")
+        kh, vh = _heads(k, *self._kv), _heads(v, *self._kv)
+        ensure((q is None) == (q_out is None), "q and q_out come together")
+        qh = oh = None
+        if q is not None:
+            ensure(q.shape == q_out.shape and q.shape[1] == rows, "q, q_out and k must have the same rows")
+            qh, oh = ctypes.byref(_heads(q, *self._query)), ctypes.byref(_heads(q_out, *self._query))
+        at = None if positions is None else _ints(positions, "positions", (rows,))
+        check(F.lib().rk_npu_hip_attention_paged_append(self.handle.raw, ctypes.byref(batch._raw(rows, self.page)),
+                                                        ctypes.byref(kh), ctypes.byref(vh), at, qh, oh,
+                                                        _stream(stream, k)), "append to the KV pages")
+
+    def read(self, batch: PagedBatch, k, v, stream=None) -> None:
+        """The batch's rows as the pages hold them, into k and v, [kv_heads][rows][head_dim]."""
+        ensure(k.shape == v.shape, "k and v must have the same shape")
+        kh, vh = _heads(k, *self._kv), _heads(v, *self._kv)
+        check(F.lib().rk_npu_hip_attention_paged_read(self.handle.raw, ctypes.byref(batch._raw(k.shape[1], self.page)),
+                                                      ctypes.byref(kh), ctypes.byref(vh), _stream(stream, k)),
+              "read the KV pages")
+
+
+def attention_paged(ctx: DeviceContext, pages: KvPages, batch: PagedBatch, q, out, ws=None, stream=None):
+    """Attention of the batch's rows q [query_heads][rows][head_dim] over their
+    sequences' pages. ws: the context's workspace of this geometry, which calls on
+    one stream share."""
+    shape = q.shape
+    ensure(shape == out.shape, "q and out must have the same shape")
+    ws = ws or ctx.attention_workspace(pages)
+    qh, oh = _heads(q, *pages._query), _heads(out, *pages._query)
+    check(F.lib().rk_npu_hip_attention_paged_run(ws.raw, pages.handle.raw, ctypes.byref(batch._raw(shape[1], pages.page)),
+                                                 ctypes.byref(qh), ctypes.byref(oh), _stream(stream, q)),
+          "attention over the KV pages")
 
 
 @contextlib.contextmanager

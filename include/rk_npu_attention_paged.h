@@ -42,8 +42,9 @@
  * that fall or pass `rows` or give a sequence more than max_rows, and a page
  * outside 0..pages - 1 (or a negative one) under a token of its sequence are noted
  * on the device, and nothing is read or written out of bounds: the sequence counts
- * as one of no rows (wrong row_offsets) or of no tokens, the page as one of no
- * tokens. rk_npu_hip_attention_paged_status() tells of it.
+ * as one of no rows (wrong row_offsets) or of no tokens; to the page nothing is
+ * appended, from it nothing is read, and the attention of the rows that see it has
+ * no meaning. rk_npu_hip_attention_paged_status() tells of it.
  *
  * Workspaces are rk_npu_attention_f16_workspace of the same geometry
  * (rk_npu_attention_f16_prepare with &config.attention).
@@ -61,10 +62,11 @@
 extern "C" {
 #endif
 
-/* Sequences and rows of a batch, and rows x query heads of an attention call, at most. */
+/* Sequences and rows of a batch, rows x query heads of an attention call, and tokens of a sequence, at most. */
 #define RK_NPU_HIP_PAGED_MAX_SEQUENCES 1024
 #define RK_NPU_HIP_PAGED_MAX_ROWS (1 << 23)
 #define RK_NPU_HIP_PAGED_MAX_QUERIES (1 << 26)
+#define RK_NPU_HIP_PAGED_MAX_TOKENS (1 << 30)
 
 typedef struct rk_npu_hip_attention_paged_config {
     rk_npu_attention_f16_config attention; /* head_dim 64, 128 or 256; max_capacity: the longest sequence

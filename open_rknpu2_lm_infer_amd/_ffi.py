@@ -195,6 +195,7 @@ class rk_npu_hip_heads(Structure):
 RK_NPU_HIP_PAGED_MAX_SEQUENCES = 1024
 RK_NPU_HIP_PAGED_MAX_ROWS = 1 << 23
 RK_NPU_HIP_PAGED_MAX_QUERIES = 1 << 26
+RK_NPU_HIP_PAGED_MAX_TOKENS = 1 << 30
 
 
 class rk_npu_hip_attention_paged_config(Structure):

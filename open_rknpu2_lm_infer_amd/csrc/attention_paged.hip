@@ -235,7 +235,7 @@ static bool valid_paged(const rk_npu_hip_attention_paged_config* c) {
             if (!std::isfinite(c->frequencies[i])) return false;
     // (kernels count the pool's 16-token tiles in 32 bits)
     return c->pages >= 1 && (int64_t)c->pages * c->attention.kv_heads * (c->page / 16) <= INT_MAX &&
-           c->attention.max_capacity <= INT_MAX - 255;
+           c->attention.max_capacity <= RK_NPU_HIP_PAGED_MAX_TOKENS;
 }
 static size_t paged_kv_bytes(const rk_npu_hip_attention_paged_config& c) {
     return (size_t)c.pages * c.page * c.attention.kv_heads * c.attention.head_dim * sizeof(__half);
@@ -293,35 +293,35 @@ static bool paged_same_geometry(const AttnWork* w, const PagedPool* c) {
            device_of(w->domain) == device_of(c->domain);
 }
 
-// Row tiles, and the blocks that splits aim at.
-static void paged_plan(AttnPagedParams& P, int D) {
+// Which kernel, its row tiles, and the blocks that splits aim at.
+static PagedPlan paged_plan(AttnPagedParams& P, int D, int64_t pool_bytes) {
     const PagedBatch& B = P.b;
-    const int G = P.qh / B.kh;
-    P.tile_rows = (int64_t)B.max_rows * G <= 8 ? 8 : 16;
+    const int G = P.qh / B.kh, cus = device_cus();
+    const int64_t R = (int64_t)B.max_rows * G;
     // (each sequence ends a tile of its own)
-    const int64_t tiles = std::min<int64_t>((int64_t)B.sequences * (((int64_t)B.max_rows * G + P.tile_rows - 1) / P.tile_rows),
-                                            (int64_t)B.rows * G / P.tile_rows + B.sequences);
-    P.tiles = (int)std::min<int64_t>(tiles, INT_MAX / 2);
+    auto tiles = [&](int rows) {
+        return std::min<int64_t>(B.sequences * ((R + rows - 1) / rows), (int64_t)B.rows * G / rows + B.sequences);
+    };
+    const int units = (B.max_tokens + 31) / 32;
+    PagedPlan plan{R > 32, D < 256 && units > 128 ? 2 : 1, false};
+    if (plan.tile) {
+        P.tile_rows = 128 * plan.units;
+    } else {
+        P.tile_rows = R <= 8 ? 8 : 16;
+        const int64_t bytes = std::min<int64_t>(pool_bytes, 4LL * B.sequences * B.max_tokens * B.kh * D);
+        plan.once = R <= P.tile_rows && bytes > (512 << 20);
+    }
+    P.tiles = (int)tiles(P.tile_rows);
     P.least = 8;
     P.target = 0;
-    const int units = (B.max_tokens + 31) / 32, want = std::max(1, 2 * device_cus() / B.kh);
-    const int64_t items = (int64_t)P.tiles + want;
+    const int blocks = plan.tile ? (plan.units == 1 && D < 256 ? 2 : 1) : B.sequences > 4 ? 4 : 1;
+    // (as many as the workspace holds partials for)
+    const int64_t room = (int64_t)(attn_partial_rows(D) / ((size_t)B.kh * P.tile_rows)) - P.tiles;
+    const int want = (int)std::min<int64_t>(std::max(1, blocks * cus / B.kh), room);
     // (units are added up in 32 bits)
-    if (units > 16 && P.tiles < want && (int64_t)P.tiles * units < (1 << 30) &&
-        (size_t)(items * B.kh * P.tile_rows) <= attn_partial_rows(D))
-        P.target = want;
-    P.items = P.target ? (int)items : P.tiles;
-}
-
-template <int D>
-static void launch_paged(const AttnPagedParams& P, hipStream_t s) {
-    const dim3 grid(P.b.kh * P.items);
-    if (P.tile_rows == 8)
-        hipLaunchKernelGGL((attn_paged_rows_kernel<D, 4, true>), grid, dim3(256), 0, s, P);
-    else
-        hipLaunchKernelGGL((attn_paged_rows_kernel<D, 4, false>), grid, dim3(256), 0, s, P);
-    if (P.target)
-        hipLaunchKernelGGL((attn_paged_join_kernel<D>), dim3(P.b.kh, P.tiles, P.tile_rows), dim3(256), 0, s, P);
+    if (units > 16 && P.tiles < want && (int64_t)P.tiles * units < (1 << 30)) P.target = want;
+    P.items = P.target ? P.tiles + want : P.tiles;
+    return plan;
 }
 
 }  // namespace hm
@@ -501,14 +501,14 @@ int rk_npu_hip_attention_paged_run(rk_npu_attention_f16_workspace* workspace, rk
     P.qh = cfg.query_heads;
     P.causal = cfg.mask_mode == RK_NPU_ATTENTION_F16_CAUSAL ? 1 : 0;
     P.scale = cfg.softmax_scale;
-    paged_plan(P, D);
+    const PagedPlan plan = paged_plan(P, D, 2 * (int64_t)c->kv_bytes);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (D == 64)
-        launch_paged<64>(P, s);
+        launch_attn_paged_64(P, plan, s);
     else if (D == 128)
-        launch_paged<128>(P, s);
+        launch_attn_paged_128(P, plan, s);
     else
-        launch_paged<256>(P, s);
+        launch_attn_paged_256(P, plan, s);
     if (hipGetLastError() != hipSuccess) return RK_NPU_ERR_DEVICE;
     c->fence.note(s);
     w->fence.note(s);

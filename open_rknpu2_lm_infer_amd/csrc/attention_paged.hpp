@@ -2,7 +2,7 @@
 //
 // Layout in HBM, per page and KV head, `page` tokens in tiles of 16:
 //   K: [4-key group][D / 8 pieces][4 keys][8 dims]; piece p of group n lies at
-//      place p ^ (n & 3). A lane of a matrix operand takes one piece, lanes of
+//      place p ^ k_turn(n). A lane of a matrix operand takes one piece, lanes of
 //      4 keys a 64-byte line;
 //   V: [key][D / 8 pieces][8 dims], piece p of key j at place p ^ v_turn(j).
 // The turned places keep 16 keys' pieces out of each other's LDS banks when a
@@ -44,11 +44,17 @@ struct PagedBatch {
     int kh, pages, page_shift;
 };
 
+// (0, 2, 3, 1: a 16-byte LDS read takes lanes 0..3, 12..15, 20..27 at a time, in operands
+// of 16 keys groups 0 and 3 of one piece with 1 and 2 of the next)
+__device__ __forceinline__ constexpr int pg_k_turn(int n) { return (0x78 >> (2 * (n & 3))) & 3; }
 __device__ __forceinline__ int pg_k_place(int D, int j, int piece) {  // of piece `piece` of key j, in 8 halves
-    return (j >> 2) * (D >> 1) + (piece ^ ((j >> 2) & 3)) * 4 + (j & 3);
+    return (j >> 2) * (D >> 1) + (piece ^ pg_k_turn(j >> 2)) * 4 + (j & 3);
 }
-// (heads of 64: two keys fill the 256 bytes of the banks)
-__device__ __forceinline__ constexpr int pg_v_turn(int D, int j) { return D == 64 ? 2 * ((j >> 1) & 3) : 2 * (j & 7); }
+// (heads of 64: two keys fill the 256 bytes of the banks; of 256: operands of 16 dims,
+// of 8 keys for 32 lanes at a time)
+__device__ __forceinline__ constexpr int pg_v_turn(int D, int j) {
+    return D == 64 ? 4 * ((j >> 1) & 1) : D == 128 ? 4 * (j & 3) : 2 * (j & 7);
+}
 __device__ __forceinline__ int pg_v_place(int D, int j, int piece) { return j * (D >> 3) + (piece ^ pg_v_turn(D, j)); }
 
 __device__ __forceinline__ void pg_flaw(const PagedBatch& B) { atomicOr(B.flaw, 1); }
@@ -78,6 +84,13 @@ __device__ __forceinline__ int pg_page(const PagedBatch& B, int s, int token) {
     if ((unsigned)p < (unsigned)B.pages) return p;
     pg_flaw(B);
     return -1;
+}
+
+// The 16-key tile of the pool that holds KV head g of such a token (of a wrong page:
+// tile 0, whose values have no meaning there).
+__device__ __forceinline__ int pg_tile(const PagedBatch& B, int s, int g, int token) {
+    const int page = pg_page(B, s, token), tiles = 1 << (B.page_shift - 4);
+    return page < 0 ? 0 : (page * B.kh + g) * tiles + ((token >> 4) & (tiles - 1));
 }
 
 struct AttnPagedParams {
@@ -119,34 +132,36 @@ struct PagedItem {
 // tile_rows) tiles, each split into as many pieces of at least `per` units of 32 keys
 // as it has; per is the batch's units over `target`, so that splits of short and long
 // sequences take the same time. Blocks of a sequence lie in the order of their tiles,
-// then splits. Counted by tiles alone (`joins`), index `at` is the tile of a join.
-// Lane l has sequences l C..l C + C - 1.
+// the last first (causal ones see the most keys), then splits. Counted by tiles alone
+// (`joins`), index `at` is the tile of a join. Lane l has sequences l C..l C + C - 1.
 __device__ __forceinline__ PagedItem pg_item(const AttnPagedParams& P, int at, int lane, bool joins) {
     const PagedBatch& B = P.b;
     const int G = P.qh / B.kh, C = (B.sequences + 63) >> 6;
-    auto tiles_of = [&](const PagedSeq& q) { return (int)(((long long)q.n * G + P.tile_rows - 1) / P.tile_rows); };
-    int per = 0x7fffffff;
+    auto tiles_of = [&](const PagedSeq& q) { return (int)(((unsigned)q.n * (unsigned)G + P.tile_rows - 1) / (unsigned)P.tile_rows); };
+    const PagedSeq none{0, 0, 0};
+    PagedSeq mine = lane * C < B.sequences ? pg_seq(B, lane * C) : none;
+    // (one sequence a lane: the one in registers)
+    auto seq = [&](int i) { return C == 1 ? mine : lane * C + i < B.sequences ? pg_seq(B, lane * C + i) : none; };
+    unsigned per = 0x7fffffff;
     if (P.target > 0) {
         int units = 0;
         for (int i = 0; i < C; ++i) {
-            const int s = lane * C + i;
-            if (s >= B.sequences) break;
-            const PagedSeq q = pg_seq(B, s);
+            const PagedSeq q = seq(i);
             units += tiles_of(q) * ((q.len + 31) >> 5);
         }
-        const int total = __builtin_amdgcn_readlane(pg_scan(units), 63);
-        per = max(P.least, (total + P.target - 1) / P.target);
+        const unsigned total = __builtin_amdgcn_readlane(pg_scan(units), 63);
+        per = max((unsigned)P.least, (total + P.target - 1) / (unsigned)P.target);
     }
     auto splits_of = [&](const PagedSeq& q) {
-        return min(PAGED_MAX_SPLITS, max(1, (int)(((q.len + 31) >> 5) + (long long)per - 1) / per));
+        const unsigned units = (unsigned)(q.len + 31) >> 5;
+        return P.target > 0 ? min(PAGED_MAX_SPLITS, max(1, (int)((units + per - 1) / per))) : 1;
     };
     int items = 0, tiles = 0;
     for (int i = 0; i < C; ++i) {
-        const int s = lane * C + i;
-        if (s >= B.sequences) break;
-        const PagedSeq q = pg_seq(B, s);
-        items += tiles_of(q) * splits_of(q);
-        tiles += tiles_of(q);
+        const PagedSeq q = seq(i);
+        const int t = tiles_of(q);
+        items += t * splits_of(q);
+        tiles += t;
     }
     const int item_end = pg_scan(items), tile_end = pg_scan(tiles);
     const int end = joins ? tile_end : item_end;
@@ -159,7 +174,14 @@ __device__ __forceinline__ PagedItem pg_item(const AttnPagedParams& P, int at, i
     int before = __builtin_amdgcn_readlane(end - (joins ? tiles : items), owner);
     for (int i = 0; i < C; ++i) {
         x.s = min(owner * C + i, B.sequences - 1);
-        const PagedSeq q = pg_seq(B, x.s);
+        PagedSeq q;
+        if (C == 1) {
+            q.row = __builtin_amdgcn_readlane(mine.row, owner);
+            q.n = __builtin_amdgcn_readlane(mine.n, owner);
+            q.len = __builtin_amdgcn_readlane(mine.len, owner);
+        } else {
+            q = pg_seq(B, x.s);
+        }
         const int t = tiles_of(q), p = splits_of(q), count = joins ? t : t * p;
         if (at < before + count) {
             const int in = at - before;
@@ -167,9 +189,10 @@ __device__ __forceinline__ PagedItem pg_item(const AttnPagedParams& P, int at, i
             x.n = q.n;
             x.len = q.len;
             x.splits = p;
-            x.tile = joins ? in : in / p;
-            x.split = joins ? 0 : in - x.tile * p;
-            x.item = first + x.tile * p;
+            const int k = joins ? in : in / p;
+            x.tile = t - 1 - k;
+            x.split = joins ? 0 : in - k * p;
+            x.item = first + k * p;
             return x;
         }
         before += count;
@@ -209,6 +232,13 @@ __device__ __forceinline__ int pg_row_min(int v) {
     return min(v, dpp_move<DPP_ROW_MIRROR>(v));
 }
 
+// The same over each 32, in every lane (both halves hold the same).
+__device__ __forceinline__ int pg_lo_min(int v) {
+    v = pg_row_min(v);
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return __builtin_amdgcn_readfirstlane(min((int)a[0], (int)a[1]));
+}
+
 // A row's maximum before it has seen a key: finite, so that differences are no NaN.
 constexpr float PG_NONE = -1e30f;
 // The weight 2^d of a partial result whose maximum lies d <= 0 below the row's:
@@ -231,6 +261,17 @@ __device__ __forceinline__ void pg_store8(const AttnPagedParams& P, long long at
         float* p = static_cast<float*>(P.out) + at;
         *reinterpret_cast<pg_f4a4*>(p) = pg_f4a4{y[0], y[1], y[2], y[3]};
         *reinterpret_cast<pg_f4a4*>(p + 4) = pg_f4a4{y[4], y[5], y[6], y[7]};
+    }
+}
+
+__device__ __forceinline__ void pg_store4(const AttnPagedParams& P, long long at, float a, float b, float c, float d) {
+    if (P.out_f16) {
+        const unsigned short h0 = __half_as_ushort(__float2half_rn(a)), h1 = __half_as_ushort(__float2half_rn(b));
+        const unsigned short h2 = __half_as_ushort(__float2half_rn(c)), h3 = __half_as_ushort(__float2half_rn(d));
+        *reinterpret_cast<pg_u2a2*>(static_cast<__half*>(P.out) + at) =
+            pg_u2a2{h0 | ((unsigned)h1 << 16), h2 | ((unsigned)h3 << 16)};
+    } else {
+        *reinterpret_cast<pg_f4a4*>(static_cast<float*>(P.out) + at) = pg_f4a4{a, b, c, d};
     }
 }
 
@@ -260,7 +301,7 @@ constexpr float PG_LAZY = 4.0f, PG_SHIFT = 10.0f;
 // is transposed there, two keys' halves a v_perm_b32. Weights go into the products
 // with V as two fp16. PACK: columns 8..15 are columns 0..7 again and take the second
 // fp16, so that both cost one product.
-template <int D, int NW, bool PACK>
+template <int D, int NW, bool PACK, bool ONCE>
 __global__ __launch_bounds__(64 * NW) void attn_paged_rows_kernel(AttnPagedParams P) {
     constexpr int KS = D / 32;                  // 32-dim steps of a score
     constexpr int DW = D == 64 ? 4 : 8;         // dims of V a lane takes of a key, H times
@@ -292,19 +333,22 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_rows_kernel(AttnPagedParam
 
     const float c = fminf(P.scale * 1.4426950408889634f, 0x1.fffffep127f);
     // Lane l's place in the table of the wave's next 32 units: unit l / 2, half l % 2,
-    // as 16-key tiles of the pool (-1: no token there).
-    const int page_tiles = 1 << (B.page_shift - 4);
+    // as 16-key tiles of the pool.
     auto places = [&](int u) {
         const int token = (u + NW * (lane >> 1)) * 32 + (lane & 1) * 16;
-        if (token >= min(seen, u_end * 32)) return -1;
-        const int page = pg_page(B, I.s, token);
-        return page < 0 ? -1 : (page * B.kh + g) * page_tiles + ((token >> 4) & (page_tiles - 1));
+        return token < min(seen, u_end * 32) ? pg_tile(B, I.s, g, token) : 0;
     };
-    int place = -1, place_at = -64 * NW;
+    int place = 0, place_at = -64 * NW;
     v4u kr[2][KS];
     v4u vr[2][4][H];
-    int tile[2];
-    auto load = [&](int u) {
+    auto get = [](const __half* p) __attribute__((always_inline)) {
+        const v4u* q = reinterpret_cast<const v4u*>(p);
+        if constexpr (ONCE)
+            return __builtin_nontemporal_load(q);
+        else
+            return *q;
+    };
+    auto load = [&](int u) __attribute__((always_inline)) {
         if (u - place_at >= 32 * NW) {
             place = places(u);
             place_at = u;
@@ -312,12 +356,11 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_rows_kernel(AttnPagedParam
         const int i = (u - place_at) / NW * 2;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            tile[t] = __builtin_amdgcn_readlane(place, i + t);
-            const size_t at = (size_t)max(tile[t], 0) * (16 * D);
-            const __half* kp = B.k + at;
-            const __half* vp = B.v + at;
+            const size_t tile = (size_t)__builtin_amdgcn_readlane(place, i + t) * (16 * D);
+            const __half* kp = B.k + tile;
+            const __half* vp = B.v + tile;
 #pragma unroll
-            for (int s = 0; s < KS; ++s) kr[t][s] = *reinterpret_cast<const v4u*>(kp + pg_k_place(D, lo, 4 * s + hi) * 8);
+            for (int s = 0; s < KS; ++s) kr[t][s] = get(kp + pg_k_place(D, lo, 4 * s + hi) * 8);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -327,7 +370,7 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_rows_kernel(AttnPagedParam
                         const uint2 x = *reinterpret_cast<const uint2*>(vp + pg_v_place(D, j, lo >> 1) * 8 + (lo & 1) * 4);
                         vr[t][k][w] = v4u{x.x, x.y, 0u, 0u};
                     } else {
-                        vr[t][k][w] = *reinterpret_cast<const v4u*>(vp + pg_v_place(D, j, 16 * w + lo) * 8);
+                        vr[t][k][w] = get(vp + pg_v_place(D, j, 16 * w + lo) * 8);
                     }
                 }
         }
@@ -348,18 +391,17 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_rows_kernel(AttnPagedParam
 #pragma unroll
             for (int i = 0; i < KS; ++i)
                 s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pg_h8, kr[t][i]), qf[i], s[t], 0, 0, 0);
-        const bool part = u * 32 + 32 > open || tile[0] < 0 || tile[1] < 0;
-        if (part) {  // (uniform)
+        if (u * 32 + 32 > open) {  // (uniform)
             unsigned odd = 0;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int key = u * 32 + 16 * t + 4 * hi + k;
-                    if (key >= lim || tile[t] < 0) s[t][k] = -INFINITY;
+                    if (key >= lim) s[t][k] = -INFINITY;
                     // (0 times what is not finite is NaN: such a value of a key that not
                     // every row sees is added after the last one)
-                    const bool none = key >= seen || tile[t] < 0;
+                    const bool none = key >= seen;
 #pragma unroll
                     for (int w = 0; w < H; ++w)
 #pragma unroll
@@ -444,9 +486,8 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_rows_kernel(AttnPagedParam
         for (int u = u_begin + wave; u < u_end; u += NW) {
 #pragma unroll 1
             for (int key = u * 32; key < min(u * 32 + 32, seen); ++key) {
-                const int page = pg_page(B, I.s, key), j = key & 15;
-                if (page < 0) continue;
-                const __half* vp = B.v + ((size_t)(page * B.kh + g) * page_tiles + ((key >> 4) & (page_tiles - 1))) * (16 * D);
+                const int j = key & 15;
+                const __half* vp = B.v + (size_t)pg_tile(B, I.s, g, key) * (16 * D);
 #pragma unroll
                 for (int w = 0; w < H; ++w)
 #pragma unroll
@@ -529,65 +570,475 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_rows_kernel(AttnPagedParam
     }
 }
 
-// The splits' partials of one row: out = sum_s w_s acc_s / sum_s w_s l_s with
-// w_s = 2^(m_s - max m). Block: one row of one row tile (blockIdx.y) and KV head; 256
-// threads, 8 dims of every 2048 / D-th split each.
-template <int D>
-__global__ __launch_bounds__(256) void attn_paged_join_kernel(AttnPagedParams P) {
-    constexpr int LD = D / 8, GS = 256 / LD;
-    __shared__ float weight[PAGED_MAX_SPLITS];
-    __shared__ float red[2][4];
-    __shared__ __attribute__((aligned(16))) float part[GS][D];
+// Many rows. Block: NW waves with W rows of one KV head of a sequence each; stages of U
+// units of 32 keys come through LDS, a 16-key tile of K or of V a wave (or half a one).
+// Operands of v_mfma_f32_32x32x16_f16 (W 32) and _16x16x32_ (W 16): A lane l = row
+// l % W, k-slots 8 (l / W)..+7; C lane l = rows 8 b + 4 (l / 32)..+3, b < 4, or 4 (l / 16)..+3,
+// of column l % W: again what B of O^T += V^T P^T wants, once V's slots name the same
+// keys (ds_read_b64_tr_b16 hands lane l of 16 one dim of 4 keys).
+//
+// In step j a wave turns the scores of unit j into weights, computes those of unit
+// j + 1 and multiplies V of unit j - 1: one straight piece of code in which matrix and
+// vector instructions do not depend on each other. In stage t K of stage t + 2 and V of
+// stage t + U - 1 go to LDS, loaded in the stage before.
+template <int D, int W, int U, int NW, bool SPLIT>
+__global__ __launch_bounds__(64 * NW) void attn_paged_tile_kernel(AttnPagedParams P) {
+    constexpr int CL = W * W / 64;                 // values of a lane in a C operand
+    constexpr int SN = 32 / W, NS = SN * CL;       // C operands of a unit's scores, a lane's scores
+    constexpr int KS = D * W / 512;                // steps of a score: 512 / W dims
+    constexpr int NB = D / W, VS = NS / 8;         // C operands of the output, key steps of a unit
+    constexpr int BUFS = U + 1, VA = U - 1, ROWS = NW * W;
+    constexpr int TILE = 32 * D;                   // bytes of 16 keys of K or V
+    constexpr int STAGE = 2 * U * TILE;            // of a stage's K, or V
+    constexpr int WT = NW / (4 * U);               // waves of a tile
+    constexpr int PT = TILE / 1024 / WT;           // 16-byte pieces of a lane's
+    constexpr float LAZY = SPLIT ? 8.0f : 6.0f, SHIFT = (SPLIT ? 14.0f : 15.0f) - LAZY;
+    static_assert(NW % (4 * U) == 0 && (U == 1 || U == 2) && (W == 16 || W == 32), "stage shape");
+    typedef float fv __attribute__((ext_vector_type(CL)));
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef short s8 __attribute__((ext_vector_type(8)));
+    typedef __attribute__((address_space(3))) s4 lds_s4;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * BUFS * STAGE];
+    __shared__ int dropped;
     const PagedBatch& B = P.b;
-    const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int g = blockIdx.x % B.kh, at = blockIdx.x / B.kh;
+    const int tid = threadIdx.x, lane = tid & 63, lo = lane % W, hi = lane / W;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const PagedItem I = pg_item(P, at, lane, false);
+    if (!I.any) return;  // (block-uniform)
+    const int G = P.qh / B.kh, R = G * I.n;
+    const int rr = (I.tile * NW + wave) * W + lo;
+    const bool live = rr < R;
+    const int r = live ? rr / G : 0, h = live ? rr - r * G : 0;
+    const int before = I.len - I.n;  // tokens before the rows' (causal)
+    const int lim = !live ? 0 : P.causal ? max(0, min(I.len, before + r + 1)) : I.len;
+    // keys below `open` every row of the wave sees
+    const int open = W == 32 ? pg_lo_min(live ? lim : 0x7fffffff)
+                             : __builtin_amdgcn_readfirstlane(pg_row_min(live ? lim : 0x7fffffff));
+    // keys that the block's last row sees, their units, and this block's
+    const int last = min(R, (I.tile + 1) * ROWS) - 1;
+    const int seen = P.causal ? max(0, min(I.len, before + last / G + 1)) : I.len, all = (seen + 31) >> 5;
+    const int each = (all + I.splits - 1) / I.splits;
+    const int u_begin = I.split * each, u_end = min(all, u_begin + each);
+    const int stages = (max(0, u_end - u_begin) + U - 1) / U;
+
+    pg_h8 qf[KS];
+    const long long q_at = (long long)(g * G + h) * P.q_head + (long long)(I.row + r) * P.q_row + 8 * hi;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) qf[i] = pg_load_q(P, q_at + 512 / W * i);
+    const float c = fminf(P.scale * 1.4426950408889634f, 0x1.fffffep127f);
+
+    // The first half of the waves loads K, the other V. Lane l has the place of the
+    // wave's tile in stage `place_at` + l.
+    const bool isv = wave >= NW / 2;
+    const int tile = wave % (NW / 2) / WT, part = wave % WT;
+    const __half* pool = isv ? B.v : B.k;
+    int place = 0, place_at = -64;
+    v4u raw[PT];
+    auto load = [&](int t) __attribute__((always_inline)) {
+        if (t - place_at >= 64) {
+            const int token = ((u_begin + (t + lane) * U) * 2 + tile) * 16;
+            place = token < min(u_end * 32, I.len) ? pg_tile(B, I.s, g, token) : 0;
+            place_at = t;
+        }
+        const __half* from = pool + (size_t)__builtin_amdgcn_readlane(place, t - place_at) * (16 * D) + (part * PT * 64 + lane) * 8;
+#pragma unroll
+        for (int i = 0; i < PT; ++i) raw[i] = *reinterpret_cast<const v4u*>(from + i * 512);
+    };
+    // (K's buffers, then V's; b: stage % BUFS)
+    uint8_t* const mine = smem + (isv ? BUFS * STAGE : 0) + tile * TILE + part * PT * 1024 + lane * 16;
+    // Values of V of keys that not every row of the block sees: what is not finite stays
+    // out of the products (0 times it is NaN) and is added after the last one.
+    const int sure = min(u_end * 32, P.causal ? max(0, min(I.len, before + I.tile * ROWS / G + 1)) : I.len);
+    auto store = [&](int t, int b) __attribute__((always_inline)) {
+        const int key0 = ((u_begin + t * U) * 2 + tile) * 16;
+        if (__builtin_expect(isv && key0 + 16 > sure, 0)) {  // (uniform)
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < PT; ++i) {
+                const int key = key0 + ((part * PT + i) * 64 + lane) / (D / 8);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    unsigned drop = (raw[i][k] & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u;
+                    drop |= (raw[i][k] & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u;
+                    if (key < sure) drop = 0u;
+                    odd |= drop != 0 && key < min(seen, u_end * 32);
+                    raw[i][k] &= ~drop;
+                }
+            }
+            if (odd) dropped = 1;
+        }
+#pragma unroll
+        for (int i = 0; i < PT; ++i) *reinterpret_cast<v4u*>(mine + b * STAGE + i * 1024) = raw[i];
+    };
+
+    float mrun = PG_NONE, lsum = 0.0f;
+    fv o[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) o[n] = fv{};
+    bool wild = false;
+    if (tid == 0) dropped = 0;
+    __syncthreads();
+    if (stages > 0) {
+        // (zeros for V of stage -1, whose weights are 0)
+        load(0);
+        if (U == 2 || !isv) store(0, 0);
+        if (isv) {
+#pragma unroll
+            for (int i = 0; i < PT; ++i) *reinterpret_cast<v4u*>(mine + (BUFS - 1) * STAGE + i * 1024) = v4u{0u, 0u, 0u, 0u};
+        } else {
+            load(1);
+            store(1, 1);
+        }
+        // In stage t: K of t + 2, V of t + VA.
+        if (U == 2 || !isv) load(isv ? VA : 2);
+        __syncthreads();
+        const int j4 = lane & 3;
+        // lane's pieces of K: key lo of the unit or tile, pieces 64 / W i + hi
+        const int kat = (W == 32 ? (lo >> 4) * TILE : 0) + ((lo & 15) >> 2) * (8 * D) + ((hi ^ pg_k_turn(lo >> 2)) * 4 + j4) * 16;
+        auto kop = [&](const uint8_t* unit, int i) {
+            return *reinterpret_cast<const pg_h8*>(unit + (W == 32 ? (kat ^ ((i & 1) * 128)) + (i >> 1) * 256 : kat + i * 256));
+        };
+        // lane's 4 halves of V: key 4 hi + (lane % 16) / 4 of 8 or 16, dims W n + 16 (lo / 16) + 4 (lane % 4)
+        const int vj = 4 * hi + ((lane & 15) >> 2);
+        const int vat = vj * 2 * D + (((lo >> 4) * 2 + (j4 >> 1)) ^ pg_v_turn(D, vj)) * 16 + (j4 & 1) * 8;
+        auto vop = [&](const uint8_t* unit, int n, int t) {
+            constexpr int MOST = 256 / (2 * W) - 1;  // (places turn within 256 bytes)
+            const uint8_t* p = unit + (vat ^ ((n & MOST) * (2 * W))) + n / (MOST + 1) * 256 + t * TILE;
+            const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p);
+            const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + (W == 32 ? 16 * D : TILE)));
+            return __builtin_bit_cast(pg_h8, s8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+        };
+        auto mfma = [](pg_h8 a, pg_h8 b, fv x) __attribute__((always_inline)) {
+            if constexpr (W == 32)
+                return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, x, 0, 0, 0);
+            else
+                return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, x, 0, 0, 0);
+        };
+        auto masked = [&](int j) { return (u_begin + j) * 32 + 32 > open || u_begin + j >= u_end; };
+        // (unit `sub` of the stage in buffers b)
+        auto scores = [&](fv (&s)[SN], int b, int sub) __attribute__((always_inline)) {
+            const uint8_t* k = smem + b * STAGE + sub * (2 * TILE);
+#pragma unroll
+            for (int x = 0; x < SN; ++x) {
+                s[x] = fv{};
+#pragma unroll
+                for (int i = 0; i < KS; ++i) s[x] = mfma(kop(k + x * TILE, i), qf[i], s[x]);
+            }
+        };
+        auto products = [&](int b, int sub, const pg_h8 (&ph)[VS], const pg_h8 (&pl)[VS]) __attribute__((always_inline)) {
+            const uint8_t* v = smem + (BUFS + b) * STAGE + sub * (2 * TILE);
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int t = 0; t < VS; ++t) {
+                    const pg_h8 a = vop(v, n, t);
+                    o[n] = mfma(a, ph[t], o[n]);
+                    if constexpr (SPLIT) o[n] = mfma(a, pl[t], o[n]);
+                }
+        };
+        // What a unit's scores need before they are weighed: masks, and whether a
+        // maximum moves.
+        float top = 0.0f;
+        auto look = [&](int j, fv (&s)[SN]) __attribute__((always_inline)) {
+            if (__builtin_expect(masked(j), 0)) {  // (uniform)
+                const bool none = u_begin + j >= u_end;
+#pragma unroll
+                for (int i = 0; i < NS; ++i) {
+                    const int key = (u_begin + j) * 32 + (W == 32 ? 8 : 16) * (i >> 2) + 4 * hi + (i & 3);
+                    if (none || key >= lim) s[i / CL][i % CL] = -INFINITY;
+                }
+            }
+            float m[NS / 4];
+#pragma unroll
+            for (int i = 0; i < NS / 4; ++i) {
+                const fv& x = s[4 * i / CL];
+                const int k = 4 * i % CL;
+                m[i] = __builtin_elementwise_maximum(__builtin_elementwise_maximum(float(x[k]), float(x[k + 1])),
+                                                     __builtin_elementwise_maximum(float(x[k + 2]), float(x[k + 3])));
+            }
+            top = __builtin_elementwise_maximum(m[0], m[1]);
+            if constexpr (NS == 16) top = __builtin_elementwise_maximum(top, __builtin_elementwise_maximum(m[2], m[3]));
+            top *= c;
+            return __builtin_amdgcn_ballot_w64(top > mrun + (LAZY + SHIFT)) != 0;
+        };
+        auto weigh = [&](const fv (&s)[SN], pg_h8 (&ph)[VS], pg_h8 (&pl)[VS]) __attribute__((always_inline)) {
+            float l[NS / 4];
+#pragma unroll
+            for (int i = 0; i < NS; i += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / CL][i % CL], c, -mrun));
+                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / CL][i % CL + 1], c, -mrun));
+                const pg_h2 x = pg_round2(p0, p1);
+                ph[i >> 3][i & 7] = x[0];
+                ph[i >> 3][(i & 7) + 1] = x[1];
+                if constexpr (SPLIT) {
+                    pl[i >> 3][i & 7] = (_Float16)(p0 - (float)x[0]);
+                    pl[i >> 3][(i & 7) + 1] = (_Float16)(p1 - (float)x[1]);
+                }
+                l[i >> 2] = i & 2 ? l[i >> 2] + (p0 + p1) : p0 + p1;
+            }
+            float sum = l[0] + l[1];
+            if constexpr (NS == 16) sum += l[2] + l[3];
+            lsum += sum;
+        };
+        fv sa[SN], sb[SN];
+        pg_h8 pha[VS], pla[VS], phb[VS], plb[VS];
+#pragma unroll
+        for (int t = 0; t < VS; ++t) pha[t] = pla[t] = phb[t] = plb[t] = pg_h8{};
+        scores(sa, 0, 0);
+        bool moves = look(0, sa);
+        // Unit j, the sub-th of stage t, whose buffers are b (bp, bn: those of the stages
+        // before and after): s and (ph0, pl0) in, of this unit and the one before; sn and
+        // (ph1, pl1) out, of the next and this one. A stage's first unit waits for the
+        // stage and fills a later one.
+        auto step = [&](int t, int sub, int bp, int b, int bn, fv (&s)[SN], pg_h8 (&ph0)[VS], pg_h8 (&pl0)[VS],
+                        fv (&sn)[SN], pg_h8 (&ph1)[VS], pg_h8 (&pl1)[VS]) __attribute__((always_inline)) {
+            if (sub == 0) __syncthreads();
+            if (__builtin_expect(moves, 0)) {  // (uniform)
+                // (whole powers of 2: the weights that wait to be added have the old maximum)
+                float tm;
+                if constexpr (W == 32) {
+                    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+                    tm = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+                } else {
+                    tm = pg_rows4_max(top);
+                }
+                tm = __builtin_ceilf(tm) - SHIFT;
+                if (tm > mrun + LAZY) {
+                    const float alpha = __builtin_amdgcn_exp2f(mrun - tm);
+                    mrun = tm;
+                    lsum *= alpha;
+#pragma unroll
+                    for (int t = 0; t < VS; ++t) {
+                        ph0[t] *= (_Float16)alpha;
+                        if constexpr (SPLIT) pl0[t] *= (_Float16)alpha;
+                    }
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) o[n] *= alpha;
+                }
+            }
+            if (sub == 0) {
+                // (U = 2, three buffers: t + 2 is in those of t - 1; U = 1, two: in t's)
+                store(isv ? t + VA : t + 2, isv ? (U == 2 ? bn : b) : (U == 2 ? bp : b));
+                load(isv ? t + VA + 1 : t + 3);
+            }
+            scores(sn, sub == U - 1 ? bn : b, sub == U - 1 ? 0 : sub + 1);
+            weigh(s, ph1, pl1);
+            products(sub == 0 ? bp : b, sub == 0 ? U - 1 : sub - 1, ph0, pl0);
+            moves = look(t * U + sub + 1, sn);
+        };
+        int b = 0, bn = 1, bp = BUFS - 1;
+        auto next = [&] {
+            bp = b;
+            b = bn;
+            bn = bn == BUFS - 1 ? 0 : bn + 1;
+        };
+        if constexpr (U == 2) {
+            for (int t = 0; t < stages; ++t) {
+                step(t, 0, bp, b, bn, sa, pha, pla, sb, phb, plb);
+                step(t, 1, bp, b, bn, sb, phb, plb, sa, pha, pla);
+                next();
+            }
+        } else {
+            // (an odd count: one stage more than there is, its scores masked)
+            for (int t = 0; t < stages; t += 2) {
+                step(t, 0, bp, b, bn, sa, pha, pla, sb, phb, plb);
+                next();
+                step(t + 1, 0, bp, b, bn, sb, phb, plb, sa, pha, pla);
+                next();
+            }
+        }
+        __syncthreads();
+        products(bp, U - 1, pha, pla);
+        wild = dropped != 0;
+    }
+    if constexpr (W == 32) {
+        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(lsum), __float_as_uint(lsum), false, false);
+        lsum = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+    } else {
+        lsum = pg_rows4_sum(lsum);
+    }
+    // Infinities and NaN among the values: the products leave NaN of them (0, or a
+    // negative second fp16, times an infinity). A result that they reach is their sum,
+    // whatever the weights, which are positive. (Lane: dims W n + 8 b + 4 hi..+3.)
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int k = 0; k < CL; ++k) wild |= !(fabsf(o[n][k]) < INFINITY);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(wild) != 0, 0)) {
+#pragma unroll 1
+        for (int n = 0; n < NB; ++n) {
+            fv sum = {};
+#pragma unroll 1
+            for (int key = u_begin * 32; key < min(u_end * 32, seen); ++key) {
+                const __half* vp = B.v + (size_t)pg_tile(B, I.s, g, key) * (16 * D);
+#pragma unroll
+                for (int k = 0; k < CL; ++k) {
+                    const int dim = W * n + 8 * (k >> 2) + 4 * hi + (k & 3);
+                    const float x = __half2float(vp[pg_v_place(D, key & 15, dim >> 3) * 8 + (dim & 7)]);
+                    sum[k] += key < lim && !(fabsf(x) < INFINITY) ? x : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < NB; ++m)
+#pragma unroll
+                for (int k = 0; k < CL; ++k)
+                    if (m == n) o[m][k] = fabsf(sum[k]) < INFINITY ? float(o[m][k]) : float(sum[k]);
+        }
+    }
+    if (!live) return;
+    if (I.splits == 1) {
+        const float il = lim == 0 ? 0.0f : 1.0f / lsum;
+        const long long to = (long long)(g * G + h) * P.o_head + (long long)(I.row + r) * P.o_row + 4 * hi;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int k = 0; k < CL; k += 4)
+                pg_store4(P, to + W * n + 2 * k, o[n][k] * il, o[n][k + 1] * il, o[n][k + 2] * il, o[n][k + 3] * il);
+    } else {
+        const size_t row_at = ((size_t)at * B.kh + g) * ROWS + W * wave + lo;
+        float* p = P.part + row_at * D + 4 * hi;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int k = 0; k < CL; k += 4)
+                *reinterpret_cast<pg_f4*>(p + W * n + 2 * k) = pg_f4{o[n][k], o[n][k + 1], o[n][k + 2], o[n][k + 3]};
+        if (hi == 0)
+            *reinterpret_cast<float2*>(P.part + (size_t)P.items * B.kh * ROWS * D + row_at * 2) = float2{mrun, lsum};
+    }
+}
+
+// The splits' partials of RPB rows of one row tile and KV head: out = sum_s w_s acc_s /
+// sum_s w_s l_s with w_s = 2^(m_s - max m). T = 256 / RPB threads a row, thread t with 4
+// dims of every GS-th split; their first loads do not wait for the weights, which the
+// row's threads find meanwhile; sums over the GS groups meet in LDS.
+template <int D, int RPB>
+__global__ __launch_bounds__(256) void attn_paged_join_kernel(AttnPagedParams P) {
+    constexpr int T = 256 / RPB, LD = D / 4, GS = T / LD, AHEAD = 8, W = PAGED_MAX_SPLITS / T;
+    static_assert(GS >= 1 && T % LD == 0 && T >= 16, "threads per row");
+    __shared__ float weight[RPB][PAGED_MAX_SPLITS];
+    __shared__ float red[RPB][2][T / 64 + 1];
+    __shared__ pg_f4 part[RPB][GS][LD];
+    const PagedBatch& B = P.b;
+    const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const PagedItem I = pg_item(P, blockIdx.y, lane, true);
     // (a block past the grid of the batch's wrong offsets has written nothing)
     if (!I.any || I.splits == 1 || I.item + I.splits > P.items) return;
-    const int G = P.qh / B.kh, row = blockIdx.z, rr = I.tile * P.tile_rows + row;
-    if (rr >= G * I.n) return;
+    const int G = P.qh / B.kh, R = min(G * I.n - I.tile * P.tile_rows, P.tile_rows), row0 = blockIdx.z * RPB;
+    if (row0 >= R) return;  // (block-uniform)
+    const int mine = tid / T, t = tid % T, d4 = t % LD, gs = t / LD, S = I.splits;
+    const int row = min(row0 + mine, R - 1);  // (threads past the last row: that row again, not written)
     const size_t step = (size_t)B.kh * P.tile_rows, at = ((size_t)I.item * B.kh + g) * P.tile_rows + row;
+    const pg_f4* acc = reinterpret_cast<const pg_f4*>(P.part + at * D) + d4;
+    pg_f4 v[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) v[i] = acc[(size_t)min(gs + i * GS, S - 1) * step * LD];
     const float2* ml = reinterpret_cast<const float2*>(P.part + (size_t)P.items * step * D) + at;
-    const float2 x = tid < I.splits ? ml[tid * step] : float2{PG_NONE, 0.0f};
-    float top = wave_max(x.x);
-    if (lane == 0) red[0][wave] = top;
+    float2 x[W];
+    float top = PG_NONE;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        x[i] = t + i * T < S ? ml[(size_t)(t + i * T) * step] : float2{PG_NONE, 0.0f};
+        top = fmaxf(top, x[i].x);
+    }
+#pragma unroll
+    for (int i = 1; i < (T < 64 ? T : 64); i <<= 1) top = fmaxf(top, __shfl_xor(top, i));
+    if constexpr (T > 64) {
+        if (lane == 0) red[mine][0][t / 64] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < T / 64; ++i) top = fmaxf(top, red[mine][0][i]);
+    }
+    float den = 0.0f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        const float w = pg_weight(x[i].x, top);
+        if (t + i * T < S) weight[mine][t + i * T] = w;
+        // (a split that saw NaN scores has a NaN sum)
+        den += x[i].y != x[i].y ? x[i].y : w * x[i].y;
+    }
+#pragma unroll
+    for (int i = 1; i < (T < 64 ? T : 64); i <<= 1) den += __shfl_xor(den, i);
+    if (T > 64 && lane == 0) red[mine][1][t / 64] = den;
     __syncthreads();
-    top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    const float w = pg_weight(x.x, top);
-    weight[tid] = w;
-    // (a split that saw NaN scores has a NaN sum)
-    float den = x.y != x.y ? x.y : w * x.y;
+    if constexpr (T > 64) {
+        den = 0.0f;
 #pragma unroll
-    for (int i = 1; i < 64; i <<= 1) den += __shfl_xor(den, i);
-    if (lane == 0) red[1][wave] = den;
-    __syncthreads();
-    const int d = tid % LD * 8, gs = tid / LD;
-    float y[8];
+        for (int i = 0; i < T / 64; ++i) den += red[mine][1][i];
+    }
+    pg_f4 num = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = gs; s < S; s += AHEAD * GS) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) y[k] = 0.0f;
-    for (int s = gs; s < I.splits; s += GS) {
-        const float* p = P.part + (at + s * step) * D + d;
-        const pg_f4 x0 = *reinterpret_cast<const pg_f4*>(p), x1 = *reinterpret_cast<const pg_f4*>(p + 4);
-        const float b = weight[s];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            y[k] += x0[k] * b;
-            y[4 + k] += x1[k] * b;
+        for (int i = 0; i < AHEAD; ++i) {
+            if (s + i * GS < S) num += v[i] * weight[mine][s + i * GS];
+            v[i] = acc[(size_t)min(s + (AHEAD + i) * GS, S - 1) * step * LD];
         }
     }
-    *reinterpret_cast<pg_f4*>(&part[gs][d]) = pg_f4{y[0], y[1], y[2], y[3]};
-    *reinterpret_cast<pg_f4*>(&part[gs][d + 4]) = pg_f4{y[4], y[5], y[6], y[7]};
-    __syncthreads();
-    if (gs) return;
-    for (int i = 1; i < min(GS, I.splits); ++i)
+    if constexpr (GS > 1) {
+        part[mine][gs][d4] = num;
+        __syncthreads();
+        if (gs) return;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) y[k] += part[i][d + k];
-    den = red[1][0] + red[1][1] + red[1][2] + red[1][3];
-    const int r = rr / G, h = rr - r * G;
+        for (int i = 1; i < GS; ++i) num += part[mine][i][d4];
+    }
+    if (row0 + mine >= R) return;
+    const int rr = I.tile * P.tile_rows + row, r = rr / G, h = rr - r * G;
     const bool empty = P.causal ? I.len - I.n + r + 1 <= 0 : I.len == 0;
-    const float il = empty ? 0.0f : 1.0f / den;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) y[k] *= il;
-    pg_store8(P, (long long)(g * G + h) * P.o_head + (long long)(I.row + r) * P.o_row + d, y);
+    num *= empty ? 0.0f : 1.0f / den;
+    pg_store4(P, (long long)(g * G + h) * P.o_head + (long long)(I.row + r) * P.o_row + 4 * d4, num[0], num[1], num[2], num[3]);
+}
+
+// The kernel of a run: attn_paged_tile_kernel in stages of `units` units, or
+// attn_paged_rows_kernel with loads that leave nothing in the caches (`once`).
+struct PagedPlan {
+    bool tile;
+    int units;
+    bool once;
+};
+
+void launch_attn_paged_64(const AttnPagedParams& P, const PagedPlan& plan, hipStream_t s);
+void launch_attn_paged_128(const AttnPagedParams& P, const PagedPlan& plan, hipStream_t s);
+void launch_attn_paged_256(const AttnPagedParams& P, const PagedPlan& plan, hipStream_t s);
+
+template <int D, int U>
+static void launch_attn_paged_tile(const AttnPagedParams& P, hipStream_t s) {
+    constexpr int W = D == 256 ? 16 : 32, NW = 128 * U / W;
+    const dim3 grid(P.b.kh * P.items), block(64 * NW);
+    if (P.out_f16)
+        hipLaunchKernelGGL((attn_paged_tile_kernel<D, W, U, NW, false>), grid, block, 0, s, P);
+    else
+        hipLaunchKernelGGL((attn_paged_tile_kernel<D, W, U, NW, true>), grid, block, 0, s, P);
+}
+
+template <int D, bool ONCE>
+static void launch_attn_paged_rows(const AttnPagedParams& P, hipStream_t s) {
+    const dim3 grid(P.b.kh * P.items);
+    if (P.tile_rows == 8)
+        hipLaunchKernelGGL((attn_paged_rows_kernel<D, 4, true, ONCE>), grid, dim3(256), 0, s, P);
+    else
+        hipLaunchKernelGGL((attn_paged_rows_kernel<D, 4, false, ONCE>), grid, dim3(256), 0, s, P);
+}
+
+template <int D>
+static void launch_attn_paged(const AttnPagedParams& P, const PagedPlan& plan, hipStream_t s) {
+    if (plan.tile) {
+        if (D < 256 && plan.units == 2)
+            launch_attn_paged_tile<D, D < 256 ? 2 : 1>(P, s);
+        else
+            launch_attn_paged_tile<D, 1>(P, s);
+    } else if (plan.once) {
+        launch_attn_paged_rows<D, true>(P, s);
+    } else {
+        launch_attn_paged_rows<D, false>(P, s);
+    }
+    if (P.target) {
+        // (many rows: as many a block as leave a row the threads for its dims)
+        constexpr int MANY = 1024 / D < 8 ? 1024 / D : 8;
+        if (P.tiles * P.tile_rows * P.b.kh >= 1024)
+            hipLaunchKernelGGL((attn_paged_join_kernel<D, MANY>), dim3(P.b.kh, P.tiles, P.tile_rows / MANY), dim3(256), 0, s, P);
+        else
+            hipLaunchKernelGGL((attn_paged_join_kernel<D, 1>), dim3(P.b.kh, P.tiles, P.tile_rows), dim3(256), 0, s, P);
+    }
 }
 
 }  // namespace hm

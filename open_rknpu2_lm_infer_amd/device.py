@@ -300,7 +300,7 @@ class PagedBatch:
 
     def _raw(self, rows: int, page: int) -> F.rk_npu_hip_paged_batch:
         most = self.table.shape[1] * page
-        tokens = min(most, 2 ** 31 - 1) if self.max_tokens is None else self.max_tokens
+        tokens = min(most, F.RK_NPU_HIP_PAGED_MAX_TOKENS) if self.max_tokens is None else self.max_tokens
         if tokens > most:
             raise NpuError(f"the table holds {most} tokens a sequence, max_tokens is {tokens}")
         lengths, offsets, table = self._at
@@ -322,7 +322,7 @@ class KvPages:
     def __init__(self, ctx: DeviceContext, query_heads: int, kv_heads: int, head_dim: int, softmax_scale: float,
                  pages: int, page: int = 64, capacity: Optional[int] = None, causal: bool = True, rotary_dim: int = 0,
                  rope_theta: float = 10000.0, interleaved: bool = False, frequencies=None):
-        capacity = min(pages * page, 2 ** 31 - 256) if capacity is None else capacity
+        capacity = min(pages * page, F.RK_NPU_HIP_PAGED_MAX_TOKENS) if capacity is None else capacity
         for name, value in (("query_heads", query_heads), ("kv_heads", kv_heads), ("head_dim", head_dim),
                             ("pages", pages), ("page", page), ("capacity", capacity), ("rotary_dim", rotary_dim)):
             int32(value, name)

@@ -61,7 +61,7 @@ def test_refused_configurations():
         cfg.frequencies = (ctypes.c_double * 8)(*([1.0] * 7 + [value]))
         assert query(cfg)[0] == F.RK_NPU_ERR_PARAM
     cfg = config()
-    cfg.attention.max_capacity = 2 ** 31 - 100
+    cfg.attention.max_capacity = 2 ** 30 + 1
     assert query(cfg)[0] == F.RK_NPU_ERR_PARAM
     assert F.lib().rk_npu_hip_attention_paged_query(ctypes.byref(config()), None) == F.RK_NPU_ERR_PARAM
     assert F.lib().rk_npu_hip_attention_paged_query(None, ctypes.byref(F.rk_npu_attention_f16_sizes())) == F.RK_NPU_ERR_PARAM

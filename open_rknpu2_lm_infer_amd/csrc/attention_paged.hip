@@ -58,148 +58,144 @@ __device__ __forceinline__ void pg_put8(const HeadsView& a, long long at, const 
 
 struct PagedRowsParams {
     PagedBatch b;
-    HeadsView k, v, q, q_out;   // (data nullptr: none)
+    HeadsView k, v, q, q_out;  // (data nullptr: none)
     const int* positions;
-    const double* turns;        // frequencies in turns (radians / 2 pi) per position
-    int D, qh, rotary, interleaved;
-    int rows_per_block, heads_per_block;
+    const double* turns;       // frequencies in turns (radians / 2 pi) per position
+    int D, qh, rotary, interleaved, heads_per_block;
 };
 
-// The sequences and tokens of a block's rows row0..row0 + n - 1, by all its threads:
-// seq[i] and token[i] (-1: no token), dest[i] (the row's place in the pool in tokens of
-// a head, page * kh * page + place; -1: none).
-template <int RB>
-__device__ __forceinline__ void pg_block_rows(const PagedBatch& B, int row0, int n, int (&seq)[RB], int (&token)[RB],
-                                              int (&page)[RB]) {
-    const int tid = threadIdx.x;
-    if (tid < RB) {
-        seq[tid] = B.offsets ? -1 : row0 + tid < B.sequences ? row0 + tid : -1;
-        token[tid] = -1;
-        page[tid] = -1;
-    }
-    __syncthreads();
+// A row's token (-1: none) and page (-1: none), the same for all of a block's threads.
+struct PagedRow {
+    int token, page;
+};
+__device__ __forceinline__ PagedRow pg_row(const PagedBatch& B, int row, int* found) {
+    int s = row < B.sequences ? row : -1;
     if (B.offsets) {
-        for (int s = tid; s < B.sequences; s += blockDim.x) {
-            const int a = B.offsets[s], b = B.offsets[s + 1];
-            if (a < 0 || b < a || b > B.rows || b - a > B.max_rows) {
+        if (threadIdx.x == 0) *found = -1;
+        __syncthreads();
+        for (int i = threadIdx.x; i < B.sequences; i += 256) {
+            const int a = B.offsets[i], b = B.offsets[i + 1];
+            if (a < 0 || b < a || b > B.rows || b - a > B.max_rows)
                 pg_flaw(B);
-                continue;
-            }
-            for (int r = max(a, row0); r < min(b, row0 + n); ++r) seq[r - row0] = s;
+            else if (a <= row && row < b)
+                *found = i;  // (of overlapping offsets: one of them)
         }
         __syncthreads();
+        s = __builtin_amdgcn_readfirstlane(*found);
     }
-    if (tid < n && seq[tid] >= 0) {
-        const int s = seq[tid];
-        const PagedSeq q = pg_seq(B, s);
-        const int t = q.len - q.n + (row0 + tid - q.row);
-        // (another thread may have found the row in a sequence of overlapping offsets)
-        if (q.n > 0 && t >= 0 && t < q.len) {
-            token[tid] = t;
-            page[tid] = pg_page(B, s, t);
-        }
-    }
-    __syncthreads();
+    PagedRow x{-1, -1};
+    if (s < 0) return x;
+    const PagedSeq q = pg_seq(B, s);
+    const int t = q.len - q.n + (row - q.row);
+    if (t < 0 || t >= q.len) return x;
+    x.token = t;
+    x.page = pg_page(B, s, t);
+    return x;
+}
+// Where a row's piece of 8 dims lies in its page.
+__device__ __forceinline__ size_t pg_at(const PagedBatch& B, int D, const PagedRow& x, int g, bool v, int piece) {
+    const int place = x.token & ((1 << B.page_shift) - 1), j = place & 15;
+    return ((((size_t)x.page * B.kh + g) << B.page_shift) + (place & ~15)) * D +
+           (size_t)(v ? pg_v_place(D, j, piece) : pg_k_place(D, j, piece)) * 8;
 }
 
-// Append. Block: `rows_per_block` rows of `heads_per_block` of the heads, counted q
-// heads, K heads, V heads. A thread takes 16 values of a row at a time, the two pieces
-// of 8 dims that turn into each other.
-template <int RB>
+constexpr int PAGED_APPEND_UNITS = 2;  // 16-value units of a thread
+
+// Append. Block: one row of some of the heads, counted q heads, K heads, V heads. A
+// thread takes two units of 16 values of a row, each the two pieces of 8 dims that turn
+// into each other (or neighbours); their loads come first, as the row's place, three
+// loads that wait for one another, has nothing to do with them. The angle's 64-bit
+// product and its reduction cost one multiplication and one rounding a pair; sine and
+// cosine of a row are computed once, into LDS.
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedRowsParams P) {
-    __shared__ int seq[RB], token[RB], page[RB];
-    __shared__ float2 turn[RB * 128];
+    __shared__ float2 turn[128];
+    __shared__ int found;
     const PagedBatch& B = P.b;
-    const int tid = threadIdx.x, row0 = blockIdx.x * RB, n = min(RB, B.rows - row0);
-    pg_block_rows<RB>(B, row0, n, seq, token, page);
+    const int tid = threadIdx.x, row = blockIdx.x, qh = P.qh;
+    const int per_head = P.D >> 4, h0 = blockIdx.y * P.heads_per_block, hn = min(P.heads_per_block, qh + 2 * B.kh - h0);
+    const int turned_units = P.rotary >> 4;
+    float x[PAGED_APPEND_UNITS][8], y[PAGED_APPEND_UNITS][8];
+    int kind[PAGED_APPEND_UNITS], g[PAGED_APPEND_UNITS], a[PAGED_APPEND_UNITS], b[PAGED_APPEND_UNITS];
+#pragma unroll
+    for (int n = 0; n < PAGED_APPEND_UNITS; ++n) {
+        const int i = n * 256 + tid, unit = i % per_head, h = h0 + i / per_head;
+        kind[n] = i >= hn * per_head ? -1 : h < qh ? 0 : h < qh + B.kh ? 1 : 2;
+        if (kind[n] < 0) continue;
+        g[n] = kind[n] == 0 ? h : h - qh - (kind[n] - 1) * B.kh;
+        // (units from turned_units on: the dims that stay)
+        const bool halves = unit < turned_units && !P.interleaved;
+        a[n] = halves ? unit : 2 * unit;
+        b[n] = halves ? unit + turned_units : 2 * unit + 1;
+        const HeadsView& src = kind[n] == 0 ? P.q : kind[n] == 1 ? P.k : P.v;
+        const long long at = (long long)g[n] * src.head + (long long)row * src.row;
+        pg_get8(src, at + 8 * a[n], x[n]);
+        pg_get8(src, at + 8 * b[n], y[n]);
+    }
+    const PagedRow R = pg_row(B, row, &found);
+    if (R.token < 0) return;  // (block-uniform)
     const int pairs = P.rotary >> 1;
-    for (int i = tid; i < n * pairs; i += 256) {
-        const int r = i / pairs, j = i - r * pairs;
-        if (token[r] < 0) continue;
-        const double at = (double)(P.positions ? P.positions[row0 + r] : token[r]) * P.turns[j];
+    if (tid < pairs) {
+        const double at = (double)(P.positions ? P.positions[row] : R.token) * P.turns[tid];
         float s, c;
         sincospif(2.0f * (float)(at - __builtin_rint(at)), &s, &c);
-        turn[i] = float2{c, s};
+        turn[tid] = float2{c, s};
     }
     __syncthreads();
-    const int per_head = P.D >> 4, heads = P.qh + 2 * B.kh, qh = P.qh;
-    const int h0 = blockIdx.y * P.heads_per_block, hn = min(P.heads_per_block, heads - h0);
-    const int page_mask = (1 << B.page_shift) - 1;
-    for (int i = tid; i < n * hn * per_head; i += 256) {
-        const int unit = i % per_head, h = h0 + i / per_head % hn, r = i / per_head / hn;
-        if (token[r] < 0) continue;
-        const int kind = h < qh ? 0 : h < qh + B.kh ? 1 : 2, g = kind == 0 ? h : h - qh - (kind - 1) * B.kh;
-        const HeadsView& src = kind == 0 ? P.q : kind == 1 ? P.k : P.v;
-        if (!src.data) continue;
-        const bool turned = unit < P.rotary >> 4 && kind != 2;
-        // pieces of 8 dims: a pair's two, or neighbours
-        const int rest = unit - (P.rotary >> 4);
-        const int a = turned && !P.interleaved ? unit : unit < P.rotary >> 4 ? 2 * unit : (P.rotary >> 3) + 2 * rest;
-        const int b = turned && !P.interleaved ? unit + (P.rotary >> 4) : a + 1;
-        const long long at = (long long)g * src.head + (long long)(row0 + r) * src.row;
-        float x[8], y[8];
-        pg_get8(src, at + 8 * a, x);
-        pg_get8(src, at + 8 * b, y);
-        if (turned) {
-            const float2* t = turn + r * pairs + 8 * unit;
+#pragma unroll
+    for (int n = 0; n < PAGED_APPEND_UNITS; ++n) {
+        if (kind[n] < 0) continue;
+        const int unit = (n * 256 + tid) % per_head;
+        if (unit < turned_units && kind[n] != 2) {
+            const float2* t = turn + 8 * unit;
             if (!P.interleaved) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    const float u = x[k], v = y[k];
-                    x[k] = u * t[k].x - v * t[k].y;
-                    y[k] = v * t[k].x + u * t[k].y;
+                    const float u = x[n][k], v = y[n][k];
+                    x[n][k] = u * t[k].x - v * t[k].y;
+                    y[n][k] = v * t[k].x + u * t[k].y;
                 }
             } else {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const float u = x[2 * k], v = x[2 * k + 1], w = y[2 * k], z = y[2 * k + 1];
-                    x[2 * k] = u * t[k].x - v * t[k].y;
-                    x[2 * k + 1] = v * t[k].x + u * t[k].y;
-                    y[2 * k] = w * t[4 + k].x - z * t[4 + k].y;
-                    y[2 * k + 1] = z * t[4 + k].x + w * t[4 + k].y;
+                    const float u = x[n][2 * k], v = x[n][2 * k + 1], w = y[n][2 * k], z = y[n][2 * k + 1];
+                    x[n][2 * k] = u * t[k].x - v * t[k].y;
+                    x[n][2 * k + 1] = v * t[k].x + u * t[k].y;
+                    y[n][2 * k] = w * t[4 + k].x - z * t[4 + k].y;
+                    y[n][2 * k + 1] = z * t[4 + k].x + w * t[4 + k].y;
                 }
             }
         }
-        if (kind == 0) {
-            const long long to = (long long)g * P.q_out.head + (long long)(row0 + r) * P.q_out.row;
-            pg_put8(P.q_out, to + 8 * a, x);
-            pg_put8(P.q_out, to + 8 * b, y);
-        } else if (page[r] >= 0) {
-            const int place = token[r] & page_mask, j = place & 15;
-            __half* to = (kind == 1 ? B.k : B.v) +
-                         (((size_t)page[r] * B.kh + g) << B.page_shift) * P.D + (size_t)(place & ~15) * P.D;
-            const int pa = kind == 1 ? pg_k_place(P.D, j, a) : pg_v_place(P.D, j, a);
-            const int pb = kind == 1 ? pg_k_place(P.D, j, b) : pg_v_place(P.D, j, b);
-            *reinterpret_cast<v4u*>(to + pa * 8) = pg_halves(x);
-            *reinterpret_cast<v4u*>(to + pb * 8) = pg_halves(y);
+        if (kind[n] == 0) {
+            const long long to = (long long)g[n] * P.q_out.head + (long long)row * P.q_out.row;
+            pg_put8(P.q_out, to + 8 * a[n], x[n]);
+            pg_put8(P.q_out, to + 8 * b[n], y[n]);
+        } else if (R.page >= 0) {
+            __half* to = kind[n] == 1 ? B.k : B.v;
+            *reinterpret_cast<v4u*>(to + pg_at(B, P.D, R, g[n], kind[n] == 2, a[n])) = pg_halves(x[n]);
+            *reinterpret_cast<v4u*>(to + pg_at(B, P.D, R, g[n], kind[n] == 2, b[n])) = pg_halves(y[n]);
         }
     }
 }
 
-// Read. Block: as the append's, over K heads then V heads; a thread takes a piece of 8
-// dims at a time.
-template <int RB>
+// Read. Block: one row, its K heads, then its V heads; a thread takes a piece of 8 dims
+// at a time.
 __global__ __launch_bounds__(256) void paged_read_kernel(PagedRowsParams P) {
-    __shared__ int seq[RB], token[RB], page[RB];
+    __shared__ int found;
     const PagedBatch& B = P.b;
-    const int tid = threadIdx.x, row0 = blockIdx.x * RB, n = min(RB, B.rows - row0);
-    pg_block_rows<RB>(B, row0, n, seq, token, page);
-    const int per_head = P.D >> 3, h0 = blockIdx.y * P.heads_per_block, hn = min(P.heads_per_block, 2 * B.kh - h0);
-    const int page_mask = (1 << B.page_shift) - 1;
-    for (int i = tid; i < n * hn * per_head; i += 256) {
-        const int piece = i % per_head, h = h0 + i / per_head % hn, r = i / per_head / hn;
-        const int which = h < B.kh ? 0 : 1, g = h - which * B.kh;
-        const HeadsView& dst = which ? P.v : P.k;
-        if (page[r] < 0 || !dst.data) continue;
-        const int place = token[r] & page_mask, j = place & 15;
-        const __half* from = (which ? B.v : B.k) + (((size_t)page[r] * B.kh + g) << B.page_shift) * P.D +
-                             (size_t)(place & ~15) * P.D;
-        const pg_h8 u = __builtin_bit_cast(
-            pg_h8, *reinterpret_cast<const v4u*>(from + (which ? pg_v_place(P.D, j, piece) : pg_k_place(P.D, j, piece)) * 8));
+    const int row = blockIdx.x, per_head = P.D >> 3;
+    const PagedRow R = pg_row(B, row, &found);
+    if (R.page < 0) return;  // (block-uniform)
+    for (int i = threadIdx.x; i < 2 * B.kh * per_head; i += 256) {
+        const int piece = i % per_head, h = i / per_head;
+        const bool v = h >= B.kh;
+        const int g = v ? h - B.kh : h;
+        const HeadsView& dst = v ? P.v : P.k;
+        if (!dst.data) continue;
+        const pg_h8 u = __builtin_bit_cast(pg_h8, *reinterpret_cast<const v4u*>((v ? B.v : B.k) + pg_at(B, P.D, R, g, v, piece)));
         float x[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[k] = (float)u[k];
-        pg_put8(dst, (long long)g * dst.head + (long long)(row0 + r) * dst.row + 8 * piece, x);
+        pg_put8(dst, (long long)g * dst.head + (long long)row * dst.row + 8 * piece, x);
     }
 }
 
@@ -444,9 +440,8 @@ int rk_npu_hip_attention_paged_append(rk_npu_hip_attention_paged_pool* pool, con
     P.positions = positions;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int heads = P.qh + 2 * kh;
-    P.rows_per_block = 1;
-    P.heads_per_block = heads;
-    hipLaunchKernelGGL(paged_append_kernel<1>, dim3(rows, 1), dim3(256), 0, s, P);
+    P.heads_per_block = 256 * PAGED_APPEND_UNITS / (D / 16);
+    hipLaunchKernelGGL(paged_append_kernel, dim3(rows, (heads + P.heads_per_block - 1) / P.heads_per_block), dim3(256), 0, s, P);
     if (hipGetLastError() != hipSuccess) return RK_NPU_ERR_DEVICE;
     c->fence.note(s);
     return RK_NPU_OK;
@@ -465,9 +460,7 @@ int rk_npu_hip_attention_paged_read(rk_npu_hip_attention_paged_pool* pool, const
     if (k) P.k = view_of(*k);
     if (v) P.v = view_of(*v);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    P.rows_per_block = 1;
-    P.heads_per_block = 2 * kh;
-    hipLaunchKernelGGL(paged_read_kernel<1>, dim3(batch->rows, 1), dim3(256), 0, s, P);
+    hipLaunchKernelGGL(paged_read_kernel, dim3(batch->rows), dim3(256), 0, s, P);
     if (hipGetLastError() != hipSuccess) return RK_NPU_ERR_DEVICE;
     c->fence.note(s);
     return RK_NPU_OK;

@@ -251,8 +251,10 @@ def _heads(t, heads: int, head_dim: int) -> F.rk_npu_hip_heads:
     shape, stride = t.shape, t.stride()
     if not (len(shape) == 3 and shape[0] == heads and shape[2] == head_dim and stride[2] == 1 and t.is_cuda):
         raise NpuError(f"attention arrays are cuda [{heads}][rows][{head_dim}] tensors with contiguous rows")
-    int32(shape[1], "rows")
-    return F.rk_npu_hip_heads(t.data_ptr(), _dtype_code(t), stride[0], stride[1])
+    if shape[1] >= 2 ** 31:
+        int32(shape[1], "rows")
+    code = _DT.get(t.dtype)
+    return F.rk_npu_hip_heads(t.data_ptr(), _dtype_code(t) if code is None else code, stride[0], stride[1])
 
 
 def attention_q8(ctx: DeviceContext, cache: KvCacheQ8, q, out, position: int, ws=None, stream=None):
@@ -294,18 +296,20 @@ class PagedBatch:
             int32(max_tokens, "max_tokens")
         self._stride = int32(table.shape[1] if n <= 1 else table.stride(0), "the table's stride")
         ensure(n <= 1 or self._stride >= table.shape[1], "the table's rows overlap")
+        self._columns = table.shape[1]
         self._at = (_ints(lengths, "lengths", (n,)),
                     None if row_offsets is None else _ints(row_offsets, "row_offsets", (n + 1,)),
-                    _ints(table, "table", (n, table.shape[1])))
+                    _ints(table, "table", (n, self._columns)), self._stride)
 
     def _raw(self, rows: int, page: int) -> F.rk_npu_hip_paged_batch:
-        most = self.table.shape[1] * page
-        tokens = min(most, F.RK_NPU_HIP_PAGED_MAX_TOKENS) if self.max_tokens is None else self.max_tokens
-        if tokens > most:
+        most, tokens = self._columns * page, self.max_tokens
+        if tokens is None:
+            tokens = min(most, F.RK_NPU_HIP_PAGED_MAX_TOKENS)
+        elif tokens > most:
             raise NpuError(f"the table holds {most} tokens a sequence, max_tokens is {tokens}")
-        lengths, offsets, table = self._at
-        return F.rk_npu_hip_paged_batch(self.sequences, int32(rows, "rows"), self.max_rows, tokens, lengths, offsets,
-                                        table, self._stride)
+        if rows >= 2 ** 31:
+            int32(rows, "rows")
+        return F.rk_npu_hip_paged_batch(self.sequences, rows, self.max_rows, tokens, *self._at)
 
 
 class KvPages:
@@ -359,26 +363,31 @@ class KvPages:
         """Puts the batch's rows k and v, [kv_heads][rows][head_dim], into their pages, k
         rotated, and the query rows q, rotated, into q_out (q itself, or another array).
         positions: cuda int32 [rows], by default the rows' tokens."""
-        rows = k.shape[1]
-        ensure(k.shape == v.shape, "k and v must have the same shape")
+        shape = k.shape
+        rows = shape[1] if len(shape) == 3 else 0
+        if shape != v.shape:
+            raise NpuError("k and v must have the same shape")
         kh, vh = _heads(k, *self._kv), _heads(v, *self._kv)
-        ensure((q is None) == (q_out is None), "q and q_out come together")
-        qh = oh = None
+        if (q is None) != (q_out is None):
+            raise NpuError("q and q_out come together")
+        qh = oh = at = None
         if q is not None:
-            ensure(q.shape == q_out.shape and q.shape[1] == rows, "q, q_out and k must have the same rows")
-            qh, oh = ctypes.byref(_heads(q, *self._query)), ctypes.byref(_heads(q_out, *self._query))
-        at = None if positions is None else _ints(positions, "positions", (rows,))
-        check(F.lib().rk_npu_hip_attention_paged_append(self.handle.raw, ctypes.byref(batch._raw(rows, self.page)),
-                                                        ctypes.byref(kh), ctypes.byref(vh), at, qh, oh,
+            qh, oh = _heads(q, *self._query), _heads(q_out, *self._query)
+            if q.shape[1] != rows or q_out.shape[1] != rows:
+                raise NpuError("q, q_out and k must have the same rows")
+        if positions is not None:
+            at = _ints(positions, "positions", (rows,))
+        check(F.lib().rk_npu_hip_attention_paged_append(self.handle.raw, batch._raw(rows, self.page), kh, vh, at, qh, oh,
                                                         _stream(stream, k)), "append to the KV pages")
 
     def read(self, batch: PagedBatch, k, v, stream=None) -> None:
         """The batch's rows as the pages hold them, into k and v, [kv_heads][rows][head_dim]."""
-        ensure(k.shape == v.shape, "k and v must have the same shape")
+        shape = k.shape
+        if shape != v.shape:
+            raise NpuError("k and v must have the same shape")
         kh, vh = _heads(k, *self._kv), _heads(v, *self._kv)
-        check(F.lib().rk_npu_hip_attention_paged_read(self.handle.raw, ctypes.byref(batch._raw(k.shape[1], self.page)),
-                                                      ctypes.byref(kh), ctypes.byref(vh), _stream(stream, k)),
-              "read the KV pages")
+        check(F.lib().rk_npu_hip_attention_paged_read(self.handle.raw, batch._raw(shape[1], self.page), kh, vh,
+                                                      _stream(stream, k)), "read the KV pages")
 
 
 def attention_paged(ctx: DeviceContext, pages: KvPages, batch: PagedBatch, q, out, ws=None, stream=None):
@@ -386,12 +395,12 @@ def attention_paged(ctx: DeviceContext, pages: KvPages, batch: PagedBatch, q, ou
     sequences' pages. ws: the context's workspace of this geometry, which calls on
     one stream share."""
     shape = q.shape
-    ensure(shape == out.shape, "q and out must have the same shape")
+    if shape != out.shape:
+        raise NpuError("q and out must have the same shape")
     ws = ws or ctx.attention_workspace(pages)
     qh, oh = _heads(q, *pages._query), _heads(out, *pages._query)
-    check(F.lib().rk_npu_hip_attention_paged_run(ws.raw, pages.handle.raw, ctypes.byref(batch._raw(shape[1], pages.page)),
-                                                 ctypes.byref(qh), ctypes.byref(oh), _stream(stream, q)),
-          "attention over the KV pages")
+    check(F.lib().rk_npu_hip_attention_paged_run(ws.raw, pages.handle.raw, batch._raw(shape[1], pages.page), qh, oh,
+                                                 _stream(stream, q)), "attention over the KV pages")
 
 
 @contextlib.contextmanager

@@ -290,7 +290,7 @@ static bool paged_same_geometry(const AttnWork* w, const PagedPool* c) {
 }
 
 // Which kernel, its row tiles, and the blocks that splits aim at.
-static PagedPlan paged_plan(AttnPagedParams& P, int D, int64_t pool_bytes) {
+static PagedPlan paged_plan(AttnPagedParams& P, int D) {
     const PagedBatch& B = P.b;
     const int G = P.qh / B.kh, cus = device_cus();
     const int64_t R = (int64_t)B.max_rows * G;
@@ -299,14 +299,8 @@ static PagedPlan paged_plan(AttnPagedParams& P, int D, int64_t pool_bytes) {
         return std::min<int64_t>(B.sequences * ((R + rows - 1) / rows), (int64_t)B.rows * G / rows + B.sequences);
     };
     const int units = (B.max_tokens + 31) / 32;
-    PagedPlan plan{R > 32, D < 256 && units > 128 ? 2 : 1, false};
-    if (plan.tile) {
-        P.tile_rows = 128 * plan.units;
-    } else {
-        P.tile_rows = R <= 8 ? 8 : 16;
-        const int64_t bytes = std::min<int64_t>(pool_bytes, 4LL * B.sequences * B.max_tokens * B.kh * D);
-        plan.once = R <= P.tile_rows && bytes > (512 << 20);
-    }
+    const PagedPlan plan{R > (D == 256 ? 16 : 32), D < 256 && units > 128 ? 2 : 1};
+    P.tile_rows = plan.tile ? 128 * plan.units : R <= 8 ? 8 : R <= 16 ? 16 : 32;
     P.tiles = (int)tiles(P.tile_rows);
     P.least = 8;
     P.target = 0;
@@ -494,7 +488,7 @@ int rk_npu_hip_attention_paged_run(rk_npu_attention_f16_workspace* workspace, rk
     P.qh = cfg.query_heads;
     P.causal = cfg.mask_mode == RK_NPU_ATTENTION_F16_CAUSAL ? 1 : 0;
     P.scale = cfg.softmax_scale;
-    const PagedPlan plan = paged_plan(P, D, 2 * (int64_t)c->kv_bytes);
+    const PagedPlan plan = paged_plan(P, D);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (D == 64)
         launch_attn_paged_64(P, plan, s);

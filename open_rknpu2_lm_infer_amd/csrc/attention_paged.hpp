@@ -139,12 +139,27 @@ __device__ __forceinline__ PagedItem pg_item(const AttnPagedParams& P, int at, i
     const int G = P.qh / B.kh, C = (B.sequences + 63) >> 6;
     auto tiles_of = [&](const PagedSeq& q) { return (int)(((unsigned)q.n * (unsigned)G + P.tile_rows - 1) / (unsigned)P.tile_rows); };
     const PagedSeq none{0, 0, 0};
+    if (!P.target && !B.offsets && G <= P.tile_rows) {
+        // (one row each, not split: block `at` has sequence `at`)
+        PagedItem x{};
+        x.s = at;
+        x.any = at < B.sequences;
+        if (!x.any) return x;
+        const PagedSeq q = pg_seq(B, at);
+        x.row = q.row;
+        x.n = q.n;
+        x.len = q.len;
+        x.splits = 1;
+        x.item = at;
+        return x;
+    }
     PagedSeq mine = lane * C < B.sequences ? pg_seq(B, lane * C) : none;
     // (one sequence a lane: the one in registers)
     auto seq = [&](int i) { return C == 1 ? mine : lane * C + i < B.sequences ? pg_seq(B, lane * C + i) : none; };
     unsigned per = 0x7fffffff;
     if (P.target > 0) {
         int units = 0;
+#pragma unroll 4
         for (int i = 0; i < C; ++i) {
             const PagedSeq q = seq(i);
             units += tiles_of(q) * ((q.len + 31) >> 5);
@@ -157,6 +172,7 @@ __device__ __forceinline__ PagedItem pg_item(const AttnPagedParams& P, int at, i
         return P.target > 0 ? min(PAGED_MAX_SPLITS, max(1, (int)((units + per - 1) / per))) : 1;
     };
     int items = 0, tiles = 0;
+#pragma unroll 4
     for (int i = 0; i < C; ++i) {
         const PagedSeq q = seq(i);
         const int t = tiles_of(q);
@@ -294,42 +310,50 @@ __device__ __forceinline__ pg_h8 pg_load_q(const AttnPagedParams& P, long long a
 // fp16 of a weight, of 2^-11 of the first, keeps its bits down to weights of 2^-13.
 constexpr float PG_LAZY = 4.0f, PG_SHIFT = 10.0f;
 
-// Few rows. Block: NW waves over one tile of 16 query rows (8 where PACK) of one KV
-// head of a sequence; wave w takes units w, w + NW, .. of 32 keys of its split, so
-// nothing is shared until the waves' partial (max, sum, accumulators) meet in LDS.
-// K comes from memory in operand order; V comes as rows, 8 keys of 8 dims a lane, and
-// is transposed there, two keys' halves a v_perm_b32. Weights go into the products
+// Few rows. Block: NW waves over one tile of RW groups of 16 query rows (one of 8 where
+// PACK) of one KV head of a sequence; wave w takes units w, w + NW, .. of 32 keys of its
+// split, so nothing is shared until the waves' partial (max, sum, accumulators) meet in
+// LDS. K comes from memory in operand order; V comes as rows, 8 keys of 8 dims a lane,
+// and is transposed there, two keys' halves a v_perm_b32. Weights go into the products
 // with V as two fp16. PACK: columns 8..15 are columns 0..7 again and take the second
-// fp16, so that both cost one product.
-template <int D, int NW, bool PACK, bool ONCE>
+// fp16, so that both cost one product. A tile holds all rows of a sequence, so pages
+// are read once, by loads that leave nothing in the caches.
+template <int D, int NW, int RW, bool PACK>
 __global__ __launch_bounds__(64 * NW) void attn_paged_rows_kernel(AttnPagedParams P) {
     constexpr int KS = D / 32;                  // 32-dim steps of a score
     constexpr int DW = D == 64 ? 4 : 8;         // dims of V a lane takes of a key, H times
     constexpr int H = D / (16 * DW), NB = H * DW;
-    constexpr int COLS = PACK ? 8 : 16, PITCH = D + 4;
+    constexpr int COLS = PACK ? 8 : 16 * RW, PITCH = D + 4;
+    static_assert(RW == 1 || !PACK, "packed columns");
+    typedef unsigned u2 __attribute__((ext_vector_type(2)));
     __shared__ __attribute__((aligned(16))) float acc[NW][COLS][PITCH];
-    __shared__ float ml[NW][2][16];
+    __shared__ float ml[NW][2][COLS];
     const PagedBatch& B = P.b;
     const int g = blockIdx.x % B.kh, at = blockIdx.x / B.kh;
     const int lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const PagedItem I = pg_item(P, at, lane, false);
     if (!I.any) return;  // (block-uniform)
-    const int G = P.qh / B.kh, R = G * I.n, col = PACK ? lo & 7 : lo;
-    const int rr = I.tile * COLS + col;
-    const bool live = rr < R;
-    const int r = live ? rr / G : 0, h = live ? rr - r * G : 0;
-    const int lim = !live ? 0 : P.causal ? max(0, min(I.len, I.len - I.n + r + 1)) : I.len;
-    // keys below `open` every row sees, from `seen` on none
-    const int open = __builtin_amdgcn_readfirstlane(pg_row_min(live ? lim : 0x7fffffff));
-    const int seen = -__builtin_amdgcn_readfirstlane(pg_row_min(-lim));
+    const int G = P.qh / B.kh, R = G * I.n;
+    int lim[RW];
+    int open = 0x7fffffff, seen = 0;  // keys below `open` every row sees, from `seen` on none
+    pg_h8 qf[RW][KS];
+#pragma unroll
+    for (int x = 0; x < RW; ++x) {
+        const int rr = I.tile * COLS + 16 * x + (PACK ? lo & 7 : lo);
+        const bool live = rr < R;
+        const int r = live ? rr / G : 0, h = live ? rr - r * G : 0;
+        lim[x] = !live ? 0 : P.causal ? max(0, min(I.len, I.len - I.n + r + 1)) : I.len;
+        open = min(open, live ? lim[x] : 0x7fffffff);
+        seen = max(seen, lim[x]);
+        const long long q_at = (long long)(g * G + h) * P.q_head + (long long)(I.row + r) * P.q_row + 8 * hi;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) qf[x][i] = pg_load_q(P, q_at + 32 * i);
+    }
+    open = __builtin_amdgcn_readfirstlane(pg_row_min(open));
+    seen = -__builtin_amdgcn_readfirstlane(pg_row_min(-seen));
     const int units = (seen + 31) >> 5, each = (units + I.splits - 1) / I.splits;
     const int u_begin = I.split * each, u_end = min(units, u_begin + each);
-
-    pg_h8 qf[KS];
-    const long long q_at = (long long)(g * G + h) * P.q_head + (long long)(I.row + r) * P.q_row + 8 * hi;
-#pragma unroll
-    for (int i = 0; i < KS; ++i) qf[i] = pg_load_q(P, q_at + 32 * i);
 
     const float c = fminf(P.scale * 1.4426950408889634f, 0x1.fffffep127f);
     // Lane l's place in the table of the wave's next 32 units: unit l / 2, half l % 2,
@@ -341,13 +365,7 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_rows_kernel(AttnPagedParam
     int place = 0, place_at = -64 * NW;
     v4u kr[2][KS];
     v4u vr[2][4][H];
-    auto get = [](const __half* p) __attribute__((always_inline)) {
-        const v4u* q = reinterpret_cast<const v4u*>(p);
-        if constexpr (ONCE)
-            return __builtin_nontemporal_load(q);
-        else
-            return *q;
-    };
+    auto get = [](const auto* p) __attribute__((always_inline)) { return __builtin_nontemporal_load(p); };
     auto load = [&](int u) __attribute__((always_inline)) {
         if (u - place_at >= 32 * NW) {
             place = places(u);
@@ -360,37 +378,45 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_rows_kernel(AttnPagedParam
             const __half* kp = B.k + tile;
             const __half* vp = B.v + tile;
 #pragma unroll
-            for (int s = 0; s < KS; ++s) kr[t][s] = get(kp + pg_k_place(D, lo, 4 * s + hi) * 8);
+            for (int s = 0; s < KS; ++s) kr[t][s] = get(reinterpret_cast<const v4u*>(kp + pg_k_place(D, lo, 4 * s + hi) * 8));
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
                 for (int w = 0; w < H; ++w) {
                     const int j = 4 * hi + k;
                     if constexpr (D == 64) {
-                        const uint2 x = *reinterpret_cast<const uint2*>(vp + pg_v_place(D, j, lo >> 1) * 8 + (lo & 1) * 4);
-                        vr[t][k][w] = v4u{x.x, x.y, 0u, 0u};
+                        const u2 x = get(reinterpret_cast<const u2*>(vp + pg_v_place(D, j, lo >> 1) * 8 + (lo & 1) * 4));
+                        vr[t][k][w] = v4u{x[0], x[1], 0u, 0u};
                     } else {
-                        vr[t][k][w] = get(vp + pg_v_place(D, j, 16 * w + lo) * 8);
+                        vr[t][k][w] = get(reinterpret_cast<const v4u*>(vp + pg_v_place(D, j, 16 * w + lo) * 8));
                     }
                 }
         }
     };
 
-    float mrun = PG_NONE, lsum = 0.0f;
-    pg_f4 o[NB];
+    float mrun[RW], lsum[RW];
+    pg_f4 o[RW][NB];
 #pragma unroll
-    for (int n = 0; n < NB; ++n) o[n] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int x = 0; x < RW; ++x) {
+        mrun[x] = PG_NONE;
+        lsum[x] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) o[x][n] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
     bool wild = false;
     const float second = PACK && lo >= 8 ? 1.0f : 0.0f;
     for (int u = u_begin + wave; u < u_end; u += NW) {
         load(u);
-        pg_f4 s[2];
-        s[0] = s[1] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        pg_f4 s[RW][2];
+#pragma unroll
+        for (int x = 0; x < RW; ++x) s[x][0] = s[x][1] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < KS; ++i)
-                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pg_h8, kr[t][i]), qf[i], s[t], 0, 0, 0);
+#pragma unroll
+                for (int x = 0; x < RW; ++x)
+                    s[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pg_h8, kr[t][i]), qf[x][i], s[x][t], 0, 0, 0);
         if (u * 32 + 32 > open) {  // (uniform)
             unsigned odd = 0;
 #pragma unroll
@@ -398,61 +424,76 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_rows_kernel(AttnPagedParam
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int key = u * 32 + 16 * t + 4 * hi + k;
-                    if (key >= lim) s[t][k] = -INFINITY;
+#pragma unroll
+                    for (int x = 0; x < RW; ++x)
+                        if (key >= lim[x]) s[x][t][k] = -INFINITY;
                     // (0 times what is not finite is NaN: such a value of a key that not
-                    // every row sees is added after the last one)
+                    // every row sees is added after the last product)
                     const bool none = key >= seen;
 #pragma unroll
                     for (int w = 0; w < H; ++w)
 #pragma unroll
                         for (int i = 0; i < DW / 2; ++i) {
-                            unsigned x = vr[t][k][w][i];
-                            unsigned drop = (x & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u;
-                            drop |= (x & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u;
+                            const unsigned v = vr[t][k][w][i];
+                            unsigned drop = (v & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u;
+                            drop |= (v & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u;
                             if (key < open) drop = 0u;
                             if (!none) odd |= drop;
-                            vr[t][k][w][i] = none ? 0u : x & ~drop;
+                            vr[t][k][w][i] = none ? 0u : v & ~drop;
                         }
                 }
             wild |= odd != 0;
         }
-        float top = __builtin_elementwise_maximum(
-            __builtin_elementwise_maximum(__builtin_elementwise_maximum(s[0][0], s[0][1]),
-                                          __builtin_elementwise_maximum(s[0][2], s[0][3])),
-            __builtin_elementwise_maximum(__builtin_elementwise_maximum(s[1][0], s[1][1]),
-                                          __builtin_elementwise_maximum(s[1][2], s[1][3])));
-        top *= c;
-        if (__builtin_amdgcn_ballot_w64(top > mrun + (PG_LAZY + PG_SHIFT)) != 0) {
-            const float tm = pg_rows4_max(top) - PG_SHIFT;
-            if (tm > mrun + PG_LAZY) {
-                const float alpha = __builtin_amdgcn_exp2f(mrun - tm);
-                mrun = tm;
-                lsum *= alpha;
+        float top[RW];
+        bool over = false;
 #pragma unroll
-                for (int n = 0; n < NB; ++n) o[n] *= alpha;
+        for (int x = 0; x < RW; ++x) {
+            float m[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                m[t] = __builtin_elementwise_maximum(
+                    __builtin_elementwise_maximum(float(s[x][t][0]), float(s[x][t][1])),
+                    __builtin_elementwise_maximum(float(s[x][t][2]), float(s[x][t][3])));
+            top[x] = c * __builtin_elementwise_maximum(m[0], m[1]);
+            over |= top[x] > mrun[x] + (PG_LAZY + PG_SHIFT);
+        }
+        if (__builtin_amdgcn_ballot_w64(over) != 0) {
+#pragma unroll
+            for (int x = 0; x < RW; ++x) {
+                const float tm = pg_rows4_max(top[x]) - PG_SHIFT;
+                if (tm > mrun[x] + PG_LAZY) {
+                    const float alpha = __builtin_amdgcn_exp2f(mrun[x] - tm);
+                    mrun[x] = tm;
+                    lsum[x] *= alpha;
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) o[x][n] *= alpha;
+                }
             }
         }
-        pg_h8 ph, pl;
-        float l[2] = {0.0f, 0.0f};
+        pg_h8 ph[RW], pl[RW];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int x = 0; x < RW; ++x) {
+            float l[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int k = 0; k < 4; k += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][k], c, -mrun));
-                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][k + 1], c, -mrun));
-                const pg_h2 x = pg_round2(p0, p1);
-                if constexpr (PACK) {
-                    ph[4 * t + k] = (_Float16)__builtin_fmaf((float)x[0], -second, p0);
-                    ph[4 * t + k + 1] = (_Float16)__builtin_fmaf((float)x[1], -second, p1);
-                } else {
-                    ph[4 * t + k] = x[0];
-                    ph[4 * t + k + 1] = x[1];
-                    pl[4 * t + k] = (_Float16)(p0 - (float)x[0]);
-                    pl[4 * t + k + 1] = (_Float16)(p1 - (float)x[1]);
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int k = 0; k < 4; k += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][t][k], c, -mrun[x]));
+                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][t][k + 1], c, -mrun[x]));
+                    const pg_h2 y = pg_round2(p0, p1);
+                    if constexpr (PACK) {
+                        ph[x][4 * t + k] = (_Float16)__builtin_fmaf((float)y[0], -second, p0);
+                        ph[x][4 * t + k + 1] = (_Float16)__builtin_fmaf((float)y[1], -second, p1);
+                    } else {
+                        ph[x][4 * t + k] = y[0];
+                        ph[x][4 * t + k + 1] = y[1];
+                        pl[x][4 * t + k] = (_Float16)(p0 - (float)y[0]);
+                        pl[x][4 * t + k + 1] = (_Float16)(p1 - (float)y[1]);
+                    }
+                    l[t] += p0 + p1;
                 }
-                l[t] += p0 + p1;
-            }
-        lsum += l[0] + l[1];
+            lsum[x] += l[0] + l[1];
+        }
 #pragma unroll
         for (int w = 0; w < H; ++w)
 #pragma unroll
@@ -463,67 +504,76 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_rows_kernel(AttnPagedParam
                     a[i] = __builtin_amdgcn_perm(vr[i >> 1][2 * (i & 1) + 1][w][d >> 1], vr[i >> 1][2 * (i & 1)][w][d >> 1],
                                                  d & 1 ? 0x07060302u : 0x05040100u);
                 const pg_h8 av = __builtin_bit_cast(pg_h8, a);
-                o[w * DW + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, ph, o[w * DW + d], 0, 0, 0);
-                if constexpr (!PACK)
-                    o[w * DW + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, pl, o[w * DW + d], 0, 0, 0);
+                const int n = w * DW + d;
+#pragma unroll
+                for (int x = 0; x < RW; ++x) {
+                    o[x][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, ph[x], o[x][n], 0, 0, 0);
+                    if constexpr (!PACK) o[x][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, pl[x], o[x][n], 0, 0, 0);
+                }
             }
     }
-    lsum = pg_rows4_sum(lsum);
     // Infinities and NaN among the values: the products leave NaN of them (0, or a
     // negative second fp16, times an infinity). A result that they reach is their sum,
     // whatever the weights, which are positive.
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) wild |= !(fabsf(o[n][k]) < INFINITY);
-    if (__builtin_amdgcn_ballot_w64(wild) != 0) {
-        float sum[NB][4];
+    for (int x = 0; x < RW; ++x) {
+        lsum[x] = pg_rows4_sum(lsum[x]);
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) sum[n][k] = 0.0f;
+            for (int k = 0; k < 4; ++k) wild |= !(fabsf(o[x][n][k]) < INFINITY);
+    }
+    if (__builtin_amdgcn_ballot_w64(wild) != 0) {
 #pragma unroll 1
-        for (int u = u_begin + wave; u < u_end; u += NW) {
+        for (int n = 0; n < NB; ++n) {
+            float sum[RW][4] = {};
 #pragma unroll 1
-            for (int key = u * 32; key < min(u * 32 + 32, seen); ++key) {
-                const int j = key & 15;
-                const __half* vp = B.v + (size_t)pg_tile(B, I.s, g, key) * (16 * D);
+            for (int u = u_begin + wave; u < u_end; u += NW) {
+#pragma unroll 1
+                for (int key = u * 32; key < min(u * 32 + 32, seen); ++key) {
+                    const __half* vp = B.v + (size_t)pg_tile(B, I.s, g, key) * (16 * D);
 #pragma unroll
-                for (int w = 0; w < H; ++w)
+                    for (int k = 0; k < 4; ++k) {
+                        const int dim = 128 * (n / DW) + (4 * hi + k) * DW + n % DW;
+                        const float v = __half2float(vp[pg_v_place(D, key & 15, dim >> 3) * 8 + (dim & 7)]);
+#pragma unroll
+                        for (int x = 0; x < RW; ++x) sum[x][k] += key < lim[x] && !(fabsf(v) < INFINITY) ? v : 0.0f;
+                    }
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < NB; ++m)
+#pragma unroll
+                for (int x = 0; x < RW; ++x)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-#pragma unroll
-                        for (int d = 0; d < DW; ++d) {
-                            const int dim = 128 * w + (4 * hi + k) * DW + d;
-                            const float x = __half2float(vp[pg_v_place(D, j, dim >> 3) * 8 + (dim & 7)]);
-                            sum[w * DW + d][k] += key < lim && !(fabsf(x) < INFINITY) ? x : 0.0f;
-                        }
-            }
+                        if (m == n) o[x][m][k] = fabsf(sum[x][k]) < INFINITY ? float(o[x][m][k]) : sum[x][k];
         }
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) o[n][k] = fabsf(sum[n][k]) < INFINITY ? float(o[n][k]) : sum[n][k];
     }
-    // The waves meet. Lane (lo, hi) has dims 128 w + (4 hi + k) DW + d of its row.
+    // The waves meet. Lane (lo, hi) has dims 128 w + (4 hi + k) DW + d of its rows.
     if constexpr (PACK) {
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) o[n][k] += dpp_move<0x128>(float(o[n][k]));  // row_ror:8
+            for (int k = 0; k < 4; ++k) o[0][n][k] += dpp_move<0x128>(float(o[0][n][k]));  // row_ror:8
     }
-    if (lo < COLS) {
+    if (!PACK || lo < 8) {
 #pragma unroll
-        for (int w = 0; w < H; ++w)
+        for (int x = 0; x < RW; ++x) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+            for (int w = 0; w < H; ++w)
 #pragma unroll
-                for (int d = 0; d < DW; d += 4)
-                    *reinterpret_cast<pg_f4*>(&acc[wave][lo][128 * w + (4 * hi + k) * DW + d]) =
-                        pg_f4{o[w * DW + d][k], o[w * DW + d + 1][k], o[w * DW + d + 2][k], o[w * DW + d + 3][k]};
-        if (hi == 0) {
-            ml[wave][0][lo] = mrun;
-            ml[wave][1][lo] = lsum;
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int d = 0; d < DW; d += 4) {
+                        const int n = w * DW + d;
+                        *reinterpret_cast<pg_f4*>(&acc[wave][16 * x + lo][128 * w + (4 * hi + k) * DW + d]) =
+                            pg_f4{o[x][n][k], o[x][n + 1][k], o[x][n + 2][k], o[x][n + 3][k]};
+                    }
+            if (hi == 0) {
+                ml[wave][0][16 * x + lo] = mrun[x];
+                ml[wave][1][16 * x + lo] = lsum[x];
+            }
         }
     }
     __syncthreads();
@@ -989,11 +1039,10 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(AttnPagedParams P)
 }
 
 // The kernel of a run: attn_paged_tile_kernel in stages of `units` units, or
-// attn_paged_rows_kernel with loads that leave nothing in the caches (`once`).
+// attn_paged_rows_kernel, whose tiles hold all rows of a sequence.
 struct PagedPlan {
     bool tile;
     int units;
-    bool once;
 };
 
 void launch_attn_paged_64(const AttnPagedParams& P, const PagedPlan& plan, hipStream_t s);
@@ -1010,27 +1059,25 @@ static void launch_attn_paged_tile(const AttnPagedParams& P, hipStream_t s) {
         hipLaunchKernelGGL((attn_paged_tile_kernel<D, W, U, NW, true>), grid, block, 0, s, P);
 }
 
-template <int D, bool ONCE>
+template <int D>
 static void launch_attn_paged_rows(const AttnPagedParams& P, hipStream_t s) {
-    const dim3 grid(P.b.kh * P.items);
+    const dim3 grid(P.b.kh * P.items), block(256);
     if (P.tile_rows == 8)
-        hipLaunchKernelGGL((attn_paged_rows_kernel<D, 4, true, ONCE>), grid, dim3(256), 0, s, P);
-    else
-        hipLaunchKernelGGL((attn_paged_rows_kernel<D, 4, false, ONCE>), grid, dim3(256), 0, s, P);
+        hipLaunchKernelGGL((attn_paged_rows_kernel<D, 4, 1, true>), grid, block, 0, s, P);
+    else if (P.tile_rows == 16)
+        hipLaunchKernelGGL((attn_paged_rows_kernel<D, 4, 1, false>), grid, block, 0, s, P);
+    else if constexpr (D < 256)
+        hipLaunchKernelGGL((attn_paged_rows_kernel<D, 4, 2, false>), grid, block, 0, s, P);
 }
 
 template <int D>
 static void launch_attn_paged(const AttnPagedParams& P, const PagedPlan& plan, hipStream_t s) {
-    if (plan.tile) {
-        if (D < 256 && plan.units == 2)
-            launch_attn_paged_tile<D, D < 256 ? 2 : 1>(P, s);
-        else
-            launch_attn_paged_tile<D, 1>(P, s);
-    } else if (plan.once) {
-        launch_attn_paged_rows<D, true>(P, s);
-    } else {
-        launch_attn_paged_rows<D, false>(P, s);
-    }
+    if (!plan.tile)
+        launch_attn_paged_rows<D>(P, s);
+    else if (D < 256 && plan.units == 2)
+        launch_attn_paged_tile<D, D < 256 ? 2 : 1>(P, s);
+    else
+        launch_attn_paged_tile<D, 1>(P, s);
     if (P.target) {
         // (many rows: as many a block as leave a row the threads for its dims)
         constexpr int MANY = 1024 / D < 8 ? 1024 / D : 8;

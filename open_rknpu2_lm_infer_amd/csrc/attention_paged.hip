@@ -311,6 +311,7 @@ static PagedPlan paged_plan(AttnPagedParams& P, int D) {
     // (units are added up in 32 bits)
     if (units > 16 && P.tiles < want && (int64_t)P.tiles * units < (1 << 30)) P.target = want;
     P.items = P.target ? P.tiles + want : P.tiles;
+    P.wave = plan.tile && P.causal ? std::max(1, cus / B.kh) : 0;
     return plan;
 }
 

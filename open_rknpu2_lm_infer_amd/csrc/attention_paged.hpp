@@ -109,6 +109,7 @@ struct AttnPagedParams {
     int least;       // units of a split, at least
     int tile_rows;   // query rows of a block
     int tiles;       // row tiles of the whole batch, at most
+    int wave;        // blocks per KV head that a block for each CU are, where long tiles come first; 0: they do not
 };
 
 __device__ __forceinline__ int pg_scan(int v) {  // inclusive, over the wave
@@ -155,6 +156,37 @@ __device__ __forceinline__ PagedItem pg_item(const AttnPagedParams& P, int at, i
     }
     PagedSeq mine = lane * C < B.sequences ? pg_seq(B, lane * C) : none;
     // (one sequence a lane: the one in registers)
+    if (!P.target && P.wave > 0 && C == 1) {
+        // By tiles' places in their sequences, the last places first: above(k) blocks have
+        // places from k on. Where two blocks a CU hold them all, the second ones come in
+        // reverse, a short one beside a long one.
+        const int t = tiles_of(mine), total = wave_sum(t);
+        PagedItem x{};
+        x.any = at < total;
+        if (!x.any) return x;
+        if (total > P.wave) {
+            const int i = at >= P.wave && total <= 2 * P.wave ? total - 1 - (at - P.wave) : at;
+            auto above = [&](int k) { return wave_sum(max(0, t - k)); };
+            int k = 0, end = (int)wave_max((float)t) + 1;
+            while (end - k > 1) {
+                const int mid = (k + end) >> 1;
+                if (above(mid) > i)
+                    k = mid;
+                else
+                    end = mid;
+            }
+            const unsigned long long has = __builtin_amdgcn_ballot_w64(t > k);
+            const int nth = i - above(k + 1);
+            const int rank = __builtin_amdgcn_mbcnt_hi((unsigned)(has >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)has, 0));
+            x.s = __builtin_ctzll(__builtin_amdgcn_ballot_w64(t > k && rank == nth) | 1ull << 63);
+            x.row = __builtin_amdgcn_readlane(mine.row, x.s);
+            x.n = __builtin_amdgcn_readlane(mine.n, x.s);
+            x.len = __builtin_amdgcn_readlane(mine.len, x.s);
+            x.tile = k;
+            x.splits = 1;
+            return x;
+        }
+    }
     auto seq = [&](int i) { return C == 1 ? mine : lane * C + i < B.sequences ? pg_seq(B, lane * C + i) : none; };
     unsigned per = 0x7fffffff;
     if (P.target > 0) {

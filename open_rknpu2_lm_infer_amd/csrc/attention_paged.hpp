@@ -676,6 +676,7 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_tile_kernel(AttnPagedParam
     constexpr int PT = TILE / 1024 / WT;           // 16-byte pieces of a lane's
     constexpr float LAZY = SPLIT ? 8.0f : 6.0f, SHIFT = (SPLIT ? 14.0f : 15.0f) - LAZY;
     static_assert(NW % (4 * U) == 0 && (U == 1 || U == 2) && (W == 16 || W == 32), "stage shape");
+    static_assert(NW * W * 128 <= 2 * BUFS * STAGE, "room for the rows on their way out");
     typedef float fv __attribute__((ext_vector_type(CL)));
     typedef short s4 __attribute__((ext_vector_type(4)));
     typedef short s8 __attribute__((ext_vector_type(8)));
@@ -694,9 +695,10 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_tile_kernel(AttnPagedParam
     const int r = live ? rr / G : 0, h = live ? rr - r * G : 0;
     const int before = I.len - I.n;  // tokens before the rows' (causal)
     const int lim = !live ? 0 : P.causal ? max(0, min(I.len, before + r + 1)) : I.len;
-    // keys below `open` every row of the wave sees
-    const int open = W == 32 ? pg_lo_min(live ? lim : 0x7fffffff)
-                             : __builtin_amdgcn_readfirstlane(pg_row_min(live ? lim : 0x7fffffff));
+    // keys below `open` every row of the wave sees (none without rows: what lies behind a
+    // sequence may be NaN)
+    const int first = live ? lim : 0x7fffffff, least = W == 32 ? pg_lo_min(first) : __builtin_amdgcn_readfirstlane(pg_row_min(first));
+    const int open = least == 0x7fffffff ? 0 : least;
     // keys that the block's last row sees, their units, and this block's
     const int last = min(R, (I.tile + 1) * ROWS) - 1;
     const int seen = P.causal ? max(0, min(I.len, before + last / G + 1)) : I.len, all = (seen + 31) >> 5;
@@ -968,25 +970,47 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_tile_kernel(AttnPagedParam
                     if (m == n) o[m][k] = fabsf(sum[k]) < INFINITY ? float(o[m][k]) : float(sum[k]);
         }
     }
-    if (!live) return;
-    if (I.splits == 1) {
-        const float il = lim == 0 ? 0.0f : 1.0f / lsum;
-        const long long to = (long long)(g * G + h) * P.o_head + (long long)(I.row + r) * P.o_row + 4 * hi;
+    // Rows leave 32 dims at a time through LDS, so that 8 lanes store a row's 128 bytes:
+    // 16-byte pieces, piece p of row r at place p ^ (r & 7).
+    __syncthreads();
+    const float il = I.splits > 1 ? 1.0f : lim == 0 ? 0.0f : 1.0f / lsum;
+    const size_t part_at = ((size_t)at * B.kh + g) * ROWS + W * wave;
+    if (I.splits > 1 && hi == 0 && live)
+        *reinterpret_cast<float2*>(P.part + (size_t)P.items * B.kh * ROWS * D + (part_at + lo) * 2) = float2{mrun, lsum};
+    const long long own = I.splits > 1 ? (long long)(part_at + lo) * D
+                                       : (long long)(g * G + h) * P.o_head + (long long)(I.row + r) * P.o_row;
+    uint8_t* const box = smem + wave * (W * 128);
+    constexpr int LR = W / 8;  // rows of a lane
+    long long to[LR];
+    bool write[LR];
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+    for (int i = 0; i < LR; ++i) {
+        const int row = (lane >> 3) + 8 * i;
+        to[i] = __shfl(own, row) + 4 * (lane & 7);
+        write[i] = (I.tile * NW + wave) * W + row < R;
+    }
 #pragma unroll
-            for (int k = 0; k < CL; k += 4)
-                pg_store4(P, to + W * n + 2 * k, o[n][k] * il, o[n][k + 1] * il, o[n][k + 2] * il, o[n][k + 3] * il);
-    } else {
-        const size_t row_at = ((size_t)at * B.kh + g) * ROWS + W * wave + lo;
-        float* p = P.part + row_at * D + 4 * hi;
+    for (int x = 0; x < D / 32; ++x) {
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+        for (int k = 0; k < 32 * W / 64; k += 4) {
+            const int n = (32 * x) / W + k / CL, piece = W == 32 ? 2 * (k >> 2) + hi : 4 * (k / CL) + hi;
+            *reinterpret_cast<pg_f4*>(box + lo * 128 + ((piece ^ (lo & 7)) * 16)) =
+                pg_f4{o[n][k % CL] * il, o[n][k % CL + 1] * il, o[n][k % CL + 2] * il, o[n][k % CL + 3] * il};
+        }
+        pg_f4 y[LR];
 #pragma unroll
-            for (int k = 0; k < CL; k += 4)
-                *reinterpret_cast<pg_f4*>(p + W * n + 2 * k) = pg_f4{o[n][k], o[n][k + 1], o[n][k + 2], o[n][k + 3]};
-        if (hi == 0)
-            *reinterpret_cast<float2*>(P.part + (size_t)P.items * B.kh * ROWS * D + row_at * 2) = float2{mrun, lsum};
+        for (int i = 0; i < LR; ++i) {
+            const int row = (lane >> 3) + 8 * i;
+            y[i] = *reinterpret_cast<const pg_f4*>(box + row * 128 + (((lane & 7) ^ (row & 7)) * 16));
+        }
+#pragma unroll
+        for (int i = 0; i < LR; ++i) {
+            if (!write[i]) continue;
+            if (I.splits > 1)
+                *reinterpret_cast<pg_f4*>(P.part + to[i] + 32 * x) = y[i];
+            else
+                pg_store4(P, to[i] + 32 * x, y[i][0], y[i][1], y[i][2], y[i][3]);
+        }
     }
 }
 

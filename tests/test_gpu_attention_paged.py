@@ -304,6 +304,32 @@ def test_what_lies_behind_a_sequence_does_not_count(ctx, causal, rows):
 
 
 @pytest.mark.parametrize("d", [64, 128, 256])
+def test_what_lies_behind_a_sequence_costs_nothing(ctx, d):
+    """The path for values that are not finite is for those that rows see."""
+    times = []
+    for fill in (0.0, float("nan")):
+        p = Pool(ctx, 4, 4, d, 1, page=256, most=2048, spare=0)
+        bad = torch.full((4, 2048, d), fill, dtype=torch.float16, device="cuda")
+        p.pages.append(p.batch([2048], [2048]), bad, bad)
+        p.fill([1810])
+        q = dev(p.rows(330, 4))
+        out = torch.empty_like(q)
+        b = p.batch([330])
+        best = 1e9
+        for _ in range(5):
+            t = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+            t[0].record()
+            for _ in range(10):
+                D.attention_paged(ctx, p.pages, b, q, out)
+            t[1].record()
+            torch.cuda.synchronize()
+            best = min(best, t[0].elapsed_time(t[1]))
+        times.append(best)
+        assert bool(torch.isfinite(out).all())
+    assert times[1] < 3 * times[0]
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("rows", [[3], [40], [130]])
 def test_wild_values_count_for_the_rows_that_see_them(ctx, d, rows):
     p = Pool(ctx, 4, 2, d, 1, page=16, most=160, seed=d)

@@ -289,7 +289,26 @@ static bool paged_same_geometry(const AttnWork* w, const PagedPool* c) {
            device_of(w->domain) == device_of(c->domain);
 }
 
-// Which kernel, its row tiles, and the blocks that splits aim at.
+// Which kernel, its row tiles, and the blocks that splits aim at. R: query rows of a
+// sequence and KV head, at most. Times in us.
+//
+// attn_paged_rows_kernel while a tile holds R, so that pages are read once: 5 rows of 12
+// sequences (R = 20, 240 MB) 51 to 56 with tiles of 32, 61 with two of 16. (Two row groups
+// of 256 dims have no registers.)
+//
+// attn_paged_tile_kernel with blocks of 128 rows for short sequences, whose long blocks
+// are what a call lasts, of 256 for long ones, whose K and V then meet twice as many rows
+// in LDS: one sequence's 2048 rows 64 and 74, 8 x 1024 131 and 142, 64 rows after 4000
+// tokens 25 and 29; 8192 rows 720 and 709, 4 x 512 after 8000 327 and 308, 2 x 4096 of 64
+// dims 118 and 113.
+//
+// Splits, in blocks a CU. Rows kernel: one where there are few sequences, as a block's rows
+// leave partials (2 sequences of 131072 tokens 196 with one, 198 with two, 201 with four;
+// one of 4000 14 with each), four where there are more, whose pieces are then of like
+// length (64 of up to 8100 tokens 194 unsplit, 181 with four, 179 with six; 16 of 256 dims
+// 66, 64 and 64; 12 x 5 rows 64 with one, 62 with four). A split holds a unit a wave at
+// least: one sequence of 4000 tokens 12.7 and 13.3 with two, 16 with four. Tile kernel: as many as stay on a CU; 8 units at least:
+// 128 rows of 256 dims after 3600 tokens 35, with 16 units 44, with 24 50.
 static PagedPlan paged_plan(AttnPagedParams& P, int D) {
     const PagedBatch& B = P.b;
     const int G = P.qh / B.kh, cus = device_cus();
@@ -302,7 +321,7 @@ static PagedPlan paged_plan(AttnPagedParams& P, int D) {
     const PagedPlan plan{R > (D == 256 ? 16 : 32), D < 256 && units > 128 ? 2 : 1};
     P.tile_rows = plan.tile ? 128 * plan.units : R <= 8 ? 8 : R <= 16 ? 16 : 32;
     P.tiles = (int)tiles(P.tile_rows);
-    P.least = 8;
+    P.least = plan.tile ? 8 : 4;
     P.target = 0;
     const int blocks = plan.tile ? (plan.units == 1 && D < 256 ? 2 : 1) : B.sequences > 4 ? 4 : 1;
     // (as many as the workspace holds partials for)

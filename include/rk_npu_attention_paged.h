@@ -33,10 +33,11 @@
  * rounded), f32 scores, weights and sums, for |scale q k| up to 10^7 (beyond, a row
  * may come out as NaN). A weight goes into the products with V as two fp16 (22
  * bits), or as one (11 bits) where the output is fp16 and a sequence may have more
- * than 16 query rows per KV head (max_rows x query heads / KV heads). A causal row
- * sees the tokens up to its own, a row without a mask all lengths[s]. A row that
- * sees no token is 0. Infinities and NaN in K or V count for the rows that see
- * their token and for no other.
+ * than 32 query rows per KV head (max_rows x query heads / KV heads; more than 16 of
+ * head_dim 256). Where fp16 has fewer bits it is off by up to 2^-30 of the row's
+ * largest weight. A causal row sees the tokens up to its own, a row without a mask
+ * all lengths[s]. A row that sees no token is 0. Infinities and NaN in K or V count
+ * for the rows that see their token and for no other.
  *
  * What the device finds wrong. A length below 0 or above max_tokens, row_offsets
  * that fall or pass `rows` or give a sequence more than max_rows, and a page
@@ -110,7 +111,8 @@ void rk_npu_hip_attention_paged_pool_free(rk_npu_hip_attention_paged_pool* pool)
 
 /* Waits for the device calls made with the pool (for a graph's launches, and calls
  * on several streams, for the whole device) and tells whether one since the last
- * status found something wrong in its batch: RK_NPU_ERR_PARAM, or RK_NPU_OK. */
+ * status found something wrong in its batch: RK_NPU_ERR_PARAM, or RK_NPU_OK. Not
+ * while a stream is being captured. */
 int rk_npu_hip_attention_paged_status(rk_npu_hip_attention_paged_pool* pool);
 
 /* ---- on the caller's stream (NULL: the null stream) ---------------------------

@@ -350,6 +350,15 @@ constexpr float PG_LAZY = 4.0f, PG_SHIFT = 10.0f;
 // with V as two fp16. PACK: columns 8..15 are columns 0..7 again and take the second
 // fp16, so that both cost one product. A tile holds all rows of a sequence, so pages
 // are read once, by loads that leave nothing in the caches.
+//
+// Measured with the join, contexts not in the last-level cache: one row of 32 heads over 8
+// of 128 and 64 sequences of 60 to 8100 tokens (1.08 GB) 182 us, 5.9 TB/s; 2 of 131072 162,
+// 6.6 (a large copy reads and writes 5.1); cached loads 202 and 214. 256 sequences of up to
+// 700 tokens of 8 heads of 64 33 (42). 16 sequences of 2 heads of 256 57: 4.6 TB/s, 216
+// registers leave two blocks a CU. One of 4000 tokens 12.3, latency: launch, table, one
+// unit's loads and products, the waves' meeting (7.6), the join (4.7). The next unit's
+// loads before this one's products changed nothing with 128 dims and lost with 256 (51 to
+// 57: registers).
 template <int D, int NW, int RW, bool PACK>
 __global__ __launch_bounds__(64 * NW) void attn_paged_rows_kernel(AttnPagedParams P) {
     constexpr int KS = D / 32;                  // 32-dim steps of a score
@@ -663,6 +672,19 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_rows_kernel(AttnPagedParam
 // j + 1 and multiplies V of unit j - 1: one straight piece of code in which matrix and
 // vector instructions do not depend on each other. In stage t K of stage t + 2 and V of
 // stage t + U - 1 go to LDS, loaded in the stage before.
+//
+// f32 output takes V's products twice (SPLIT). W: 32 rows a wave halve the LDS reads of a
+// product; of 256 dims they need 448 registers, one wave a SIMD (57600 keys, 1024 rows of
+// 2 heads 239 us, with 16 rows 202; 4-wave blocks of 64 rows 267).
+//
+// Measured with the join: 512 rows of 32 heads over 8 of 128 after 65000 tokens 556 us, 0.98
+// PFLOP/s of a large matrix product's 1.17; matrix cores 54 % busy, LDS 34 %, at 1.7 to 1.8
+// GHz: the power limit holds the clock. LDS reads without turned places 28 % longer. 6
+// prompts of 17 to 1365 rows 54 us: a long prompt's last block walks 43 units alone
+// or beside one other. 100 to 200 rows of 16 heads over 2 of 256, f32 output, 72: matrix
+// cores 43 % busy (51 % and 1.5 GHz over longer contexts), two fp16 for a weight, the join 10. Matrix
+// and vector instructions or LDS reads put in turns by scheduling groups: no difference
+// of 128 dims or 256.
 template <int D, int W, int U, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW) void attn_paged_tile_kernel(AttnPagedParams P) {
     constexpr int CL = W * W / 64;                 // values of a lane in a C operand
@@ -1018,6 +1040,9 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_tile_kernel(AttnPagedParam
 // sum_s w_s l_s with w_s = 2^(m_s - max m). T = 256 / RPB threads a row, thread t with 4
 // dims of every GS-th split; their first loads do not wait for the weights, which the
 // row's threads find meanwhile; sums over the GS groups meet in LDS.
+//
+// Measured: one row of 32 heads, 32 splits 4.7 us; 2048 rows of 8 heads, 4 splits (33 MB
+// read) 11 (36 with a block a row).
 template <int D, int RPB>
 __global__ __launch_bounds__(256) void attn_paged_join_kernel(AttnPagedParams P) {
     constexpr int T = 256 / RPB, LD = D / 4, GS = T / LD, AHEAD = 8, W = PAGED_MAX_SPLITS / T;

@@ -61,11 +61,12 @@ def attention_bound(q, k, scale, half_out, one_weight, tokens):
     products' sums by one f32 rounding a step, at most tokens / 32 + 16 steps in a row
     of 32-key matrix steps and joins (2^-24 each; a matrix step's own 32 products round
     within 2^-22). All of it counts twice: in the weights' products and in their
-    sum. The second fp16 of a small weight has steps of 2^-24 where the row's largest
-    weight is above 2^10: 2^-35 of it for each token. fp16 output: half a unit, 2^-11."""
+    sum. Below 2^-14 fp16 has steps of 2^-24, half of which is lost of each token's
+    weight, where the row's largest weight is above 2^5: 2^-30 of it. fp16 output: half a
+    unit, 2^-11."""
     q, k = np.asarray(q, np.float64), np.asarray(k, np.float64)
     s = scale * np.sqrt((q ** 2).sum(-1).max() * (k ** 2).sum(-1).max())
     d = q.shape[-1]
     weight = (d + 3) * 2.0 ** -24 * s + 2.0 ** -22 + (2.0 ** -11 if one_weight else 2.0 ** -22)
-    sums = (tokens / 32 + 16) * 2.0 ** -24 + 2.0 ** -22 + tokens * 2.0 ** -35
+    sums = (tokens / 32 + 16) * 2.0 ** -24 + 2.0 ** -22 + tokens * 2.0 ** -30
     return 2.0 * (weight + sums) + (2.0 ** -11 if half_out else 0.0)

@@ -285,12 +285,12 @@ class PagedBatch:
     token t being table[s][t // page]; lengths [sequences], the call's rows among
     them; row_offsets [sequences + 1], sequence s having rows row_offsets[s] to
     row_offsets[s + 1], or None: row s. No sequence has more than max_rows rows or
-    max_tokens tokens (default: what the table holds)."""
+    max_tokens tokens (default: what the table and the pages' capacity hold)."""
 
     def __init__(self, table, lengths, row_offsets=None, max_rows: int = 1, max_tokens: Optional[int] = None):
         ensure(len(table.shape) == 2 and len(lengths.shape) == 1, "a table is [sequences][pages], lengths [sequences]")
         n = lengths.shape[0]
-        self.table, self.lengths, self.row_offsets = table, lengths, row_offsets
+        self._tensors = table, lengths, row_offsets
         self.sequences, self.max_rows, self.max_tokens = n, int32(max_rows, "max_rows"), max_tokens
         if max_tokens is not None:
             int32(max_tokens, "max_tokens")
@@ -301,10 +301,22 @@ class PagedBatch:
                     None if row_offsets is None else _ints(row_offsets, "row_offsets", (n + 1,)),
                     _ints(table, "table", (n, self._columns)), self._stride)
 
-    def _raw(self, rows: int, page: int) -> F.rk_npu_hip_paged_batch:
+    @property
+    def table(self):
+        return self._tensors[0]
+
+    @property
+    def lengths(self):
+        return self._tensors[1]
+
+    @property
+    def row_offsets(self):
+        return self._tensors[2]
+
+    def _raw(self, rows: int, page: int, capacity: int = F.RK_NPU_HIP_PAGED_MAX_TOKENS) -> F.rk_npu_hip_paged_batch:
         most, tokens = self._columns * page, self.max_tokens
         if tokens is None:
-            tokens = min(most, F.RK_NPU_HIP_PAGED_MAX_TOKENS)
+            tokens = min(most, capacity)
         elif tokens > most:
             raise NpuError(f"the table holds {most} tokens a sequence, max_tokens is {tokens}")
         if rows >= 2 ** 31:
@@ -347,7 +359,7 @@ class KvPages:
         check(L.rk_npu_hip_attention_paged_pool_create(ctx.domain, ctypes.byref(cfg), ctypes.byref(raw)),
               "create the KV pages")
         self.handle = _Handle(raw.value, L.rk_npu_hip_attention_paged_pool_free, "KV pages", ctx.shared)
-        self.ctx, self.config, self.page = ctx, cfg, page
+        self.ctx, self.config, self.page, self.capacity = ctx, cfg, page, capacity
         self._kv, self._query = (kv_heads, head_dim), (query_heads, head_dim)
 
     def bytes(self) -> int:
@@ -377,7 +389,7 @@ class KvPages:
                 raise NpuError("q, q_out and k must have the same rows")
         if positions is not None:
             at = _ints(positions, "positions", (rows,))
-        check(F.lib().rk_npu_hip_attention_paged_append(self.handle.raw, batch._raw(rows, self.page), kh, vh, at, qh, oh,
+        check(F.lib().rk_npu_hip_attention_paged_append(self.handle.raw, batch._raw(rows, self.page, self.capacity), kh, vh, at, qh, oh,
                                                         _stream(stream, k)), "append to the KV pages")
 
     def read(self, batch: PagedBatch, k, v, stream=None) -> None:
@@ -386,7 +398,7 @@ class KvPages:
         if shape != v.shape:
             raise NpuError("k and v must have the same shape")
         kh, vh = _heads(k, *self._kv), _heads(v, *self._kv)
-        check(F.lib().rk_npu_hip_attention_paged_read(self.handle.raw, batch._raw(shape[1], self.page), kh, vh,
+        check(F.lib().rk_npu_hip_attention_paged_read(self.handle.raw, batch._raw(shape[1], self.page, self.capacity), kh, vh,
                                                       _stream(stream, k)), "read the KV pages")
 
 
@@ -399,7 +411,7 @@ def attention_paged(ctx: DeviceContext, pages: KvPages, batch: PagedBatch, q, ou
         raise NpuError("q and out must have the same shape")
     ws = ws or ctx.attention_workspace(pages)
     qh, oh = _heads(q, *pages._query), _heads(out, *pages._query)
-    check(F.lib().rk_npu_hip_attention_paged_run(ws.raw, pages.handle.raw, batch._raw(shape[1], pages.page), qh, oh,
+    check(F.lib().rk_npu_hip_attention_paged_run(ws.raw, pages.handle.raw, batch._raw(shape[1], pages.page, pages.capacity), qh, oh,
                                                  _stream(stream, q)), "attention over the KV pages")
 
 

@@ -107,6 +107,9 @@ def test_batches():
     raw = b._raw(20, 16)
     assert (raw.sequences, raw.rows, raw.max_rows, raw.max_tokens, raw.table_stride) == (3, 20, 7, 80, 5)
     assert D.PagedBatch(Ints(3, 5, stride=(9, 1)), Ints(3), max_tokens=33)._raw(3, 16).table_stride == 9
+    assert b._raw(20, 16, 50).max_tokens == 50      # (the pages' capacity)
+    with pytest.raises(AttributeError):
+        b.lengths = Ints(3)
     for build in (lambda: D.PagedBatch(Ints(3, 5), Ints(2)), lambda: D.PagedBatch(Ints(3, 5), Ints(3), Ints(3)),
                   lambda: D.PagedBatch(Ints(3, 5, stride=(1, 3)), Ints(3)),
                   lambda: D.PagedBatch(Ints(3, 5, stride=(4, 1)), Ints(3)),

@@ -269,6 +269,97 @@ def test_long_lengths_are_split_and_joined(ctx, d, qh, kh, lengths, rows):
         p.attend(rows, dtype=dtype, max_tokens=max(lengths))
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("causal", [True, False])
+def test_drafts(ctx, d, causal):
+    """2 to 8 rows of 4 heads a KV head: every row tile of few rows, whole and split."""
+    p = Pool(ctx, 8, 2, d, 5, page=16, most=1500, causal=causal, seed=d)
+    p.fill([1500, 5, 33, 700, 64])
+    for rows in ([2, 2, 2, 2, 2], [4, 1, 3, 4, 0], [5, 5, 5, 5, 5], [8, 7, 1, 0, 8]):
+        for dtype in (torch.float32, torch.float16):
+            p.attend(rows, dtype=dtype, behind=1)
+    p.attend([8, 7, 1, 0, 8], [1400, 5, 3, 0, 40])
+
+
+@pytest.mark.parametrize("qh,kh,d", [(64, 1, 64), (256, 1, 64), (32, 32, 128), (40, 1, 256), (96, 3, 64)])
+def test_many_heads(ctx, qh, kh, d):
+    """One row whose heads fill several row tiles, many KV heads, a number that 8 does not divide."""
+    p = Pool(ctx, qh, kh, d, 3, page=32, most=900, seed=qh)
+    p.fill([900, 1, 40])
+    for dtype in (torch.float32, torch.float16):
+        p.attend([1, 1, 1], dtype=dtype)
+    n = p.lengths()
+    q = p.rows(3, qh)
+    out = torch.full((qh, 3, d), 77.0, device="cuda")
+    D.attention_paged(ctx, p.pages, D.PagedBatch(dev(p.table), ints(n)), dev(q), out)
+    p.compare([1, 1, 1], n, q, out)
+
+
+@pytest.mark.parametrize("rows", [[700, 40, 500], [900, 700, 500]])
+def test_prompts_of_many_blocks(ctx, rows):
+    """More row tiles than CUs: long ones first, over all sequences."""
+    p = Pool(ctx, 32, 8, 64, 3, page=64, most=1000, seed=1)
+    p.fill([rows[0], rows[1] + 33, rows[2]])
+    p.attend(rows, dtype=torch.float16, pad=1)
+
+
+def test_many_sequences_split(ctx):
+    """More sequences than a wave has lanes, one long: splits, and a schedule of several a lane."""
+    p = Pool(ctx, 4, 2, 64, 150, page=32, most=2100, seed=5)
+    n = [int(x) for x in p.rng.integers(0, 60, 150)]
+    n[140], n[3] = 2100, 1000
+    p.fill(n)
+    p.attend([1] * 150)
+    p.attend([int(x) for x in p.rng.integers(0, 9, 150)], dtype=torch.float16)
+    p.attend([int(x) for x in p.rng.integers(0, 30, 150)])
+
+
+@pytest.mark.parametrize("d,qh,kh,sequences,rows,tokens", [
+    (64, 32, 32, 40, 1, 9000), (128, 64, 32, 40, 3, 9000), (64, 32, 8, 33, 16, 9000), (256, 16, 8, 17, 20, 5000)])
+def test_long_lengths_in_one_block(ctx, d, qh, kh, sequences, rows, tokens):
+    """Blocks that walk thousands of tokens: many sequences over the same pages, a table with room between its rows."""
+    p = Pool(ctx, qh, kh, d, 1, page=64, most=tokens, seed=d)
+    p.fill([tokens])
+    wide = torch.full((sequences, p.table.shape[1] + 5), -7, dtype=torch.int32, device="cuda")
+    wide[:, :p.table.shape[1]] = dev(p.table)
+    q = p.rows(sequences * rows, qh)
+    lengths = [tokens - 3 * i for i in range(sequences)]
+    b = D.PagedBatch(wide[:, :p.table.shape[1]], ints(lengths), ints([rows * i for i in range(sequences + 1)]), max_rows=rows)
+    for dtype in (torch.float32, torch.float16):
+        out = torch.full((qh, sequences * rows, d), 77.0, dtype=dtype, device="cuda")
+        D.attention_paged(ctx, p.pages, b, dev(q), out)
+        p.pages.check()
+        assert bool(torch.isfinite(out).all()) and float(out.abs().max()) < 70.0
+        for s in (0, sequences // 2, sequences - 1):
+            mine = slice(s * rows, (s + 1) * rows)
+            p.compare([rows], [lengths[s]], q[:, mine], out[:, mine])
+
+
+def test_pages_beyond_32_bits(ctx):
+    """A pool whose K and V pass 2^32 bytes each, rows in its last pages."""
+    pages = D.KvPages(ctx, 8, 8, 256, 0.0625, 4200, page=256, rotary_dim=0)
+    assert pages.bytes() == 2 * 4200 * 256 * 8 * 256 * 2 > 2 ** 33
+    rng = np.random.default_rng(0)
+    k, v = (rng.standard_normal((8, 300, 256)).astype(np.float16) for _ in range(2))
+    table = ints([[4199, 4198], [4100, 0]])
+    b = D.PagedBatch(table, ints([290, 10]), ints([0, 290, 300]), max_rows=290)
+    pages.append(b, dev(k), dev(v))
+    got = [torch.empty(8, 300, 256, dtype=torch.float16, device="cuda") for _ in range(2)]
+    pages.read(b, *got)
+    assert np.array_equal(got[0].cpu().numpy(), k) and np.array_equal(got[1].cpu().numpy(), v)
+    for rows in ([1, 1], [20, 10]):
+        total = sum(rows)
+        q = rng.standard_normal((8, total, 256)).astype(np.float16)
+        out = torch.empty(8, total, 256, device="cuda")
+        D.attention_paged(ctx, pages, D.PagedBatch(table, ints([290, 10]), ints([0, rows[0], total]), max_rows=rows[0]), dev(q), out)
+        pages.check()
+        for mine, keys in ((slice(0, rows[0]), slice(0, 290)), (slice(rows[0], total), slice(290, 300))):
+            n = mine.stop - mine.start
+            want = M.attention(q[:, mine], k[:, keys], v[:, keys], 0.0625, keys.stop - keys.start - n, True)
+            most = M.attention_bound(q[:, mine], k[:, keys], 0.0625, False, False, 290) * np.abs(v).max()
+            assert np.abs(out.double().cpu().numpy()[:, mine] - want).max() <= most
+
+
 def test_f32_queries_and_strides(ctx):
     """f32 queries are rounded to fp16; token-major q and output views; no alignment beyond the type's."""
     p = Pool(ctx, 4, 2, 128, 3, most=200)
@@ -330,7 +421,7 @@ def test_what_lies_behind_a_sequence_costs_nothing(ctx, d):
 
 
 @pytest.mark.parametrize("d", [64, 128, 256])
-@pytest.mark.parametrize("rows", [[3], [40], [130]])
+@pytest.mark.parametrize("rows", [[3], [7], [10], [40], [130]])
 def test_wild_values_count_for_the_rows_that_see_them(ctx, d, rows):
     p = Pool(ctx, 4, 2, d, 1, page=16, most=160, seed=d)
     k, v = p.rows(160, 2), p.rows(160, 2)

@@ -10,7 +10,6 @@
 #include <cmath>
 #include <cstring>
 #include <new>
-#include <vector>
 
 #include "attention.hpp"
 #pragma clang diagnostic push

@@ -291,7 +291,8 @@ __device__ __forceinline__ int pg_lo_min(int v) {
 constexpr float PG_NONE = -1e30f;
 // The weight 2^d of a partial result whose maximum lies d <= 0 below the row's:
 // never 0, so that an infinite accumulator stays one (0 times it is NaN). A finite sum
-// gains by that 2^-106 of the row's at most (weights lie below 2^14).
+// gains by that 2^-105 of a key's value at most (weights lie below 2^15), where the row's
+// own sum is above 2^5.
 __device__ __forceinline__ float pg_weight(float m, float top) {
     return fmaxf(__builtin_amdgcn_exp2f(m - top), 0x1p-120f);
 }

@@ -57,18 +57,19 @@ struct DevFence {
         (void)hipGetLastError();
         return false;
     }
-    // Note device-path work just enqueued on stream s.
-    void note(hipStream_t s) {
+    // Note device-path work just enqueued on stream s. Whether it was captured: such
+    // work runs at launches that are noted nowhere.
+    bool note(hipStream_t s) {
         std::lock_guard<std::mutex> lock(mu);
         if (!s) {
             null_new = true;
-            return;
+            return false;
         }
         hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
         if (hipStreamIsCapturing(s, &st) != hipSuccess || st != hipStreamCaptureStatusNone) {
             (void)hipGetLastError();
             broad = true;
-            return;
+            return true;
         }
         if (used && s != last) {
             const hipError_t q = hipEventQuery(ev);
@@ -77,10 +78,11 @@ struct DevFence {
         }
         if (!create(ev) || !record(ev, s)) {
             broad = true;
-            return;
+            return false;
         }
         used = true;
         last = s;
+        return false;
     }
     // Order stream s after the noted work (s == nullptr: the host waits).
     hipError_t wait(hipStream_t s) {

@@ -221,6 +221,13 @@ struct PagedPool {
     int* flaw;
     size_t kv_bytes, turn_bytes;  // of one array each
     DevFence fence;               // device calls that note flaws
+    std::atomic<bool> captured{false};  // graphs hold some, whose launches the fence does not see
+
+    void note(hipStream_t s) {
+        if (fence.note(s)) captured = true;
+    }
+    // The host waits for the device calls made, and for launches of graphs that hold any.
+    hipError_t wait() { return captured ? hipDeviceSynchronize() : fence.wait(nullptr); }
 };
 
 constexpr size_t PAGED_FLAW_BYTES = 256;
@@ -413,7 +420,7 @@ void rk_npu_hip_attention_paged_pool_free(rk_npu_hip_attention_paged_pool* pool)
     PagedPool* c = as_pool(pool);
     if (!c) return;
     DeviceGuard dev(device_of(c->domain));
-    (void)c->fence.wait(nullptr);
+    (void)c->wait();
     c->fence.destroy();
     for (int i = 0; i < 2; ++i) domain_free(c->domain, c->kv[i], c->kv_bytes);
     domain_free(c->domain, c->turns, c->turn_bytes);
@@ -426,7 +433,7 @@ int rk_npu_hip_attention_paged_status(rk_npu_hip_attention_paged_pool* pool) {
     PagedPool* c = as_pool(pool);
     if (!c) return RK_NPU_ERR_PARAM;
     DeviceGuard dev(device_of(c->domain));
-    if (!dev.ok || c->fence.wait(nullptr) != hipSuccess) return RK_NPU_ERR_DEVICE;
+    if (!dev.ok || c->wait() != hipSuccess) return RK_NPU_ERR_DEVICE;
     int flaw = 0;
     const int zero = 0;
     if (hipMemcpy(&flaw, c->flaw, sizeof(flaw), hipMemcpyDeviceToHost) != hipSuccess) return RK_NPU_ERR_DEVICE;
@@ -467,7 +474,7 @@ int rk_npu_hip_attention_paged_append(rk_npu_hip_attention_paged_pool* pool, con
     P.heads_per_block = 256 * PAGED_APPEND_UNITS / (D / 16);
     hipLaunchKernelGGL(paged_append_kernel, dim3(rows, (heads + P.heads_per_block - 1) / P.heads_per_block), dim3(256), 0, s, P);
     if (hipGetLastError() != hipSuccess) return RK_NPU_ERR_DEVICE;
-    c->fence.note(s);
+    c->note(s);
     return RK_NPU_OK;
 }
 
@@ -486,7 +493,7 @@ int rk_npu_hip_attention_paged_read(rk_npu_hip_attention_paged_pool* pool, const
     hipStream_t s = static_cast<hipStream_t>(stream);
     hipLaunchKernelGGL(paged_read_kernel, dim3(batch->rows), dim3(256), 0, s, P);
     if (hipGetLastError() != hipSuccess) return RK_NPU_ERR_DEVICE;
-    c->fence.note(s);
+    c->note(s);
     return RK_NPU_OK;
 }
 
@@ -527,7 +534,7 @@ int rk_npu_hip_attention_paged_run(rk_npu_attention_f16_workspace* workspace, rk
     else
         launch_attn_paged_256(P, plan, s);
     if (hipGetLastError() != hipSuccess) return RK_NPU_ERR_DEVICE;
-    c->fence.note(s);
+    c->note(s);
     w->fence.note(s);
     return RK_NPU_OK;
 }

@@ -691,6 +691,37 @@ def test_captured_step_follows_the_lengths(ctx):
     p.pages.check()
 
 
+def test_every_launch_of_a_graph_is_told_of(ctx):
+    """check() waits for each launch of a captured call, on a stream of its own, and not only for the first."""
+    p = Pool(ctx, 4, 2, 64, 2, page=16, most=64, spare=1)
+    p.fill([20, 20])
+    table = dev(p.table)
+    b = D.PagedBatch(table, ints([20, 20]))
+    q, k, v = dev(p.rows(2, 4)), dev(p.rows(2, 2)), dev(p.rows(2, 2))
+    out, ws = torch.empty_like(q), ctx.attention_workspace(p.pages, own=True)
+
+    def step():
+        p.pages.append(b, k, v)
+        D.attention_paged(ctx, p.pages, b, q, out, ws=ws)
+    step()
+    p.pages.check()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        step()
+    p.pages.check()
+    for wrong in (True, False, True, True, False):
+        table[1, 1] = -1 if wrong else int(p.table[1, 1])
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(100_000_000)     # (the launch waits here while check() is called)
+            graph.replay()
+        if wrong:
+            with pytest.raises(npu.NpuError):
+                p.pages.check()
+        p.pages.check()
+        assert side.query()
+
+
 def test_prompt_then_decode(ctx):
     """Prompts in ragged pieces, then drafts, then single tokens, rotated on the way:
     attention over what the pages hold, and what they hold over the whole run."""

@@ -87,7 +87,7 @@ typedef struct rk_npu_hip_attention_paged_pool rk_npu_hip_attention_paged_pool;
 typedef struct rk_npu_hip_paged_batch {
     int32_t sequences;          /* 1..RK_NPU_HIP_PAGED_MAX_SEQUENCES */
     int32_t rows;               /* rows of the call's arrays, 1..RK_NPU_HIP_PAGED_MAX_ROWS */
-    int32_t max_rows;           /* no sequence has more rows; 1 without row_offsets */
+    int32_t max_rows;           /* no sequence has more rows: 1..rows, 1 without row_offsets */
     int32_t max_tokens;         /* no sequence is longer: 1..table_stride x page, max_capacity at most */
     const int32_t* lengths;     /* [sequences]: tokens, the call's rows among them */
     const int32_t* row_offsets; /* [sequences + 1], or NULL: a row each, rows >= sequences */

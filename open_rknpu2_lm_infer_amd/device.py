@@ -321,7 +321,7 @@ class PagedBatch:
             raise NpuError(f"the table holds {most} tokens a sequence, max_tokens is {tokens}")
         if rows >= 2 ** 31:
             int32(rows, "rows")
-        return F.rk_npu_hip_paged_batch(self.sequences, rows, self.max_rows, tokens, *self._at)
+        return F.rk_npu_hip_paged_batch(self.sequences, rows, min(self.max_rows, rows), tokens, *self._at)
 
 
 class KvPages:

@@ -124,6 +124,14 @@ def test_batches():
             build()
 
 
+def test_more_rows_allowed_than_there_are():
+    """max_rows is a bound: the call's rows are another."""
+    b = D.PagedBatch(Ints(3, 50), Ints(3), Ints(4), max_rows=512)
+    assert [b._raw(n, 16).max_rows for n in (1, 300, 512, 700)] == [1, 300, 512, 512]
+    for n in (0, -1):
+        assert D.PagedBatch(Ints(3, 50), Ints(3), Ints(4), max_rows=n)._raw(300, 16).max_rows == n    # (refused by the call)
+
+
 @pytest.mark.parametrize("n", [2 ** 31, 2 ** 32 + 5, -2 ** 31 - 1])
 @pytest.mark.parametrize("name", ["query_heads", "kv_heads", "head_dim", "pages", "page", "capacity", "rotary_dim"])
 def test_numbers_beyond_32_bits(name, n):

@@ -269,6 +269,25 @@ def test_long_lengths_are_split_and_joined(ctx, d, qh, kh, lengths, rows):
         p.attend(rows, dtype=dtype, max_tokens=max(lengths))
 
 
+@pytest.mark.parametrize("rows", [[1, 0], [3, 4], [100, 57]])
+def test_more_rows_allowed_than_there_are(ctx, rows):
+    """A batch whose max_rows passes the call's rows: append, read and attention."""
+    p = Pool(ctx, 4, 2, 64, 2, page=16, most=200)
+    p.fill([30, 20])
+    k, v = p.rows(sum(rows), 2), p.rows(sum(rows), 2)
+    lengths = [a + n for a, n in zip(p.lengths(), rows)]
+    b = p.batch(rows, lengths, max_rows=512)
+    p.pages.append(b, dev(k), dev(v))
+    got = [torch.empty(2, sum(rows), 64, dtype=torch.float16, device="cuda") for _ in range(2)]
+    p.pages.read(b, *got)
+    assert np.array_equal(got[0].cpu().numpy(), k) and np.array_equal(got[1].cpu().numpy(), v)
+    for s, at in enumerate((0, rows[0])):
+        p.k[s] = np.concatenate([p.k[s], k[:, at:at + rows[s]]], axis=1)
+        p.v[s] = np.concatenate([p.v[s], v[:, at:at + rows[s]]], axis=1)
+    for dtype in (torch.float32, torch.float16):
+        p.attend(rows, dtype=dtype, max_rows=512)
+
+
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("causal", [True, False])
 def test_drafts(ctx, d, causal):

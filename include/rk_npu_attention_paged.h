@@ -77,7 +77,8 @@ typedef struct rk_npu_hip_attention_paged_config {
     int32_t rotary_dim;                    /* dims rotated, a multiple of 16 up to head_dim; 0: none */
     int32_t interleaved;                   /* 0: pairs (j, j + rotary_dim / 2); 1: pairs (2j, 2j + 1) */
     double rope_theta;                     /* frequency[j] = rope_theta^(-2j / rotary_dim), where frequencies is NULL */
-    const double* frequencies;             /* rotary_dim / 2 of them, radians per position; read by create only */
+    const double* frequencies;             /* rotary_dim / 2 of them, radians per position (below 2^995, as
+                                              rope_theta's are); read by query and create only */
 } rk_npu_hip_attention_paged_config;
 
 typedef struct rk_npu_hip_attention_paged_pool rk_npu_hip_attention_paged_pool;

@@ -237,15 +237,21 @@ static PagedPool* as_pool(const void* p) {
     return (c && c->magic == MAGIC_PAGED_POOL) ? c : nullptr;
 }
 
+// Turns (radians / 2 pi) of pair j per position.
+static double paged_turns(const rk_npu_hip_attention_paged_config& c, int j) {
+    const double around = 6.283185307179586476925286766559;
+    return (c.frequencies ? c.frequencies[j] : std::pow(c.rope_theta, -2.0 * j / c.rotary_dim)) / around;
+}
+
 static bool valid_paged(const rk_npu_hip_attention_paged_config* c) {
     if (!c || !valid_config(&c->attention)) return false;
     if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128 && c->page != 256) return false;
     if (c->rotary_dim < 0 || c->rotary_dim > c->attention.head_dim || c->rotary_dim % 16) return false;
     if (c->interleaved != 0 && c->interleaved != 1) return false;
     if (c->rotary_dim > 0 && !c->frequencies && !(std::isfinite(c->rope_theta) && c->rope_theta > 0.0)) return false;
-    if (c->rotary_dim > 0 && c->frequencies)
-        for (int i = 0; i < c->rotary_dim / 2; ++i)
-            if (!std::isfinite(c->frequencies[i])) return false;
+    // (the angles of all 32-bit positions are finite)
+    for (int j = 0; j < c->rotary_dim / 2; ++j)
+        if (!std::isfinite(paged_turns(*c, j) * 0x1p31)) return false;
     // (kernels count the pool's 16-token tiles in 32 bits)
     return c->pages >= 1 && (int64_t)c->pages * c->attention.kv_heads * (c->page / 16) <= INT_MAX &&
            c->attention.max_capacity <= RK_NPU_HIP_PAGED_MAX_TOKENS;
@@ -393,9 +399,7 @@ int rk_npu_hip_attention_paged_pool_create(rk_npu_iommu_domain* domain,
     const int pairs = config->rotary_dim / 2;
     c->turn_bytes = std::max<size_t>(1, pairs) * sizeof(double);
     double turns[128];
-    const double around = 6.283185307179586476925286766559;
-    for (int j = 0; j < pairs; ++j)
-        turns[j] = (config->frequencies ? config->frequencies[j] : std::pow(config->rope_theta, -(double)j / pairs)) / around;
+    for (int j = 0; j < pairs; ++j) turns[j] = paged_turns(*config, j);
     auto* raw = reinterpret_cast<rk_npu_hip_attention_paged_pool*>(c);
     c->flaw = static_cast<int*>(domain_alloc(d, PAGED_FLAW_BYTES));
     c->turns = c->flaw ? static_cast<double*>(domain_alloc(d, c->turn_bytes)) : nullptr;

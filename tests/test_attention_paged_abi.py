@@ -67,6 +67,20 @@ def test_refused_configurations():
     assert F.lib().rk_npu_hip_attention_paged_query(None, ctypes.byref(F.rk_npu_attention_f16_sizes())) == F.RK_NPU_ERR_PARAM
 
 
+def test_frequencies_whose_angles_pass_64_bits():
+    """An angle that is not finite at a 32-bit position would make NaN of a row: refused. (2^31
+    positions of 5.2e299 radians, in turns, are the largest number of 64 bits.)"""
+    for theta in (5e-324, 1e-310, 1e-306):
+        assert query(config(rotary=128, rope_theta=theta))[0] == F.RK_NPU_ERR_PARAM, theta
+    for theta in (1e-301, 1e-3, 1.0, 1e300, 1.7e308):
+        assert query(config(rotary=128, rope_theta=theta))[0] == F.RK_NPU_OK, theta
+    assert query(config(rotary=16, rope_theta=1e-320))[0] == F.RK_NPU_OK    # (at most theta^(-7/8))
+    for value, rc in ((1.7e308, F.RK_NPU_ERR_PARAM), (-1e300, F.RK_NPU_ERR_PARAM), (1e298, F.RK_NPU_OK), (-1e298, F.RK_NPU_OK)):
+        cfg = config(rotary=16)
+        cfg.frequencies = (ctypes.c_double * 8)(*([1.0] * 7 + [value]))
+        assert query(cfg)[0] == rc, value
+
+
 def test_null_handles():
     """Every call on no pool, and on memory that is no pool."""
     L, cfg = F.lib(), config()

@@ -297,6 +297,12 @@ __device__ __forceinline__ float pg_weight(float m, float top) {
     return fmaxf(__builtin_amdgcn_exp2f(m - top), 0x1p-120f);
 }
 
+// A mean of fp16 values lies in their range. One whose weights are rounded to one fp16
+// after they are summed may pass its end by 2^-11, where fp16 has infinities: it is that end.
+__device__ __forceinline__ float pg_in_range(float y) {
+    return fabsf(y) < INFINITY ? __builtin_amdgcn_fmed3f(y, -65504.0f, 65504.0f) : y;
+}
+
 // 8 consecutive outputs of any alignment.
 __device__ __forceinline__ void pg_store8(const AttnPagedParams& P, long long at, const float (&y)[8]) {
     if (P.out_f16) {
@@ -985,10 +991,14 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_tile_kernel(AttnPagedParam
     // Infinities and NaN among the values: the products leave NaN of them (0, or a
     // negative second fp16, times an infinity). A result that they reach is their sum,
     // whatever the weights, which are positive. (Lane: dims W n + 8 b + 4 hi..+3.)
+    float most = 0.0f;
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int k = 0; k < CL; ++k) wild |= !(fabsf(o[n][k]) < INFINITY);
+        for (int k = 0; k < CL; ++k) {
+            wild |= !(fabsf(o[n][k]) < INFINITY);
+            most = fmaxf(most, fabsf(o[n][k]));
+        }
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(wild) != 0, 0)) {
 #pragma unroll 1
         for (int n = 0; n < NB; ++n) {
@@ -1013,7 +1023,14 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_tile_kernel(AttnPagedParam
     // Rows leave 32 dims at a time through LDS, so that 8 lanes store a row's 128 bytes:
     // 16-byte pieces, piece p of row r at place p ^ (r & 7).
     __syncthreads();
-    const float il = I.splits > 1 ? 1.0f : lim == 0 ? 0.0f : 1.0f / lsum;
+    float il = I.splits > 1 ? 1.0f : lim == 0 ? 0.0f : 1.0f / lsum;
+    if (!SPLIT && I.splits == 1 && __builtin_expect(__builtin_amdgcn_ballot_w64(wild || most * il > 65504.0f) != 0, 0)) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int k = 0; k < CL; ++k) o[n][k] = pg_in_range(o[n][k] * il);
+        il = 1.0f;
+    }
     const size_t part_at = ((size_t)at * B.kh + g) * ROWS + W * wave;
     if (I.splits > 1 && hi == 0 && live)
         *reinterpret_cast<float2*>(P.part + (size_t)P.items * B.kh * ROWS * D + (part_at + lo) * 2) = float2{mrun, lsum};
@@ -1134,6 +1151,7 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(AttnPagedParams P)
     const int rr = I.tile * P.tile_rows + row, r = rr / G, h = rr - r * G;
     const bool empty = P.causal ? I.len - I.n + r + 1 <= 0 : I.len == 0;
     num *= empty ? 0.0f : 1.0f / den;
+    if (P.out_f16) num = pg_f4{pg_in_range(num[0]), pg_in_range(num[1]), pg_in_range(num[2]), pg_in_range(num[3])};
     pg_store4(P, (long long)(g * G + h) * P.o_head + (long long)(I.row + r) * P.o_row + 4 * d4, num[0], num[1], num[2], num[3]);
 }
 

@@ -94,3 +94,25 @@ def test_a_maximum_that_jumps(ctx, d, causal, dtype):
     q, held = jumping(ctx, d, causal, 31, d + 1)   # (an odd number of units, split)
     for rows in (8, 20):
         held.check(q[:, :, :rows], dtype, max_tokens=992)
+
+
+# --- values at the end of fp16's range -----------------------------------------------
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_the_largest_values(ctx, d, causal):
+    """Keys of like weight, which rounds up by nearly half a step, and values of 65504 and
+    -65504: a mean of finite values is finite."""
+    tokens = 400
+    k = np.zeros((2, 2, tokens, d), np.float16)
+    k[..., 0] = np.log2(1.0 + 1.03 * 2.0 ** -11)
+    v = np.full((2, 2, tokens, d), 65504.0, np.float16)
+    v[..., ::2] *= -1
+    v[..., 5] = 1.0
+    q = np.zeros((2, 8, 20, d), np.float16)
+    q[..., 0] = 1.0
+    held = Held(ctx, 8, k, v, B.SCALE, causal=causal)
+    for dtype in (F32, F16):
+        for rows in (1, 4, 8, 20):
+            for most in (400, 8192):
+                held.check(q[:, :, :rows], dtype, max_tokens=most)

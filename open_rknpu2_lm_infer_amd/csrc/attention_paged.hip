@@ -332,6 +332,13 @@ static bool paged_same_geometry(const AttnWork* w, const PagedPool* c) {
 // 66, 64 and 64; 12 x 5 rows 64 with one, 62 with four). A split holds a unit a wave at
 // least: one sequence of 4000 tokens 12.7 and 13.3 with two, 16 with four. Tile kernel: as many as stay on a CU; 8 units at least:
 // 128 rows of 256 dims after 3600 tokens 35, with 16 units 44, with 24 50.
+//
+// Rows kernel, more sequences than blocks to aim at (128 of 8 KV heads): where one may be
+// longer than 4096 tokens, further splits of long ones follow the sequences' own blocks, as
+// many as are aimed at, of 32 units at least (256 sequences of 300 to 700 tokens and one of
+// 131072 188 and unsplit 1450, of 8192 101 and 146, of 4096 99 and 103; none longer, but
+// allowed, 88 and 85; 200 of up to 8100 557 and 580; 1000 of 16 heads over 8 of 64 with a long one 250 and 965,
+// without 190 and 170).
 static PagedPlan paged_plan(AttnPagedParams& P, int D) {
     const PagedBatch& B = P.b;
     const int G = P.qh / B.kh, cus = device_cus();
@@ -341,18 +348,27 @@ static PagedPlan paged_plan(AttnPagedParams& P, int D) {
         return std::min<int64_t>(B.sequences * ((R + rows - 1) / rows), (int64_t)B.rows * G / rows + B.sequences);
     };
     const int units = (B.max_tokens + 31) / 32;
-    const PagedPlan plan{R > (D == 256 ? 16 : 32), D < 256 && units > 128 ? 2 : 1};
+    PagedPlan plan{R > (D == 256 ? 16 : 32), D < 256 && units > 128 ? 2 : 1, false};
     P.tile_rows = plan.tile ? 128 * plan.units : R <= 8 ? 8 : R <= 16 ? 16 : 32;
     P.tiles = (int)tiles(P.tile_rows);
     P.least = plan.tile ? 8 : 4;
     P.target = 0;
     const int blocks = plan.tile ? (plan.units == 1 && D < 256 ? 2 : 1) : B.sequences > 4 ? 4 : 1;
     // (as many as the workspace holds partials for)
-    const int64_t room = (int64_t)(attn_partial_rows(D) / ((size_t)B.kh * P.tile_rows)) - P.tiles;
-    const int want = (int)std::min<int64_t>(std::max(1, blocks * cus / B.kh), room);
+    const int64_t slots = (int64_t)(attn_partial_rows(D) / ((size_t)B.kh * P.tile_rows));
+    const int aim = std::max(1, blocks * cus / B.kh), want = (int)std::min<int64_t>(aim, slots - P.tiles);
     // (units are added up in 32 bits)
-    if (units > 16 && P.tiles < want && (int64_t)P.tiles * units < (1 << 30)) P.target = want;
-    P.items = P.target ? P.tiles + want : P.tiles;
+    if (units > 16 && (int64_t)P.tiles * units < (1 << 30)) {
+        if (P.tiles < want) {
+            P.target = want;
+        } else if (!plan.tile && units > 128) {
+            plan.behind = true;
+            P.least = 32;
+            P.target = (int)std::min<int64_t>(aim, slots / 2);
+        }
+    }
+    P.items = P.target ? P.tiles + P.target : P.tiles;
+    P.slots = plan.behind ? 2 * P.target : P.items;
     P.wave = plan.tile && P.causal ? std::max(1, cus / B.kh) : 0;
     return plan;
 }

@@ -101,10 +101,11 @@ struct AttnPagedParams {
     void* out;
     int out_f16;
     long long o_head, o_row;
-    float* part;     // accumulators [item][kh][tile rows][D], then (max, sum) pairs
+    float* part;     // accumulators [slot][kh][tile rows][D], then (max, sum) pairs
     int qh, causal;
     float scale;
     int items;       // blocks per KV head
+    int slots;       // of partials per KV head
     int target;      // blocks per KV head that splits aim at; 0: no splits
     int least;       // units of a split, at least
     int tile_rows;   // query rows of a block
@@ -123,11 +124,75 @@ __device__ __forceinline__ int pg_scan(int v) {  // inclusive, over the wave
 }
 
 // One block's work: row tile `tile` of a sequence, split `split` of `splits` of its
-// keys; `item`: the sequence's first block of that tile.
+// keys. Partials of split 0 of that tile lie in slot `first`, of split i > 0 in `more` + i.
 struct PagedItem {
-    int s, row, n, len, tile, split, splits, item;
+    int s, row, n, len, tile, split, splits, first, more;
     bool any;
 };
+
+// The schedule where sequences of few rows are more than the blocks that splits aim at:
+// block s has sequence s, or its first split, blocks from B.sequences on have the further
+// splits of long ones: more than P.least units, and more than the batch's units over
+// P.target. Who has P.least at most looks at no other sequence. Slots: further splits in
+// their order, then, P.target behind each sequence's second one, the first ones. (A join's
+// tile is a sequence.)
+__device__ __forceinline__ PagedItem pg_item_behind(const AttnPagedParams& P, int at, int lane) {
+    const PagedBatch& B = P.b;
+    auto units_of = [](const PagedSeq& q) { return q.n > 0 ? (q.len + 31) >> 5 : 0; };
+    PagedItem x{};
+    PagedSeq own{0, 0, 0};
+    if (at < B.sequences) {
+        own = pg_seq(B, at);
+        x.s = at;
+        x.row = own.row;
+        x.n = own.n;
+        x.len = own.len;
+        x.splits = 1;
+        x.any = own.n > 0;
+        if (units_of(own) <= P.least) return x;
+    }
+    const int C = (B.sequences + 63) >> 6, end = min(lane * C + C, B.sequences);
+    int units = 0;
+#pragma unroll 4
+    for (int s = lane * C; s < end; ++s) units += units_of(pg_seq(B, s));
+    const unsigned total = __builtin_amdgcn_readlane(pg_scan(units), 63);
+    const unsigned per = max((unsigned)P.least, (total + P.target - 1) / (unsigned)P.target);
+    auto more_of = [&](const PagedSeq& q) {
+        return min(PAGED_MAX_SPLITS, max(1, (int)(((unsigned)units_of(q) + per - 1) / per))) - 1;
+    };
+    int more = 0;
+#pragma unroll 4
+    for (int s = lane * C; s < end; ++s) more += more_of(pg_seq(B, s));
+    const int more_end = pg_scan(more);
+    int k = 0, owner, before;
+    if (at < B.sequences) {
+        owner = at / C;
+        before = __builtin_amdgcn_readlane(more_end - more, owner);
+        for (int s = owner * C; s < at; ++s) before += more_of(pg_seq(B, s));
+    } else {
+        k = at - B.sequences;
+        const unsigned long long over = __builtin_amdgcn_ballot_w64(more_end > k);
+        if (over == 0) return x;
+        owner = __builtin_ctzll(over);
+        before = __builtin_amdgcn_readlane(more_end - more, owner);
+        for (x.s = owner * C; x.s < B.sequences; ++x.s) {
+            own = pg_seq(B, x.s);
+            if (k < before + more_of(own)) break;
+            before += more_of(own);
+        }
+        x.split = 1 + k - before;
+        x.row = own.row;
+        x.n = own.n;
+        x.len = own.len;
+    }
+    x.splits = 1 + more_of(own);
+    x.first = P.target + before;
+    x.more = before - 1;
+    // (not so if the lengths changed meanwhile)
+    x.any = x.s < B.sequences && x.splits > x.split && before < P.target && x.more + x.splits <= P.target;
+    if (x.splits == 1) x.any = at < B.sequences;
+    return x;
+}
 
 // The schedule, made by every wave from the lengths alone: a sequence has ceil(rows /
 // tile_rows) tiles, each split into as many pieces of at least `per` units of 32 keys
@@ -151,7 +216,6 @@ __device__ __forceinline__ PagedItem pg_item(const AttnPagedParams& P, int at, i
         x.n = q.n;
         x.len = q.len;
         x.splits = 1;
-        x.item = at;
         return x;
     }
     PagedSeq mine = lane * C < B.sequences ? pg_seq(B, lane * C) : none;
@@ -240,7 +304,7 @@ __device__ __forceinline__ PagedItem pg_item(const AttnPagedParams& P, int at, i
             const int k = joins ? in : in / p;
             x.tile = t - 1 - k;
             x.split = joins ? 0 : in - k * p;
-            x.item = first + k * p;
+            x.first = x.more = first + k * p;
             return x;
         }
         before += count;
@@ -366,7 +430,7 @@ constexpr float PG_LAZY = 4.0f, PG_SHIFT = 10.0f;
 // unit's loads and products, the waves' meeting (7.6), the join (4.7). The next unit's
 // loads before this one's products changed nothing with 128 dims and lost with 256 (51 to
 // 57: registers).
-template <int D, int NW, int RW, bool PACK>
+template <int D, int NW, int RW, bool PACK, bool BEHIND>
 __global__ __launch_bounds__(64 * NW) void attn_paged_rows_kernel(AttnPagedParams P) {
     constexpr int KS = D / 32;                  // 32-dim steps of a score
     constexpr int DW = D == 64 ? 4 : 8;         // dims of V a lane takes of a key, H times
@@ -380,7 +444,7 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_rows_kernel(AttnPagedParam
     const int g = blockIdx.x % B.kh, at = blockIdx.x / B.kh;
     const int lane = threadIdx.x & 63, lo = lane & 15, hi = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const PagedItem I = pg_item(P, at, lane, false);
+    const PagedItem I = BEHIND ? pg_item_behind(P, at, lane) : pg_item(P, at, lane, false);
     if (!I.any) return;  // (block-uniform)
     const int G = P.qh / B.kh, R = G * I.n;
     int lim[RW];
@@ -658,12 +722,12 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_rows_kernel(AttnPagedParam
             for (int k = 0; k < 8; ++k) y[k] *= il;
             pg_store8(P, (long long)(g * G + h) * P.o_head + (long long)(I.row + r) * P.o_row + d, y);
         } else {
-            const size_t row_at = ((size_t)at * B.kh + g) * COLS + row;
+            const size_t row_at = ((size_t)(I.split ? I.more + I.split : I.first) * B.kh + g) * COLS + row;
             float* p = P.part + row_at * D + d;
             *reinterpret_cast<pg_f4*>(p) = pg_f4{y[0], y[1], y[2], y[3]};
             *reinterpret_cast<pg_f4*>(p + 4) = pg_f4{y[4], y[5], y[6], y[7]};
             if (d == 0)
-                *reinterpret_cast<float2*>(P.part + (size_t)P.items * B.kh * COLS * D + row_at * 2) = float2{top, l};
+                *reinterpret_cast<float2*>(P.part + (size_t)P.slots * B.kh * COLS * D + row_at * 2) = float2{top, l};
         }
     }
 }
@@ -1033,7 +1097,7 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_tile_kernel(AttnPagedParam
     }
     const size_t part_at = ((size_t)at * B.kh + g) * ROWS + W * wave;
     if (I.splits > 1 && hi == 0 && live)
-        *reinterpret_cast<float2*>(P.part + (size_t)P.items * B.kh * ROWS * D + (part_at + lo) * 2) = float2{mrun, lsum};
+        *reinterpret_cast<float2*>(P.part + (size_t)P.slots * B.kh * ROWS * D + (part_at + lo) * 2) = float2{mrun, lsum};
     const long long own = I.splits > 1 ? (long long)(part_at + lo) * D
                                        : (long long)(g * G + h) * P.o_head + (long long)(I.row + r) * P.o_row;
     uint8_t* const box = smem + wave * (W * 128);
@@ -1078,7 +1142,7 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_tile_kernel(AttnPagedParam
 //
 // Measured: one row of 32 heads, 32 splits 4.7 us; 2048 rows of 8 heads, 4 splits (33 MB
 // read) 11 (36 with a block a row).
-template <int D, int RPB>
+template <int D, int RPB, bool BEHIND>
 __global__ __launch_bounds__(256) void attn_paged_join_kernel(AttnPagedParams P) {
     constexpr int T = 256 / RPB, LD = D / 4, GS = T / LD, AHEAD = 8, W = PAGED_MAX_SPLITS / T;
     static_assert(GS >= 1 && T % LD == 0 && T >= 16, "threads per row");
@@ -1087,24 +1151,26 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(AttnPagedParams P)
     __shared__ pg_f4 part[RPB][GS][LD];
     const PagedBatch& B = P.b;
     const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-    const PagedItem I = pg_item(P, blockIdx.y, lane, true);
+    const PagedItem I = BEHIND ? pg_item_behind(P, blockIdx.y, lane) : pg_item(P, blockIdx.y, lane, true);
     // (a block past the grid of the batch's wrong offsets has written nothing)
-    if (!I.any || I.splits == 1 || I.item + I.splits > P.items) return;
+    if (!I.any || I.splits == 1 || I.more + I.splits > P.slots) return;
     const int G = P.qh / B.kh, R = min(G * I.n - I.tile * P.tile_rows, P.tile_rows), row0 = blockIdx.z * RPB;
     if (row0 >= R) return;  // (block-uniform)
     const int mine = tid / T, t = tid % T, d4 = t % LD, gs = t / LD, S = I.splits;
     const int row = min(row0 + mine, R - 1);  // (threads past the last row: that row again, not written)
-    const size_t step = (size_t)B.kh * P.tile_rows, at = ((size_t)I.item * B.kh + g) * P.tile_rows + row;
-    const pg_f4* acc = reinterpret_cast<const pg_f4*>(P.part + at * D) + d4;
+    // (split i's row lies i steps from that of slot `more`, the first one's `zero`)
+    const long long step = (long long)B.kh * P.tile_rows, at = ((long long)I.more * B.kh + g) * P.tile_rows + row;
+    const long long zero = (long long)(I.first - I.more) * step;
+    const pg_f4* acc = reinterpret_cast<const pg_f4*>(P.part) + at * LD + d4;
     pg_f4 v[AHEAD];
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) v[i] = acc[(size_t)min(gs + i * GS, S - 1) * step * LD];
-    const float2* ml = reinterpret_cast<const float2*>(P.part + (size_t)P.items * step * D) + at;
+    for (int i = 0; i < AHEAD; ++i) v[i] = acc[(i || gs ? min(gs + i * GS, S - 1) * step : zero) * LD];
+    const float2* ml = reinterpret_cast<const float2*>(P.part + (size_t)P.slots * step * D) + at;
     float2 x[W];
     float top = PG_NONE;
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-        x[i] = t + i * T < S ? ml[(size_t)(t + i * T) * step] : float2{PG_NONE, 0.0f};
+        x[i] = t + i * T < S ? ml[i || t ? (t + i * T) * step : zero] : float2{PG_NONE, 0.0f};
         top = fmaxf(top, x[i].x);
     }
 #pragma unroll
@@ -1137,7 +1203,7 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(AttnPagedParams P)
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
             if (s + i * GS < S) num += v[i] * weight[mine][s + i * GS];
-            v[i] = acc[(size_t)min(s + (AHEAD + i) * GS, S - 1) * step * LD];
+            v[i] = acc[min(s + (AHEAD + i) * GS, S - 1) * step * LD];
         }
     }
     if constexpr (GS > 1) {
@@ -1156,10 +1222,12 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(AttnPagedParams P)
 }
 
 // The kernel of a run: attn_paged_tile_kernel in stages of `units` units, or
-// attn_paged_rows_kernel, whose tiles hold all rows of a sequence.
+// attn_paged_rows_kernel, whose tiles hold all rows of a sequence; behind: the latter with
+// the schedule of pg_item_behind.
 struct PagedPlan {
     bool tile;
     int units;
+    bool behind;
 };
 
 void launch_attn_paged_64(const AttnPagedParams& P, const PagedPlan& plan, hipStream_t s);
@@ -1176,33 +1244,41 @@ static void launch_attn_paged_tile(const AttnPagedParams& P, hipStream_t s) {
         hipLaunchKernelGGL((attn_paged_tile_kernel<D, W, U, NW, true>), grid, block, 0, s, P);
 }
 
-template <int D>
+template <int D, bool BEHIND>
 static void launch_attn_paged_rows(const AttnPagedParams& P, hipStream_t s) {
     const dim3 grid(P.b.kh * P.items), block(256);
     if (P.tile_rows == 8)
-        hipLaunchKernelGGL((attn_paged_rows_kernel<D, 4, 1, true>), grid, block, 0, s, P);
+        hipLaunchKernelGGL((attn_paged_rows_kernel<D, 4, 1, true, BEHIND>), grid, block, 0, s, P);
     else if (P.tile_rows == 16)
-        hipLaunchKernelGGL((attn_paged_rows_kernel<D, 4, 1, false>), grid, block, 0, s, P);
+        hipLaunchKernelGGL((attn_paged_rows_kernel<D, 4, 1, false, BEHIND>), grid, block, 0, s, P);
     else if constexpr (D < 256)
-        hipLaunchKernelGGL((attn_paged_rows_kernel<D, 4, 2, false>), grid, block, 0, s, P);
+        hipLaunchKernelGGL((attn_paged_rows_kernel<D, 4, 2, false, BEHIND>), grid, block, 0, s, P);
+}
+
+template <int D, bool BEHIND>
+static void launch_attn_paged_join(const AttnPagedParams& P, hipStream_t s) {
+    // (many rows: as many a block as leave a row the threads for its dims)
+    constexpr int MANY = 1024 / D < 8 ? 1024 / D : 8;
+    if (P.tiles * P.tile_rows * P.b.kh >= 1024)
+        hipLaunchKernelGGL((attn_paged_join_kernel<D, MANY, BEHIND>), dim3(P.b.kh, P.tiles, P.tile_rows / MANY), dim3(256), 0, s, P);
+    else
+        hipLaunchKernelGGL((attn_paged_join_kernel<D, 1, BEHIND>), dim3(P.b.kh, P.tiles, P.tile_rows), dim3(256), 0, s, P);
 }
 
 template <int D>
 static void launch_attn_paged(const AttnPagedParams& P, const PagedPlan& plan, hipStream_t s) {
+    if (plan.behind) {
+        launch_attn_paged_rows<D, true>(P, s);
+        launch_attn_paged_join<D, true>(P, s);
+        return;
+    }
     if (!plan.tile)
-        launch_attn_paged_rows<D>(P, s);
+        launch_attn_paged_rows<D, false>(P, s);
     else if (D < 256 && plan.units == 2)
         launch_attn_paged_tile<D, D < 256 ? 2 : 1>(P, s);
     else
         launch_attn_paged_tile<D, 1>(P, s);
-    if (P.target) {
-        // (many rows: as many a block as leave a row the threads for its dims)
-        constexpr int MANY = 1024 / D < 8 ? 1024 / D : 8;
-        if (P.tiles * P.tile_rows * P.b.kh >= 1024)
-            hipLaunchKernelGGL((attn_paged_join_kernel<D, MANY>), dim3(P.b.kh, P.tiles, P.tile_rows / MANY), dim3(256), 0, s, P);
-        else
-            hipLaunchKernelGGL((attn_paged_join_kernel<D, 1>), dim3(P.b.kh, P.tiles, P.tile_rows), dim3(256), 0, s, P);
-    }
+    if (P.target) launch_attn_paged_join<D, false>(P, s);
 }
 
 }  // namespace hm

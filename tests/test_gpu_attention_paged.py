@@ -333,6 +333,138 @@ def test_many_sequences_split(ctx):
     p.attend([int(x) for x in p.rng.integers(0, 30, 150)])
 
 
+class Shared:
+    """Many sequences over the pages of one, each as long as it says."""
+
+    def __init__(self, ctx, qh, kh, d, sequences, tokens, most=5000, causal=True):
+        self.p = Pool(ctx, qh, kh, d, 1, page=64, most=most, causal=causal, seed=d + sequences)
+        self.p.fill([tokens])
+        self.table = dev(self.p.table).expand(sequences, -1).contiguous()
+        self.lengths = torch.zeros(sequences, dtype=torch.int32, device="cuda")
+
+    def attend(self, rows, lengths, dtype, out=None, run=True, max_tokens=5000):
+        """rows: of each sequence (None: a row each, no offsets). Only checks where not run."""
+        p, each = self.p, [1] * len(lengths) if rows is None else rows
+        begins = np.concatenate([[0], np.cumsum(each)])
+        if run:
+            self.lengths.copy_(ints(lengths))
+            offsets = None if rows is None else ints(begins.tolist())
+            self.b = D.PagedBatch(self.table, self.lengths, offsets, max_rows=max(each), max_tokens=max_tokens)
+            self.q = p.rows(int(begins[-1]), p.qh)
+            out = torch.full((p.qh, int(begins[-1]), p.d), 77.0, dtype=dtype, device="cuda")
+            D.attention_paged(p.ctx, p.pages, self.b, dev(self.q), out)
+            p.pages.check()
+        # paged_model's attention and bound, in 64 bits on the GPU
+        half, group = out.dtype == torch.float16, p.qh // p.kh
+        one = half and max(each) * group > (16 if p.d == 256 else 32)
+        most = M.attention_bound(self.q, p.k[0], p.scale, half, one, max(lengths)) * np.abs(p.v[0]).max()
+        k, v = (dev(a[0]).double() for a in (p.k, p.v))
+        q, got = dev(self.q).double(), out.double()
+        for s, (n, length) in enumerate(zip(each, lengths)):
+            mine = slice(int(begins[s]), int(begins[s]) + n)
+            if n == 0 or length == 0:
+                assert bool((got[:, mine] == 0.0).all())
+                continue
+            scores = p.scale * torch.matmul(q[:, mine].reshape(p.kh, group * n, p.d), k[:, :length].transpose(1, 2).contiguous())
+            scores = scores.view(p.kh, group, n, length)
+            if p.causal:
+                seen = torch.arange(length - n, length, device="cuda")
+                scores.masked_fill_(torch.arange(length, device="cuda")[None, :] > seen[:, None], -np.inf)
+            weights = torch.softmax(scores, dim=-1).nan_to_num_(0.0)     # (rows that see no token)
+            want = torch.matmul(weights.view(p.kh, group * n, length), v[:, :length]).view(p.qh, n, p.d)
+            err = float((got[:, mine] - want).abs().max())
+            assert err <= most, f"sequence {s}: {err} > {most}"
+        return out
+
+
+@pytest.mark.parametrize("d,qh,kh,sequences,rows", [
+    (64, 32, 32, 33, 1), (128, 32, 32, 40, 1), (64, 64, 32, 70, 3), (256, 32, 32, 36, 1), (128, 16, 16, 66, 2), (64, 16, 8, 130, 1),
+    (128, 64, 32, 34, 5), (256, 32, 16, 65, 5)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_long_sequences_among_many(ctx, causal, d, qh, kh, sequences, rows):
+    """More sequences than the blocks that splits aim at: one long, some, at the border of
+    being split, all of them, none; idle ones and ones of no rows among them."""
+    x = Shared(ctx, qh, kh, d, sequences, 2100, causal=causal)
+    rng = np.random.default_rng(sequences)
+    few = [int(n) for n in rng.integers(0, 70, sequences)]
+    for where in ([sequences - 1], [0, 1, 20], [sequences // 2, 5, 31, 32], range(0, sequences, 5), []):
+        lengths = list(few)
+        for i, s in enumerate(where):
+            lengths[s] = (2100, 1025, 1024, 2049, 1057, 2048)[i % 6]
+        for dtype in (torch.float32, torch.float16):
+            x.attend(None if rows == 1 else [int(n) for n in rng.integers(0, rows + 1, sequences - 1)] + [rows], lengths, dtype)
+    lengths = [1200 - 7 * i for i in range(sequences)]
+    x.attend(None if rows == 1 else [rows] * sequences, lengths, torch.float16)
+
+
+def test_a_long_sequence_among_a_thousand(ctx):
+    x = Shared(ctx, 8, 8, 64, 1024, 9000, most=9000)
+    rng = np.random.default_rng(0)
+    for where in ([1023], [0, 1, 500], []):
+        lengths = [int(n) for n in rng.integers(0, 50, 1024)]
+        for s in where:
+            lengths[s] = 9000 - s
+        x.attend(None, lengths, torch.float32, max_tokens=9000)
+        x.attend([int(n) for n in rng.integers(0, 3, 1023)] + [2], lengths, torch.float16, max_tokens=9000)
+
+
+def test_a_captured_step_of_many_follows_the_long_ones(ctx):
+    """One captured step whose long sequences come and go, and one of a wrong length."""
+    x = Shared(ctx, 32, 32, 64, 40, 5000)
+    p, ws = x.p, ctx.attention_workspace(x.p.pages, own=True)
+    x.attend(None, [30] * 40, torch.float32)
+    q, out = dev(x.q), torch.zeros(32, 40, 64, device="cuda")
+    D.attention_paged(ctx, p.pages, x.b, q, out, ws=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        D.attention_paged(ctx, p.pages, x.b, q, out, ws=ws)
+    for i in range(6):
+        lengths = [(7 * s + i) % 60 for s in range(40)]
+        for s in range(i):
+            lengths[(11 * s + i) % 40] = 5000 - 600 * s
+        x.lengths.copy_(ints(lengths))
+        out.fill_(77.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        p.pages.check()
+        x.attend(None, lengths, torch.float32, out=out, run=False)
+    for wrong in (-1, 5001, 2 ** 31 - 1):
+        told = [20] * 40
+        told[3], told[4] = wrong, 5000
+        x.lengths.copy_(ints(told))
+        graph.replay()
+        with pytest.raises(npu.NpuError):
+            p.pages.check()
+        told[3] = 0
+        x.attend(None, told, torch.float32, out=out, run=False)
+
+
+def test_one_more_short_sequence_does_not_hold_up_a_long_one(ctx):
+    """A long sequence is split among 300 others as among 100, where the blocks that
+    splits aim at are between (9 times the call's time where it was not)."""
+    times = []
+    for sequences in (100, 300):
+        p = Pool(ctx, 8, 8, 64, 1, page=256, most=65536, seed=1)
+        p.fill([65536])
+        lengths = [20] * sequences
+        lengths[50] = 65536
+        b = D.PagedBatch(dev(p.table).expand(sequences, -1).contiguous(), ints(lengths))
+        q = dev(p.rows(sequences, 8))
+        out = torch.empty_like(q)
+        best = 1e9
+        for _ in range(8):
+            t = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+            t[0].record()
+            for _ in range(5):
+                D.attention_paged(ctx, p.pages, b, q, out)
+            t[1].record()
+            torch.cuda.synchronize()
+            best = min(best, t[0].elapsed_time(t[1]))
+        times.append(best)
+    assert times[1] < 4 * times[0]
+
+
 @pytest.mark.parametrize("d,qh,kh,sequences,rows,tokens", [
     (64, 32, 32, 40, 1, 9000), (128, 64, 32, 40, 3, 9000), (64, 32, 8, 33, 16, 9000), (256, 16, 8, 17, 20, 5000)])
 def test_long_lengths_in_one_block(ctx, d, qh, kh, sequences, rows, tokens):

@@ -34,10 +34,12 @@
  * may come out as NaN). A weight goes into the products with V as two fp16 (22
  * bits), or as one (11 bits) where the output is fp16 and a sequence may have more
  * than 32 query rows per KV head (max_rows x query heads / KV heads; more than 16 of
- * head_dim 256). Where fp16 has fewer bits it is off by up to 2^-30 of the row's
- * largest weight. A causal row sees the tokens up to its own, a row without a mask
- * all lengths[s]. A row that sees no token is 0. Infinities and NaN in K or V count
- * for the rows that see their token and for no other.
+ * head_dim 256); f32 output always takes two. Where fp16 has fewer bits a weight is
+ * off by up to 2^-30 of the row's largest. A causal row sees the tokens up to its own,
+ * a row without a mask all lengths[s]. A row that sees no token is 0. Infinities and
+ * NaN in K or V count for the rows that see their token and for no other; those in V
+ * however small the token's weight (calls whose rows see some take up to 70 times as
+ * long). Means of finite values are finite.
  *
  * What the device finds wrong. A length below 0 or above max_tokens, row_offsets
  * that fall or pass `rows` or give a sequence more than max_rows, and a page

@@ -115,8 +115,8 @@ constexpr int PAGED_APPEND_UNITS = 2;  // 16-value units of a thread
 //
 // Measured: one row each of 64 sequences, 32 + 16 heads of 128, 5.0 us: launch, three
 // memory round trips, sine and cosine, a store (6.0 with the loads last). 3677 f32 rows
-// 38: 3.6 TB/s read and written, two rounds of blocks; 15.6 where the rows are still in
-// the last-level cache.
+// 36: 3.7 TB/s read and written, two rounds of blocks; 14 where the rows are still in the
+// last-level cache.
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedRowsParams P) {
     __shared__ float2 turn[128];
     __shared__ int found;
@@ -325,20 +325,22 @@ static bool paged_same_geometry(const AttnWork* w, const PagedPool* c) {
 // tokens 25 and 29; 8192 rows 720 and 709, 4 x 512 after 8000 327 and 308, 2 x 4096 of 64
 // dims 118 and 113.
 //
-// Splits, in blocks a CU. Rows kernel: one where there are few sequences, as a block's rows
-// leave partials (2 sequences of 131072 tokens 196 with one, 198 with two, 201 with four;
-// one of 4000 14 with each), four where there are more, whose pieces are then of like
-// length (64 of up to 8100 tokens 194 unsplit, 181 with four, 179 with six; 16 of 256 dims
-// 66, 64 and 64; 12 x 5 rows 64 with one, 62 with four). A split holds a unit a wave at
-// least: one sequence of 4000 tokens 12.7 and 13.3 with two, 16 with four. Tile kernel: as many as stay on a CU; 8 units at least:
+// Splits, in blocks a CU. Rows kernel: one for few sequences, as a block's rows leave
+// partials, four for more than 4, whose pieces are then of like length. With one and with
+// four, 32 heads over 8 of 128, contexts not in the last-level cache: sequences of 16000
+// tokens, 1 20 and 23, 2 30 and 32, 3 49 and 43, 4 52 and 55, 5 74 and 62, 6 85 and 73, 8 91
+// and 94, 12 160 and 142, 24 245 and 247; of 1000 to 16000, 4 36 and 35, 5 44 and 39, 8 63 and
+// 58, 24 168 and 144. Of 16 over 2 of 256 four win from 12 on (96 and 80; ragged 57 and 52),
+// 5 37 and 47, 8 53 and 59. A split holds a unit a wave at least: one sequence of 4000 tokens
+// 12.7 and 13.3 with two, 16 with four. Tile kernel: as many as stay on a CU; 8 units at least:
 // 128 rows of 256 dims after 3600 tokens 35, with 16 units 44, with 24 50.
 //
 // Rows kernel, more sequences than blocks to aim at (128 of 8 KV heads): where one may be
 // longer than 4096 tokens, further splits of long ones follow the sequences' own blocks, as
 // many as are aimed at, of 32 units at least (256 sequences of 300 to 700 tokens and one of
 // 131072 188 and unsplit 1450, of 8192 101 and 146, of 4096 99 and 103; none longer, but
-// allowed, 88 and 85; 200 of up to 8100 557 and 580; 1000 of 16 heads over 8 of 64 with a long one 250 and 965,
-// without 190 and 170).
+// allowed, 90 and 88; 200 of up to 8100 557 and 580; 1000 of 16 heads over 8 of 64 with a
+// long one 250 and 965, without 190 and 170).
 static PagedPlan paged_plan(AttnPagedParams& P, int D) {
     const PagedBatch& B = P.b;
     const int G = P.qh / B.kh, cus = device_cus();

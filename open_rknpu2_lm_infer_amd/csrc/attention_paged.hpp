@@ -424,10 +424,10 @@ constexpr float PG_LAZY = 4.0f, PG_SHIFT = 10.0f;
 //
 // Measured with the join, contexts not in the last-level cache: one row of 32 heads over 8
 // of 128 and 64 sequences of 60 to 8100 tokens (1.08 GB) 182 us, 5.9 TB/s; 2 of 131072 162,
-// 6.6 (a large copy reads and writes 5.1); cached loads 202 and 214. 256 sequences of up to
-// 700 tokens of 8 heads of 64 33 (42). 16 sequences of 2 heads of 256 57: 4.6 TB/s, 216
-// registers leave two blocks a CU. One of 4000 tokens 12.3, latency: launch, table, one
-// unit's loads and products, the waves' meeting (7.6), the join (4.7). The next unit's
+// 6.6 (large reads alone reach 6.7, a copy reads and writes 5.1); cached loads 202 and 214.
+// 256 sequences of up to 700 tokens of 8 heads of 64 33 (42). 16 sequences of 2 heads of 256
+// 57: 4.6 TB/s, 220 registers leave two blocks a CU. One of 4000 tokens 12.4, latency: launch,
+// table, one unit's loads and products, the waves' meeting (8.0), the join (4.4). The next unit's
 // loads before this one's products changed nothing with 128 dims and lost with 256 (51 to
 // 57: registers).
 template <int D, int NW, int RW, bool PACK, bool BEHIND>
@@ -744,18 +744,21 @@ __global__ __launch_bounds__(64 * NW) void attn_paged_rows_kernel(AttnPagedParam
 // vector instructions do not depend on each other. In stage t K of stage t + 2 and V of
 // stage t + U - 1 go to LDS, loaded in the stage before.
 //
-// f32 output takes V's products twice (SPLIT). W: 32 rows a wave halve the LDS reads of a
-// product; of 256 dims they need 448 registers, one wave a SIMD (57600 keys, 1024 rows of
-// 2 heads 239 us, with 16 rows 202; 4-wave blocks of 64 rows 267).
+// f32 output takes V's products twice, with 22 bits of a weight (SPLIT). fp16 output, which
+// rounds by 2^-11 itself, takes them once: outputs are 2.9e-4 off instead of 2.0e-4 (twice
+// cost 850 us for 631 in the first case below, 72 for 61 in the second, 512 rows of 8 heads
+// of 64 after 8000 tokens 81 for 65; who wants more has f32 output). W: 32 rows a wave halve
+// the LDS reads of a product; of 256 dims they need 448 registers, one wave a SIMD (57600
+// keys, 1024 rows of 2 heads 239 us, with 16 rows 202; 4-wave blocks of 64 rows 267).
 //
 // Measured with the join: 512 rows of 32 heads over 8 of 128 after 65000 tokens 556 us, 0.98
-// PFLOP/s of a large matrix product's 1.17; matrix cores 54 % busy, LDS 34 %, at 1.7 to 1.8
+// PFLOP/s of a large matrix product's 1.17; matrix cores 55 % busy, LDS 35 %, at 1.7 to 1.8
 // GHz: the power limit holds the clock. LDS reads without turned places 28 % longer. 6
-// prompts of 17 to 1365 rows 54 us: a long prompt's last block walks 43 units alone
-// or beside one other. 100 to 200 rows of 16 heads over 2 of 256, f32 output, 72: matrix
-// cores 43 % busy (51 % and 1.5 GHz over longer contexts), two fp16 for a weight, the join 10. Matrix
-// and vector instructions or LDS reads put in turns by scheduling groups: no difference
-// of 128 dims or 256.
+// prompts of 17 to 1365 rows 55 us: a long prompt's last block walks 43 units alone or beside
+// one other (1.9 waves a SIMD of a busy CU). 100 to 200 rows of 16 heads over 2 of 256, f32
+// output, 72: matrix cores 43 % busy (51 % and 1.5 GHz over longer contexts), two fp16 for a
+// weight, the join 10. Matrix and vector instructions or LDS reads put in turns by scheduling
+// groups: no difference of 128 dims or 256.
 template <int D, int W, int U, int NW, bool SPLIT>
 __global__ __launch_bounds__(64 * NW) void attn_paged_tile_kernel(AttnPagedParams P) {
     constexpr int CL = W * W / 64;                 // values of a lane in a C operand

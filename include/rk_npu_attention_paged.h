@@ -115,7 +115,9 @@ void rk_npu_hip_attention_paged_pool_free(rk_npu_hip_attention_paged_pool* pool)
 /* Waits for the device calls made with the pool (for calls on several streams, and
  * always once a call has been captured, for the whole device: graphs may be launched
  * at any time) and tells whether one since the last status found something wrong in
- * its batch: RK_NPU_ERR_PARAM, or RK_NPU_OK. Not while a stream is being captured. */
+ * its batch: RK_NPU_ERR_PARAM, or RK_NPU_OK. What a call that another thread makes
+ * meanwhile finds wrong is told by this status or the next. Not while a stream is
+ * being captured. */
 int rk_npu_hip_attention_paged_status(rk_npu_hip_attention_paged_pool* pool);
 
 /* ---- on the caller's stream (NULL: the null stream) ---------------------------
